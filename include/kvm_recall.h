@@ -737,6 +737,165 @@ int kvm_prefill_attention(kvm_ctx* ctx, const kvm_prefill_desc* desc, const void
                           uint64_t q_head_stride, const kvm_kcache* k, const kvm_kcache* v, void* out,
                           uint64_t out_row_stride, uint64_t out_head_stride, float* page_lse, void* stream);
 
+/* ------------------------------------------------------- decode attention */
+
+/* The attention that reads the cache which the recall path fills. Both entry
+ * points take fp16 or bf16 queries and write out in the queries' type; sums and
+ * softmax statistics are 32-bit. They have no counterpart in the reference,
+ * whose engine attends with its own kernels. Common rules:
+ *  - head_dim 64, 128 or 256; q_heads a multiple of kv_heads (query head h reads
+ *    KV head h / (q_heads / kv_heads)); scale 0 selects 1/sqrt(head_dim).
+ *  - Base pointers and strides of q, out and 16-bit K / V are multiples of 16
+ *    bytes, else KVM_ERR_UNSUPPORTED. out overlaps none of the inputs.
+ *  - A row that sees no key gives out = 0 and lse = -inf. Keys that a row does
+ *    not see do not reach it, whatever bytes they hold (infinities and NaN too).
+ *  - lse (optional, may be NULL): device f32 [sequence][row][q_heads], the natural
+ *    log of the row's sum of exp(scale * <q, K>); rows of two calls over different
+ *    keys are joined by it.
+ *  - Arrays marked "device" may be rewritten between replays of a captured call:
+ *    grids depend on host values only. Values out of range in them are reported
+ *    by kvm_ctx_status: the affected sequence's rows are left as they were
+ *    (KVM_ERR_LENGTH), or the page is left out (below).
+ *  - Rows at or past seq_rows[i] are left as they were.
+ *  - Split key ranges are joined in device scratch of the context: calls on one
+ *    context are ordered by their stream, and calls that may overlap (two streams,
+ *    two graphs replayed at once) take two contexts. Scratch grows on the first
+ *    call of a size and is kept until the context is destroyed, so a captured
+ *    call stays valid; growing it inside a capture is KVM_ERR_LENGTH (make the
+ *    call once before). With a bound workspace (kvm_ctx_bind_workspace) that is
+ *    used instead, with as many chunks as it has room for.
+ * Asynchronous on `stream`. */
+
+/* Sliding window with sinks over a dense cache: row i of sequence b stands at
+ * position p = base_b + i and sees the keys t <= p with t < sinks or p - t <
+ * window (window 1: itself; window 0: sinks only). K and V of the rows are in the
+ * cache already (capacity_tokens >= base_b + rows).
+ * q / out: element (b, i, h, d) at data + b*seq_stride + i*row_stride +
+ * h*head_stride + 2*d. k, v: kvm_kcache views of the desc's type whose
+ * layer_stride is the stride between sequences. width = 1 is the form for
+ * single tokens. */
+typedef struct kvm_window_desc {
+    uint32_t q_heads, kv_heads, head_dim;
+    int32_t type;              /* KVM_F16 or KVM_BF16: q, k, v, out */
+    uint32_t seqs, width;      /* sequences; rows per sequence (padded) */
+    uint32_t window, sinks;
+    uint64_t base;             /* position of row 0, when seq_base is NULL */
+    const uint64_t* seq_base;  /* device [seqs] or NULL */
+    const uint32_t* seq_rows;  /* device [seqs]: rows used (<= width), or NULL: width */
+    float scale;
+    uint32_t reserved;
+} kvm_window_desc;
+typedef struct kvm_rows {      /* a [sequence][row][head][head_dim] tensor, byte strides */
+    void* data;
+    uint64_t seq_stride, row_stride, head_stride;
+} kvm_rows;
+int kvm_window_attention(kvm_ctx* ctx, const kvm_window_desc* desc, const kvm_rows* q, const kvm_kcache* k,
+                         const kvm_kcache* v, const kvm_rows* out, float* lse, void* stream);
+
+/* A tree of drafted tokens over the pages of a residency pool: sequence i reads
+ * pool row row0 + i*row_step, its listed pages where kvm_plan_residency put them,
+ * then its tail: `recent` committed tokens that are in no page yet, then its
+ * drafted nodes. Node n sees every token t < tokens of the listed pages (page p
+ * holds tokens p*page_tokens ..), every recent token, and the nodes j whose bit j
+ * is set in its words of `tree` (bit j%32 of word j/32; without a tree, j <= n).
+ * nodes = 1 is plain decode attention over the recalled pages.
+ *  - Pages: sel_ids / sel_n are device lists as kvm_select_topk writes them (one
+ *    row of sel_stride per sequence; a page listed twice counts twice); NULL
+ *    reads every resident page of the row. A listed page that is not resident is
+ *    left out and reported as KVM_ERR_STALE, an id past the pool's pages (or a
+ *    count past sel_stride) as KVM_ERR_INVALID_ARGUMENT.
+ *  - layout: dev_base / dev_row_stride / dev_slot_stride of planes 0 (K) and 1 (V)
+ *    as for kvm_stagein_pool (host fields unused). A page is token-major,
+ *    [page_tokens][kv_heads] rows of its type; k_type / v_type: both the desc's
+ *    type, or both of KVM_Q8_0 and KVM_Q4_0. Per-KV-head selections (pool rows =
+ *    (layer, KV head)) are calls with kv_heads = 1 and one sequence per head.
+ *  - tail_k / tail_v: kvm_kcache views of the desc's type, layer_stride between
+ *    sequences, capacity_tokens >= recent + nodes.
+ *  - Block scales of quantised V above 1023 with fp16 queries are reported as
+ *    KVM_ERR_NONFINITE (their products would leave the range of fp16).
+ * kvm_plan_residency, the stage-in and this call are ordered by the stream;
+ * KVM_ERR_PENDING while a transfer is pending on the pool. */
+typedef struct kvm_tree_desc {
+    uint32_t q_heads, kv_heads, head_dim;
+    int32_t type;                 /* KVM_F16 or KVM_BF16: q, tail, out */
+    int32_t k_type, v_type;       /* the pages' planes */
+    uint32_t seqs, nodes;         /* sequences; drafted nodes per sequence (padded) */
+    uint32_t row0, row_step;
+    uint32_t page_tokens;
+    uint32_t recent;              /* when seq_recent is NULL */
+    uint64_t tokens;              /* history length, when seq_tokens is NULL */
+    const uint64_t* seq_tokens;   /* device [seqs] or NULL */
+    const uint32_t* seq_recent;   /* device [seqs] or NULL */
+    const uint32_t* seq_rows;     /* device [seqs]: nodes used (<= nodes), or NULL: nodes */
+    const uint32_t* sel_ids;      /* device [seqs][sel_stride] or NULL: every resident page */
+    const uint32_t* sel_n;        /* device [seqs] (with sel_ids) */
+    uint32_t sel_stride;
+    uint32_t tree_words;          /* words per node, >= ceil(nodes / 32) */
+    const uint32_t* tree;         /* device [seqs][nodes][tree_words] or NULL: a chain */
+    uint64_t tree_stride;         /* words between sequences' trees; 0: one tree for all */
+    float scale;
+    uint32_t reserved;
+} kvm_tree_desc;
+int kvm_tree_attention(kvm_ctx* ctx, const kvm_pool* pool, const kvm_tree_desc* desc, const kvm_stage_layout* layout,
+                       const kvm_rows* q, const kvm_kcache* tail_k, const kvm_kcache* tail_v, const kvm_rows* out,
+                       float* lse, void* stream);
+
+/* The `tree` words of a tree given by parents (host code): node i sees itself and
+ * what parents[i] sees (-1: a root). parents[i] < i, else KVM_ERR_INVALID_ARGUMENT.
+ * words: host u32 [nodes][tree_words]. */
+int kvm_tree_mask(const int32_t* parents, uint32_t nodes, uint32_t tree_words, uint32_t* words);
+
+/* ----------------------------------------------------------- pages of a pool */
+
+/* Pages copied, shared by copy, dropped and moved between the slots of a pool on
+ * the device, beside kvm_plan_residency and the stage-in (no counterpart in the
+ * reference, whose store keeps one working set per session). Rows are pool rows,
+ * given as host arrays; `layout` as for kvm_stagein_pool with the host fields
+ * unused (1 or 2 planes); `ctas` bounds the copy's CTAs (0 = all SMs). Every call
+ * drops the restore lists of the rows that it changes: stage planned pages in
+ * first. The tables change with the bytes, in stream order; nothing synchronises.
+ * KVM_ERR_PENDING while a transfer is pending on the pool.
+ *
+ * kvm_pool_fork: row dst_rows[i] becomes a copy of row src_rows[i]: every page
+ * below page_end that is resident there, in the same slot; what dst held before is
+ * dropped. A source may be forked into many rows (it is read once); a row that is
+ * a destination twice, or a source and a destination, is KVM_ERR_INVALID_ARGUMENT. */
+int kvm_pool_fork(kvm_ctx* ctx, kvm_pool* pool, const kvm_stage_layout* layout, const uint32_t* src_rows,
+                  const uint32_t* dst_rows, uint32_t n, uint32_t page_end, uint32_t ctas, void* stream);
+
+/* kvm_pool_copy: page src_page of src_row is copied to page dst_page of dst_row,
+ * into the slot that page has there, else into the row's lowest free slots in the
+ * order of the items (its pages take part in the selection rules from then on).
+ * Items whose source is not resident are left out and reported as KVM_ERR_STALE,
+ * those that find no free slot as KVM_ERR_BUDGET_EXCEEDED (kvm_ctx_status). A
+ * destination named twice, or one that is also a source, is
+ * KVM_ERR_INVALID_ARGUMENT. */
+typedef struct kvm_page_copy {
+    uint32_t src_row, src_page, dst_row, dst_page;
+} kvm_page_copy;
+int kvm_pool_copy(kvm_ctx* ctx, kvm_pool* pool, const kvm_stage_layout* layout, const kvm_page_copy* items, uint32_t n,
+                  uint32_t ctas, void* stream);
+
+/* kvm_pool_free: drops the listed pages of rows[i] (device lists ids
+ * [n][stride], counts[n], as kvm_select_topk writes them); their slots are free.
+ * Pages that are not resident and repeated pages are no error; an id past the
+ * pool's pages, or a count past stride, is left out and reported as
+ * KVM_ERR_INVALID_ARGUMENT. A row given twice is KVM_ERR_INVALID_ARGUMENT. */
+int kvm_pool_free(kvm_ctx* ctx, kvm_pool* pool, const uint32_t* rows, uint32_t n, const uint32_t* ids,
+                  const uint32_t* counts, uint32_t stride, void* stream);
+
+/* kvm_pool_compact: the c resident pages of each given row are brought into slots
+ * 0 .. c-1 with the fewest moves: the k-th resident slot >= c goes to the k-th
+ * free slot < c (both ascending). used: device u32 [n] = c, or NULL. A row given
+ * twice is KVM_ERR_INVALID_ARGUMENT. */
+int kvm_pool_compact(kvm_ctx* ctx, kvm_pool* pool, const kvm_stage_layout* layout, const uint32_t* rows, uint32_t n,
+                     uint32_t* used, uint32_t ctas, void* stream);
+
+/* The pool's device tables, for the caller's own kernels to read: slot_of
+ * [rows][pages] (-1 = not resident), page_of [rows][slots] (-1 = free). Valid
+ * until the pool is destroyed. */
+int kvm_pool_tables(const kvm_pool* pool, const int32_t** slot_of, const int32_t** page_of);
+
 /* Bytes of one D-element row of `type` (0 for an unknown type). */
 uint64_t kvm_row_bytes(int type, uint32_t dim);
 

@@ -121,6 +121,33 @@ class PrefillDesc(C.Structure):
 
 PREFILL_MAX_SAMPLES = 4096
 
+
+class Rows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("seq_stride", C.c_uint64), ("row_stride", C.c_uint64),
+                ("head_stride", C.c_uint64)]
+
+
+class WindowDesc(C.Structure):
+    _fields_ = [("q_heads", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("type", C.c_int32),
+                ("seqs", C.c_uint32), ("width", C.c_uint32), ("window", C.c_uint32), ("sinks", C.c_uint32),
+                ("base", C.c_uint64), ("seq_base", C.c_void_p), ("seq_rows", C.c_void_p), ("scale", C.c_float),
+                ("reserved", C.c_uint32)]
+
+
+class TreeDesc(C.Structure):
+    _fields_ = [("q_heads", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("type", C.c_int32),
+                ("k_type", C.c_int32), ("v_type", C.c_int32), ("seqs", C.c_uint32), ("nodes", C.c_uint32),
+                ("row0", C.c_uint32), ("row_step", C.c_uint32), ("page_tokens", C.c_uint32), ("recent", C.c_uint32),
+                ("tokens", C.c_uint64), ("seq_tokens", C.c_void_p), ("seq_recent", C.c_void_p),
+                ("seq_rows", C.c_void_p), ("sel_ids", C.c_void_p), ("sel_n", C.c_void_p), ("sel_stride", C.c_uint32),
+                ("tree_words", C.c_uint32), ("tree", C.c_void_p), ("tree_stride", C.c_uint64), ("scale", C.c_float),
+                ("reserved", C.c_uint32)]
+
+
+class PageCopy(C.Structure):
+    _fields_ = [("src_row", C.c_uint32), ("src_page", C.c_uint32), ("dst_row", C.c_uint32), ("dst_page", C.c_uint32)]
+
+
 SIGNATURES = {
     "kvm_ctx_create": ([_i, C.POINTER(C.c_void_p)], _i),
     "kvm_ctx_destroy": ([_vp], _i),
@@ -190,6 +217,16 @@ SIGNATURES = {
     "kvm_ipc_close": ([_i, _vp], _i),
     "kvm_prefill_attention": ([_vp, C.POINTER(PrefillDesc), _vp, _u64, _u64, C.POINTER(KCache), C.POINTER(KCache),
                                _vp, _u64, _u64, _vp, _vp], _i),
+    "kvm_window_attention": ([_vp, C.POINTER(WindowDesc), C.POINTER(Rows), C.POINTER(KCache), C.POINTER(KCache),
+                              C.POINTER(Rows), _vp, _vp], _i),
+    "kvm_tree_attention": ([_vp, _vp, C.POINTER(TreeDesc), C.POINTER(StageLayout), C.POINTER(Rows), C.POINTER(KCache),
+                            C.POINTER(KCache), C.POINTER(Rows), _vp, _vp], _i),
+    "kvm_tree_mask": ([_vp, _u32, _u32, _vp], _i),
+    "kvm_pool_fork": ([_vp, _vp, C.POINTER(StageLayout), _vp, _vp, _u32, _u32, _u32, _vp], _i),
+    "kvm_pool_copy": ([_vp, _vp, C.POINTER(StageLayout), _vp, _u32, _u32, _vp], _i),
+    "kvm_pool_free": ([_vp, _vp, _vp, _u32, _vp, _vp, _u32, _vp], _i),
+    "kvm_pool_compact": ([_vp, _vp, C.POINTER(StageLayout), _vp, _u32, _vp, _u32, _vp], _i),
+    "kvm_pool_tables": ([_vp, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p)], _i),
     "kvm_row_bytes": ([_i, _u32], _u64),
     "kvm_ctx_launches": ([_vp], _u64),
 }

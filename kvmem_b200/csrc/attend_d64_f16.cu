@@ -1,0 +1,5 @@
+#include "attend_launch.cuh"
+
+namespace kvmb {
+template int launch_attend_t<64, false>(kvm_ctx*, const AttendParams&, int, bool, int, cudaStream_t);
+}  // namespace kvmb

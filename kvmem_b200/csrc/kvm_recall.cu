@@ -9,12 +9,14 @@
 #include <unordered_map>
 #include <vector>
 
+#include "attend_launch.cuh"
 #include "common.cuh"
 #include "layerwise.cuh"
 #include "lse_launch.cuh"
 #include "page_mass_tc.cuh"
 #include "meank.cuh"
 #include "page_norm.cuh"
+#include "pool_pages.cuh"
 #include "post.cuh"
 #include "prefill_attn.cuh"
 #include "restore.cuh"
@@ -31,6 +33,8 @@ struct kvm_pool {
     kvm_ctx* ctx = nullptr;
     PoolView view{};
     void* mem = nullptr;
+    int2* moves = nullptr;        // move lists of the page operations: max(rows * slots, kPcGroups)
+    uint32_t* n_moves = nullptr;  // max(rows, kPcGroups)
     kvm_transfer* pending = nullptr;  // the prepared, not yet published or aborted transfer
 };
 
@@ -832,6 +836,8 @@ int kvm_ctx_destroy(kvm_ctx* c) {
     if (c->small) cudaFree(c->small);
     if (c->aux) cudaFree(c->aux);
     if (c->aux_done) cudaEventDestroy(c->aux_done);
+    if (c->attn_ws) cudaFree(c->attn_ws);
+    for (void* w : c->attn_retired) cudaFree(w);
     for (auto& L : c->copy_lists) {
         if (L.done) cudaEventDestroy(L.done);
         if (L.host) cudaFreeHost(L.host);
@@ -882,7 +888,7 @@ int kvm_ctx_bind_workspace(kvm_ctx* c, void* ws, size_t bytes) {
 }
 
 size_t kvm_ctx_device_bytes(const kvm_ctx* c) {
-    return c ? (c->ws_borrowed ? 0 : c->ws_bytes) + c->small_bytes : 0;
+    return c ? (c->ws_borrowed ? 0 : c->ws_bytes) + c->small_bytes + c->attn_ws_bytes + c->attn_retired_bytes : 0;
 }
 
 int kvm_score_pages(kvm_ctx* c, const kvm_score_desc* d, const kvm_query* q, const kvm_kcache* k, float* mass_rows,
@@ -1058,7 +1064,9 @@ int kvm_pool_create(kvm_ctx* c, uint32_t rows, uint32_t pages, uint32_t slots, k
     p->ctx = c;
     const size_t a = align256(size_t(rows) * pages * 4), b = align256(size_t(rows) * slots * 4),
                  n = align256(size_t(rows) * 4);
-    if (cudaMalloc(&p->mem, a + 3 * b + n) != cudaSuccess) {
+    const size_t mv = align256(std::max<size_t>(size_t(rows) * slots, kPcGroups) * 8),
+                 nm = align256(std::max<size_t>(rows, kPcGroups) * 4);
+    if (cudaMalloc(&p->mem, a + 3 * b + n + mv + nm) != cudaSuccess) {
         cudaGetLastError();
         delete p;
         return KVM_ERR_CUDA;
@@ -1069,6 +1077,8 @@ int kvm_pool_create(kvm_ctx* c, uint32_t rows, uint32_t pages, uint32_t slots, k
     p->view.restore = reinterpret_cast<uint32_t*>(base + a + b);
     p->view.restore_slot = reinterpret_cast<uint32_t*>(base + a + 2 * b);
     p->view.n_restore = reinterpret_cast<uint32_t*>(base + a + 3 * b);
+    p->moves = reinterpret_cast<int2*>(base + a + 3 * b + n);
+    p->n_moves = reinterpret_cast<uint32_t*>(base + a + 3 * b + n + mv);
     p->view.rows = rows;
     p->view.pages = pages;
     p->view.slots = slots;
@@ -2203,6 +2213,461 @@ int kvm_prefill_attention(kvm_ctx* c, const kvm_prefill_desc* d, const void* q, 
     }
     KVM_TRY(kvmb::launch_prefill(c, maps, p, d->head_dim, d->type == KVM_BF16, s));
     return table ? aux_release(c, s) : KVM_OK;
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------ decode attention
+
+namespace {
+
+bool al16(uint64_t x) { return (x & 15) == 0; }
+bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool aligned_to(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// Scratch of `bytes` for partial rows: the bound workspace, else the context's own,
+// which grows by keeping the old one (a captured call may still use it). Fails with
+// KVM_ERR_LENGTH when it would have to grow inside a capture.
+int ensure_attn_ws(kvm_ctx* c, size_t bytes, cudaStream_t s, void** out) {
+    if (c->ws_borrowed) {
+        *out = c->ws;
+        return bytes <= c->ws_bytes ? KVM_OK : KVM_ERR_LENGTH;
+    }
+    if (bytes > c->attn_ws_bytes) {
+        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+        KVM_CUDA(cudaStreamIsCapturing(s, &st));
+        if (st != cudaStreamCaptureStatusNone) return KVM_ERR_LENGTH;
+        const size_t want = align256(std::max<size_t>({bytes, c->attn_ws_bytes * 2, size_t(8) << 20}));
+        try {
+            c->attn_retired.reserve(c->attn_retired.size() + 1);
+        } catch (const std::bad_alloc&) {
+            return KVM_ERR_LENGTH;
+        }
+        void* p = nullptr;
+        KVM_CUDA(cudaMalloc(&p, want));
+        if (c->attn_ws) {
+            c->attn_retired.push_back(c->attn_ws);
+            c->attn_retired_bytes += c->attn_ws_bytes;
+        }
+        c->attn_ws = p;
+        c->attn_ws_bytes = want;
+    }
+    *out = c->attn_ws;
+    return KVM_OK;
+}
+
+// Checks and fills what both attention calls share: heads, rows, q / out, the dense keys.
+int attend_common(const kvm_ctx* c, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, int32_t type, uint32_t seqs,
+                  uint32_t width, float scale, const kvm_rows* q, const kvm_kcache* k, const kvm_kcache* v,
+                  const kvm_rows* out, float* lse, AttendParams* p) {
+    if (!q->data || !out->data || !k->data || !v->data) return KVM_ERR_INVALID_ARGUMENT;
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256) return KVM_ERR_UNSUPPORTED;
+    if (type != KVM_F16 && type != KVM_BF16) return KVM_ERR_UNSUPPORTED;
+    if (k->type != type || v->type != type) return KVM_ERR_INVALID_ARGUMENT;
+    if (!q_heads || !kv_heads || q_heads % kv_heads) return KVM_ERR_INVALID_ARGUMENT;
+    if (!(scale >= 0.f) || !std::isfinite(scale)) return KVM_ERR_INVALID_ARGUMENT;
+    const uint64_t rb = uint64_t(head_dim) * 2;
+    if (!al16(q->data) || !al16(out->data) || !al16(k->data) || !al16(v->data) || !aligned_to(lse, 4))
+        return KVM_ERR_UNSUPPORTED;
+    for (uint64_t st : {q->seq_stride, q->row_stride, q->head_stride, out->seq_stride, out->row_stride, out->head_stride,
+                        k->layer_stride, k->token_stride, k->head_stride, v->layer_stride, v->token_stride,
+                        v->head_stride})
+        if (!al16(st)) return KVM_ERR_UNSUPPORTED;
+    // Strides of a single sequence, row or head are free; others may not overlap a row.
+    if ((q_heads > 1 && (q->head_stride < rb || out->head_stride < rb)) ||
+        (width > 1 && (q->row_stride < rb || out->row_stride < rb)) ||
+        (seqs > 1 && (q->seq_stride < rb || out->seq_stride < rb)) ||
+        (kv_heads > 1 && (k->head_stride < rb || v->head_stride < rb)) || k->token_stride < rb || v->token_stride < rb)
+        return KVM_ERR_INVALID_ARGUMENT;
+    const uint64_t cap = std::min(k->capacity_tokens, v->capacity_tokens);
+    if (uint64_t(width) * (q_heads / kv_heads) > 0x7fffffffull || uint64_t(seqs) * width > 0x7fffffffull)
+        return KVM_ERR_LENGTH;
+    p->q = static_cast<const uint8_t*>(q->data);
+    p->q_seq = q->seq_stride, p->q_row = q->row_stride, p->q_head = q->head_stride;
+    p->out = static_cast<uint8_t*>(out->data);
+    p->o_seq = out->seq_stride, p->o_row = out->row_stride, p->o_head = out->head_stride;
+    p->lse = lse;
+    p->seqs = seqs, p->width = width, p->q_heads = q_heads, p->kv_heads = kv_heads, p->group = q_heads / kv_heads;
+    p->scale_log2 = (scale > 0.f ? scale : 1.f / std::sqrt(float(head_dim))) * 1.4426950408889634f;
+    p->k = static_cast<const uint8_t*>(k->data), p->v = static_cast<const uint8_t*>(v->data);
+    p->k_seq = k->layer_stride, p->k_tok = k->token_stride, p->k_head = k->head_stride;
+    p->v_seq = v->layer_stride, p->v_tok = v->token_stride, p->v_head = v->head_stride;
+    p->capacity = uint32_t(std::min<uint64_t>(cap, 0x7fffff00ull));
+    p->status = c->status;
+    return KVM_OK;
+}
+
+// Chooses the M tile and the key chunks, takes the scratch and launches. `tiles`:
+// key tiles of the longest unit.
+int attend_launch(kvm_ctx* c, AttendParams& p, uint32_t head_dim, bool bf16, int mode, bool quant, uint64_t tiles,
+                  cudaStream_t s) {
+    const uint32_t packed = p.width * p.group;
+    const int wm = packed <= 16 ? 1 : packed <= 32 ? 2 : 4;
+    p.m_tiles = (packed + 16 * wm - 1) / (16 * wm);
+    // Key chunks: the modelled time of `waves` waves of CTAs, each of its tiles' copies at
+    // the SM's share of HBM plus its start and end, and the joining of the chunks.
+    const uint32_t smem = at_smem_bytes(int(head_dim), wm, quant);
+    const uint32_t occ = std::max(1u, 227u * 1024u / (smem + 1024u));
+    const double tile_us = double(kAtKeys) * 4 * head_dim * c->num_sms * occ / 6.4e6;
+    const uint64_t units = uint64_t(p.seqs) * p.kv_heads * p.m_tiles;
+    const uint64_t rows = uint64_t(p.seqs) * p.width * p.q_heads;
+    const size_t row_bytes = size_t(head_dim) * 4 + 8;
+    const uint64_t slots = uint64_t(c->num_sms) * occ;
+    uint32_t splits = 1;
+    double best = 0;
+    for (uint32_t sp = 1; sp <= std::min<uint64_t>(tiles, 256); ++sp) {
+        if (sp > 1 && (units * (sp - 1) >= 4 * slots || rows * sp * row_bytes > (size_t(1) << 30))) break;
+        const uint64_t waves = (units * sp + slots - 1) / slots;
+        const double t = double(waves) * (double((tiles + sp - 1) / sp) * tile_us + 3.0) +
+                         (sp > 1 ? 3.0 + double(rows * sp * row_bytes) / 3e6 : 0.0);
+        if (sp == 1 || t < best) best = t, splits = sp;
+    }
+    if (const char* e = std::getenv("KVM_ATTEND_SPLITS")) {  // the tests reach the joining pass on small problems with it
+        const long v = std::strtol(e, nullptr, 10);
+        if (v >= 1 && v <= 256) splits = uint32_t(v);
+    }
+    if (c->ws_borrowed)
+        while (splits > 1 && rows * splits * row_bytes + 256 > c->ws_bytes) --splits;
+    p.splits = splits;
+    if (splits > 1) {
+        const size_t po = align256(rows * splits * head_dim * 4);
+        void* ws = nullptr;
+        KVM_TRY(ensure_attn_ws(c, po + rows * splits * 8, s, &ws));
+        p.part_o = static_cast<float*>(ws);
+        p.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(ws) + po);
+    }
+    switch (head_dim) {
+        case 64: return bf16 ? launch_attend_t<64, true>(c, p, mode, quant, wm, s) : launch_attend_t<64, false>(c, p, mode, quant, wm, s);
+        case 128: return bf16 ? launch_attend_t<128, true>(c, p, mode, quant, wm, s) : launch_attend_t<128, false>(c, p, mode, quant, wm, s);
+        default: return bf16 ? launch_attend_t<256, true>(c, p, mode, quant, wm, s) : launch_attend_t<256, false>(c, p, mode, quant, wm, s);
+    }
+}
+
+// Device side of a layout's planes (host fields unused).
+int device_layout(const kvm_stage_layout* L, GatherLayout* g) {
+    if (!L || L->planes < 1 || L->planes > 2) return KVM_ERR_INVALID_ARGUMENT;
+    g->planes = L->planes;
+    for (uint32_t j = 0; j < L->planes; ++j) {
+        if (!L->dev_base[j] || !L->bytes[j] || L->dev_slot_stride[j] < L->bytes[j]) return KVM_ERR_INVALID_ARGUMENT;
+        g->dev_base[j] = static_cast<uint8_t*>(L->dev_base[j]);
+        g->dev_row_stride[j] = L->dev_row_stride[j];
+        g->dev_slot_stride[j] = L->dev_slot_stride[j];
+        g->bytes[j] = L->bytes[j];
+    }
+    return KVM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int kvm_window_attention(kvm_ctx* c, const kvm_window_desc* d, const kvm_rows* q, const kvm_kcache* k,
+                         const kvm_kcache* v, const kvm_rows* out, float* lse, void* stream) {
+    if (!c || !d || !q || !k || !v || !out) return KVM_ERR_INVALID_ARGUMENT;
+    if (!d->seqs || !d->width) return KVM_OK;
+    AttendParams p{};
+    KVM_TRY(attend_common(c, d->q_heads, d->kv_heads, d->head_dim, d->type, d->seqs, d->width, d->scale, q, k, v, out, lse,
+                          &p));
+    if (!aligned_to(d->seq_base, 8) || !aligned_to(d->seq_rows, 4)) return KVM_ERR_INVALID_ARGUMENT;
+    if (!d->seq_base && (d->base > p.capacity || d->width > p.capacity - d->base)) {
+        if (!d->seq_rows) return KVM_ERR_LENGTH;
+        if (d->base > p.capacity) return KVM_ERR_LENGTH;
+    }
+    p.base = d->base;
+    p.seq_base = d->seq_base;
+    p.seq_rows = d->seq_rows;
+    p.window = d->window;
+    p.sinks = d->sinks;
+    // Keys of the longest M tile (at most 64 packed rows).
+    const uint64_t reach = std::min<uint64_t>(uint64_t(d->window) + 64, p.capacity);
+    const uint64_t tiles = (std::min<uint64_t>(d->sinks, p.capacity) + kAtKeys - 1) / kAtKeys + (reach + kAtKeys - 1) / kAtKeys;
+    const uint64_t most = (uint64_t(p.capacity) + kAtKeys - 1) / kAtKeys + 1;
+    DeviceGuard guard(c->device);
+    return attend_launch(c, p, d->head_dim, d->type == KVM_BF16, kAtWindow, false, std::min(tiles, most),
+                         static_cast<cudaStream_t>(stream));
+}
+
+int kvm_tree_attention(kvm_ctx* c, const kvm_pool* pool, const kvm_tree_desc* d, const kvm_stage_layout* layout,
+                       const kvm_rows* q, const kvm_kcache* tail_k, const kvm_kcache* tail_v, const kvm_rows* out,
+                       float* lse, void* stream) {
+    if (!c || !pool || pool->ctx != c || !d || !layout || !q || !tail_k || !tail_v || !out) return KVM_ERR_INVALID_ARGUMENT;
+    if (!d->seqs || !d->nodes) return KVM_OK;
+    if (pool->pending) return KVM_ERR_PENDING;
+    AttendParams p{};
+    KVM_TRY(attend_common(c, d->q_heads, d->kv_heads, d->head_dim, d->type, d->seqs, d->nodes, d->scale, q, tail_k, tail_v,
+                          out, lse, &p));
+    const bool quant = d->k_type != d->type || d->v_type != d->type;
+    if (quant && ((d->k_type != KVM_Q8_0 && d->k_type != KVM_Q4_0) || (d->v_type != KVM_Q8_0 && d->v_type != KVM_Q4_0)))
+        return KVM_ERR_UNSUPPORTED;
+    const auto& view = pool->view;
+    if (!d->page_tokens || uint64_t(d->row0) + uint64_t(d->seqs - 1) * d->row_step >= view.rows) return KVM_ERR_INVALID_ARGUMENT;
+    if (!aligned_to(d->seq_tokens, 8) || !aligned_to(d->seq_recent, 4) || !aligned_to(d->seq_rows, 4) ||
+        !aligned_to(d->sel_ids, 4) || !aligned_to(d->sel_n, 4) || !aligned_to(d->tree, 4))
+        return KVM_ERR_INVALID_ARGUMENT;
+    if (d->sel_ids && (!d->sel_n || !d->sel_stride)) return KVM_ERR_INVALID_ARGUMENT;
+    if (d->tree && (uint64_t(d->tree_words) * 32 < d->nodes ||
+                    (d->tree_stride && d->tree_stride < uint64_t(d->nodes) * d->tree_words)))
+        return KVM_ERR_INVALID_ARGUMENT;
+    const uint64_t list = d->sel_ids ? d->sel_stride : view.slots;
+    if (list * d->page_tokens > 0x7fffff00ull) return KVM_ERR_LENGTH;
+    if (!d->seq_recent && (d->recent > p.capacity || (!d->seq_rows && d->nodes > p.capacity - d->recent))) return KVM_ERR_LENGTH;
+    GatherLayout g{};
+    KVM_TRY(device_layout(layout, &g));
+    if (g.planes != 2) return KVM_ERR_INVALID_ARGUMENT;
+    const int32_t types[2] = {d->k_type, d->v_type};
+    uint32_t gran[2];
+    for (int j = 0; j < 2; ++j) {
+        const uint64_t rb = row_bytes_of(types[j], d->head_dim);
+        if (g.bytes[j] < rb * d->kv_heads * d->page_tokens) return KVM_ERR_INVALID_ARGUMENT;
+        const uint64_t all = reinterpret_cast<uintptr_t>(g.dev_base[j]) | g.dev_row_stride[j] | g.dev_slot_stride[j] | rb |
+                             (quant ? 0 : rb * d->kv_heads);
+        gran[j] = (all & 15) == 0 ? 16 : (all & 7) == 0 ? 8 : 4;
+        if (all & (quant ? 3 : 15)) return KVM_ERR_UNSUPPORTED;
+    }
+    p.pk = g.dev_base[0], p.pv = g.dev_base[1];
+    p.pk_row = g.dev_row_stride[0], p.pv_row = g.dev_row_stride[1];
+    p.pk_slot = g.dev_slot_stride[0], p.pv_slot = g.dev_slot_stride[1];
+    p.pk_type = d->k_type, p.pv_type = d->v_type;
+    p.pk_bytes = uint32_t(row_bytes_of(d->k_type, d->head_dim)), p.pv_bytes = uint32_t(row_bytes_of(d->v_type, d->head_dim));
+    p.pk_head = p.pk_bytes, p.pv_head = p.pv_bytes;
+    p.pk_tok = uint64_t(p.pk_bytes) * d->kv_heads, p.pv_tok = uint64_t(p.pv_bytes) * d->kv_heads;
+    p.pk_gran = gran[0], p.pv_gran = gran[1];
+    p.slot_of = view.slot_of, p.page_of = view.page_of;
+    p.pool_pages = view.pages, p.pool_slots = view.slots;
+    p.row0 = d->row0, p.row_step = d->row_step;
+    p.sel_ids = d->sel_ids, p.sel_n = d->sel_n, p.sel_stride = d->sel_stride;
+    p.page_tokens = d->page_tokens;
+    uint32_t lg = 0;
+    while ((1ull << lg) < d->page_tokens) ++lg;
+    p.pt_shift = 32 + lg;
+    p.pt_magic = ((1ull << p.pt_shift) + d->page_tokens - 1) / d->page_tokens;
+    p.tokens = d->tokens, p.seq_tokens = d->seq_tokens;
+    p.recent = d->recent, p.seq_recent = d->seq_recent;
+    p.seq_rows = d->seq_rows;
+    p.tree = d->tree, p.tree_seq = d->tree_stride, p.tree_words = d->tree_words;
+    const uint64_t dense = d->seq_recent ? std::min<uint64_t>(p.capacity, uint64_t(d->page_tokens) + d->nodes) : uint64_t(d->recent) + d->nodes;
+    const uint64_t tiles = (list * d->page_tokens + kAtKeys - 1) / kAtKeys + (dense + kAtKeys - 1) / kAtKeys;
+    DeviceGuard guard(c->device);
+    return attend_launch(c, p, d->head_dim, d->type == KVM_BF16, kAtTree, quant, tiles, static_cast<cudaStream_t>(stream));
+}
+
+int kvm_tree_mask(const int32_t* parents, uint32_t nodes, uint32_t tree_words, uint32_t* words) {
+    if (!nodes) return KVM_OK;
+    if (!parents || !words || uint64_t(tree_words) * 32 < nodes) return KVM_ERR_INVALID_ARGUMENT;
+    for (uint32_t i = 0; i < nodes; ++i)
+        if (parents[i] < -1 || (parents[i] >= 0 && uint32_t(parents[i]) >= i)) return KVM_ERR_INVALID_ARGUMENT;
+    for (uint32_t i = 0; i < nodes; ++i) {
+        uint32_t* w = words + size_t(i) * tree_words;
+        if (parents[i] >= 0) std::memcpy(w, words + size_t(parents[i]) * tree_words, size_t(tree_words) * 4);
+        else std::memset(w, 0, size_t(tree_words) * 4);
+        w[i / 32] |= 1u << (i % 32);
+    }
+    return KVM_OK;
+}
+
+}  // extern "C"
+
+// ----------------------------------------------------------- pages of a pool
+
+namespace {
+
+int pages_check(const kvm_ctx* c, const kvm_pool* pool) {
+    if (!c || !pool || pool->ctx != c) return KVM_ERR_INVALID_ARGUMENT;
+    return pool->pending ? KVM_ERR_PENDING : KVM_OK;
+}
+
+// Rows in range and each given once.
+int distinct_rows(const kvm_pool* pool, const uint32_t* rows, uint32_t n, std::vector<uint8_t>* seen) {
+    seen->assign(pool->view.rows, 0);
+    for (uint32_t i = 0; i < n; ++i) {
+        if (rows[i] >= pool->view.rows || (*seen)[rows[i]]) return KVM_ERR_INVALID_ARGUMENT;
+        (*seen)[rows[i]] = 1;
+    }
+    return KVM_OK;
+}
+
+int copy_pages(kvm_ctx* c, const kvm_pool* pool, const PageGroups& gr, const GatherLayout& g, uint32_t list_stride,
+               uint32_t ctas, cudaStream_t s) {
+    PageCopy pc{};
+    pc.lay = g;
+    pc.moves = pool->moves;
+    pc.n_moves = pool->n_moves;
+    pc.list_stride = list_stride;
+    pc.status = c->status;
+    pc.chunk = kPcChunk;
+    bool bulk = true;
+    for (uint32_t j = 0; j < g.planes; ++j) {
+        pc.chunks[j] = uint32_t((g.bytes[j] + kPcChunk - 1) / kPcChunk);
+        bulk = bulk && al16(g.dev_base[j]) && al16(g.dev_row_stride[j]) && al16(g.dev_slot_stride[j]) && al16(g.bytes[j]);
+    }
+    // At most this many chunks: no more CTAs than that.
+    const uint64_t most = uint64_t(gr.n) * list_stride * (pc.chunks[0] + pc.chunks[1]);
+    if (bulk) {
+        KVM_CUDA(smem_attr(reinterpret_cast<const void*>(page_copy_kernel), int(kPcSmem)));
+        const uint32_t grid = uint32_t(std::min<uint64_t>(most, ctas ? ctas : uint32_t(c->num_sms)));
+        page_copy_kernel<<<grid, 32, kPcSmem, s>>>(gr, pc);
+    } else {
+        const uint32_t grid = uint32_t(std::min<uint64_t>(most, ctas ? ctas : uint32_t(c->num_sms) * 8));
+        page_copy_plain_kernel<<<grid, kPcPlainThreads, 0, s>>>(gr, pc);
+    }
+    ++c->launches;
+    KVM_CUDA(cudaGetLastError());
+    return KVM_OK;
+}
+
+int page_layout(const kvm_stage_layout* layout, GatherLayout* g) {
+    KVM_TRY(device_layout(layout, g));
+    for (uint32_t j = 0; j < g->planes; ++j)
+        if (g->bytes[j] > 0xffff0000ull) return KVM_ERR_LENGTH;
+    return KVM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int kvm_pool_fork(kvm_ctx* c, kvm_pool* pool, const kvm_stage_layout* layout, const uint32_t* src_rows,
+                  const uint32_t* dst_rows, uint32_t n, uint32_t page_end, uint32_t ctas, void* stream) try {
+    KVM_TRY(pages_check(c, pool));
+    GatherLayout g{};
+    KVM_TRY(page_layout(layout, &g));
+    if (!n) return KVM_OK;
+    if (!src_rows || !dst_rows) return KVM_ERR_INVALID_ARGUMENT;
+    std::vector<uint8_t> seen;
+    KVM_TRY(distinct_rows(pool, dst_rows, n, &seen));
+    std::vector<uint32_t> order(n);
+    for (uint32_t i = 0; i < n; ++i) {
+        if (src_rows[i] >= pool->view.rows || seen[src_rows[i]]) return KVM_ERR_INVALID_ARGUMENT;
+        order[i] = i;
+    }
+    std::stable_sort(order.begin(), order.end(), [&](uint32_t a, uint32_t b) { return src_rows[a] < src_rows[b]; });
+    DeviceGuard guard(c->device);
+    auto s = static_cast<cudaStream_t>(stream);
+    for (uint32_t at = 0; at < n; at += kPcGroups) {
+        PageGroups gr;
+        gr.n = 0;
+        gr.n_dst = std::min(n - at, kPcGroups);
+        for (uint32_t i = 0; i < gr.n_dst; ++i) {
+            const uint32_t o = order[at + i];
+            if (i == 0 || src_rows[o] != gr.src_row[gr.n - 1]) {
+                gr.src_row[gr.n] = src_rows[o];
+                gr.first[gr.n++] = i;
+            }
+            gr.dst_row[i] = dst_rows[o];
+        }
+        gr.first[gr.n] = gr.n_dst;
+        fork_plan_kernel<<<gr.n_dst, kPcPlanThreads, 0, s>>>(pool->view, gr, page_end, pool->moves, pool->n_moves);
+        ++c->launches;
+        KVM_CUDA(cudaGetLastError());
+        KVM_TRY(copy_pages(c, pool, gr, g, pool->view.slots, ctas, s));
+    }
+    return KVM_OK;
+} catch (const std::bad_alloc&) {
+    return KVM_ERR_LENGTH;
+}
+
+int kvm_pool_copy(kvm_ctx* c, kvm_pool* pool, const kvm_stage_layout* layout, const kvm_page_copy* items, uint32_t n,
+                  uint32_t ctas, void* stream) try {
+    KVM_TRY(pages_check(c, pool));
+    GatherLayout g{};
+    KVM_TRY(page_layout(layout, &g));
+    if (!n) return KVM_OK;
+    if (!items) return KVM_ERR_INVALID_ARGUMENT;
+    const auto& v = pool->view;
+    auto key = [](uint32_t row, uint32_t page) { return uint64_t(row) << 32 | page; };
+    std::vector<uint64_t> dst(n);
+    std::vector<uint32_t> order(n);
+    for (uint32_t i = 0; i < n; ++i) {
+        const auto& x = items[i];
+        if (x.src_row >= v.rows || x.dst_row >= v.rows || x.src_page >= v.pages || x.dst_page >= v.pages)
+            return KVM_ERR_INVALID_ARGUMENT;
+        dst[i] = key(x.dst_row, x.dst_page);
+        order[i] = i;
+    }
+    std::sort(dst.begin(), dst.end());
+    if (std::adjacent_find(dst.begin(), dst.end()) != dst.end()) return KVM_ERR_INVALID_ARGUMENT;
+    for (uint32_t i = 0; i < n; ++i)
+        if (std::binary_search(dst.begin(), dst.end(), key(items[i].src_row, items[i].src_page))) return KVM_ERR_INVALID_ARGUMENT;
+    std::stable_sort(order.begin(), order.end(), [&](uint32_t a, uint32_t b) { return items[a].dst_row < items[b].dst_row; });
+    DeviceGuard guard(c->device);
+    auto s = static_cast<cudaStream_t>(stream);
+    for (uint32_t at = 0; at < n; at += kPcGroups) {
+        PageItems it;
+        PageGroups gr;
+        it.n = gr.n = gr.n_dst = std::min(n - at, kPcGroups);
+        it.n_rows = 0;
+        for (uint32_t i = 0; i < it.n; ++i) {
+            const auto& x = items[order[at + i]];
+            if (i == 0 || x.dst_row != it.item[i - 1].dst_row) it.first[it.n_rows++] = i;
+            it.item[i] = x;
+            gr.src_row[i] = x.src_row;
+            gr.dst_row[i] = x.dst_row;
+            gr.first[i] = i;
+        }
+        it.first[it.n_rows] = gr.first[it.n] = it.n;
+        copy_plan_kernel<<<it.n_rows, kPcPlanThreads, 0, s>>>(v, it, pool->moves, pool->n_moves, c->status);
+        ++c->launches;
+        KVM_CUDA(cudaGetLastError());
+        KVM_TRY(copy_pages(c, pool, gr, g, 1, ctas, s));
+    }
+    return KVM_OK;
+} catch (const std::bad_alloc&) {
+    return KVM_ERR_LENGTH;
+}
+
+int kvm_pool_free(kvm_ctx* c, kvm_pool* pool, const uint32_t* rows, uint32_t n, const uint32_t* ids,
+                  const uint32_t* counts, uint32_t stride, void* stream) try {
+    KVM_TRY(pages_check(c, pool));
+    if (!n) return KVM_OK;
+    if (!rows || !ids || !counts || !stride || !aligned_to(ids, 4) || !aligned_to(counts, 4)) return KVM_ERR_INVALID_ARGUMENT;
+    std::vector<uint8_t> seen;
+    KVM_TRY(distinct_rows(pool, rows, n, &seen));
+    DeviceGuard guard(c->device);
+    for (uint32_t at = 0; at < n; at += kPcGroups) {
+        PageRows pr;
+        pr.n = std::min(n - at, kPcGroups);
+        std::copy(rows + at, rows + at + pr.n, pr.row);
+        free_kernel<<<pr.n, kPcPlanThreads, 0, static_cast<cudaStream_t>(stream)>>>(pool->view, pr, at, ids, counts, stride,
+                                                                                    c->status);
+        ++c->launches;
+        KVM_CUDA(cudaGetLastError());
+    }
+    return KVM_OK;
+} catch (const std::bad_alloc&) {
+    return KVM_ERR_LENGTH;
+}
+
+int kvm_pool_compact(kvm_ctx* c, kvm_pool* pool, const kvm_stage_layout* layout, const uint32_t* rows, uint32_t n,
+                     uint32_t* used, uint32_t ctas, void* stream) try {
+    KVM_TRY(pages_check(c, pool));
+    GatherLayout g{};
+    KVM_TRY(page_layout(layout, &g));
+    if (!n) return KVM_OK;
+    if (!rows || !aligned_to(used, 4)) return KVM_ERR_INVALID_ARGUMENT;
+    std::vector<uint8_t> seen;
+    KVM_TRY(distinct_rows(pool, rows, n, &seen));
+    DeviceGuard guard(c->device);
+    auto s = static_cast<cudaStream_t>(stream);
+    for (uint32_t at = 0; at < n; at += kPcGroups) {
+        PageGroups gr;
+        gr.n = gr.n_dst = std::min(n - at, kPcGroups);
+        for (uint32_t i = 0; i < gr.n; ++i) gr.src_row[i] = gr.dst_row[i] = rows[at + i], gr.first[i] = i;
+        gr.first[gr.n] = gr.n;
+        compact_plan_kernel<<<gr.n, kPcPlanThreads, 0, s>>>(pool->view, gr, pool->moves, pool->n_moves, used ? used + at : nullptr);
+        ++c->launches;
+        KVM_CUDA(cudaGetLastError());
+        KVM_TRY(copy_pages(c, pool, gr, g, pool->view.slots, ctas, s));
+    }
+    return KVM_OK;
+} catch (const std::bad_alloc&) {
+    return KVM_ERR_LENGTH;
+}
+
+int kvm_pool_tables(const kvm_pool* pool, const int32_t** slot_of, const int32_t** page_of) {
+    if (!pool) return KVM_ERR_INVALID_ARGUMENT;
+    if (slot_of) *slot_of = pool->view.slot_of;
+    if (page_of) *page_of = pool->view.page_of;
+    return KVM_OK;
 }
 
 }  // extern "C"

@@ -28,6 +28,12 @@ struct kvm_ctx {
     size_t aux_bytes = 0;
     cudaEvent_t aux_done = nullptr;  // recorded after the last kernel that read `aux`
     bool aux_pending = false;
+    // Scratch of the decode-attention calls (partial rows of split key ranges). A
+    // larger one replaces it, but the old ones are kept: captured calls hold them.
+    void* attn_ws = nullptr;
+    size_t attn_ws_bytes = 0;
+    std::vector<void*> attn_retired;
+    size_t attn_retired_bytes = 0;
     std::vector<uint32_t> keep_cached;
     bool keep_valid = false;
     uint64_t launches = 0;

@@ -31,6 +31,70 @@ def _stream_ptr(stream) -> int:
     return stream.cuda_stream
 
 
+def _stream_on(device: int, stream) -> "torch.cuda.Stream":
+    """The given stream, else the current stream of `device` (whichever device is current)."""
+    return stream if stream is not None else torch.cuda.current_stream(device)
+
+
+def _on_device(device: int, where: str, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and (t.device.type != "cuda" or t.device.index != device):
+            raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{where}: {name} is on {t.device}, the context on cuda:{device}")
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _u64_arg(x, device: int, n: int, where: str):
+    """(scalar, device pointer) of a per-sequence argument: an int, or an int64 tensor [n]."""
+    return _seq_arg(x, device, n, where, torch.int64)
+
+
+def _u32_arg(x, device: int, n: int, where: str):
+    """(scalar, device pointer) of a per-sequence argument: an int, or an int32 tensor [n]."""
+    return _seq_arg(x, device, n, where, torch.int32)
+
+
+def _seq_arg(x, device, n, where, dtype):
+    if isinstance(x, torch.Tensor):
+        _on_device(device, where, argument=x)
+        if x.dtype != dtype or x.dim() != 1 or x.shape[0] < n or not x.is_contiguous():
+            raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{where}: a per-sequence tensor is contiguous {dtype} [{n}]")
+        return 0, x.data_ptr()
+    if x < 0:
+        raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{where}: negative argument")
+    return int(x), None
+
+
+def _rows4(t: torch.Tensor, where: str) -> A.Rows:
+    """kvm_rows of a [sequence][row][head][dim] tensor (dim contiguous)."""
+    if t.stride(3) != 1 and t.shape[3] != 1:
+        raise A.KvmError(A.ERR_UNSUPPORTED, f"{where}: the last dimension must be contiguous")
+    es = t.element_size()
+    # The stride of a dimension of one element says nothing: it is taken as one row.
+    st = [(t.stride(i) if t.shape[i] > 1 else t.shape[3]) * es for i in range(3)]
+    return A.Rows(t.data_ptr(), *st)
+
+
+def _dense4(t: torch.Tensor, where: str) -> A.KCache:
+    """kvm_kcache of a [sequence][token][head][dim] tensor (dim contiguous)."""
+    r = _rows4(t, where)
+    kc = A.KCache()
+    kc.data, kc.type = r.data, _TORCH_QTYPE[t.dtype]
+    kc.layer_stride, kc.token_stride, kc.head_stride = r.seq_stride, r.row_stride, r.head_stride
+    kc.capacity_tokens = t.shape[1]
+    return kc
+
+
+class _DeviceTable:
+    """Device memory of the library as __cuda_array_interface__ (int32)."""
+
+    def __init__(self, ptr: int, shape: tuple, owner):
+        self.owner = owner
+        self.__cuda_array_interface__ = {"data": (ptr, False), "shape": shape, "typestr": "<i4", "version": 3}
+
+
 def row_bytes(ktype: int, dim: int) -> int:
     return int(A.load().kvm_row_bytes(ktype, dim))
 
@@ -183,6 +247,38 @@ class RecallContext:
                                             _stream_ptr(stream))
         A.check(rc, "kvm_prefill_attention")
         return out, (page_lse if rows else None)
+
+    def window_attention(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, base, window: int, sinks: int = 0,
+                         rows: Optional[torch.Tensor] = None, scale: float = 0.0, out: Optional[torch.Tensor] = None,
+                         lse: Optional[torch.Tensor] = None, want_lse: bool = False, stream=None):
+        """Attention with a sliding window and `sinks` first tokens that stay visible (kvm_window_attention).
+
+        q: [seqs][width][q_heads][head_dim] (or [width][q_heads][head_dim]) fp16 / bf16, row i at position
+        base + i; k, v: [seqs][capacity][kv_heads][head_dim] (or without seqs) views of the cache, any strides that
+        are multiples of 16 bytes. base: int, or int64 tensor [seqs] on the device; rows: int32 tensor [seqs], the
+        rows used per sequence (the others keep what `out` and `lse` hold).
+        Returns (out like q, lse [seqs][width][q_heads] f32 or None)."""
+        w = "kvm_window_attention"
+        flat = q.dim() == 3
+        if flat:
+            q, k, v = q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0)
+            out = None if out is None else out.unsqueeze(0)
+            lse = None if lse is None else lse.unsqueeze(0)
+        _on_device(self.device, w, q=q, k=k, v=v, out=out, lse=lse)
+        out, lse = _attention_out(w, q, k, v, out, lse, want_lse, _stream_on(self.device, stream))
+        B, W, Hq, D = q.shape
+        d = A.WindowDesc()
+        d.q_heads, d.kv_heads, d.head_dim, d.type = Hq, k.shape[2], D, _TORCH_QTYPE[q.dtype]
+        d.seqs, d.width, d.window, d.sinks, d.scale = B, W, min(window, 0xFFFFFFFF), min(sinks, 0xFFFFFFFF), scale
+        d.base, d.seq_base = _u64_arg(base, self.device, B, w)
+        if rows is not None:
+            d.seq_rows = _u32_arg(rows, self.device, B, w)[1]
+        qq, kk, vv, oo = _rows4(q, w), _dense4(k, w), _dense4(v, w), _rows4(out, w)
+        A.check(self.lib.kvm_window_attention(self.h, C.byref(d), C.byref(qq), C.byref(kk), C.byref(vv), C.byref(oo),
+                                              _ptr(lse), _stream_on(self.device, stream).cuda_stream), w)
+        if flat:
+            return out[0], (None if lse is None else lse[0])
+        return out, lse
 
     def page_mass_from_lse(self, desc: A.ScoreDesc, rows: int, lse: torch.Tensor, *, want_rows=True,
                            want_mean=True, stream=None):
@@ -426,6 +522,116 @@ class ResidencyPool:
         return slot_of, page_of
 
 
+    # -- attention over the resident pages ---------------------------------
+    def tree_attention(self, q: torch.Tensor, tail_k: torch.Tensor, tail_v: torch.Tensor, *, layout: A.StageLayout,
+                       page_tokens: int, tokens, recent=0, sel_ids: Optional[torch.Tensor] = None,
+                       sel_n: Optional[torch.Tensor] = None, tree: Optional[torch.Tensor] = None,
+                       rows: Optional[torch.Tensor] = None, row0: int = 0, row_step: int = 1,
+                       k_type: Optional[int] = None, v_type: Optional[int] = None, scale: float = 0.0,
+                       out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, want_lse: bool = False,
+                       stream=None):
+        """Attention of drafted tokens (one per sequence: plain decode) over this pool's pages and each sequence's
+        tail (kvm_tree_attention).
+
+        q: [seqs][nodes][q_heads][head_dim] fp16 / bf16; tail_k, tail_v: [seqs][>= recent + nodes][kv_heads][head_dim]
+        of the same type, the recent committed tokens and then the drafted ones. Sequence i reads pool row row0 +
+        i * row_step: the pages listed in sel_ids [seqs][.] / sel_n [seqs] (select_topk's outputs), or every resident
+        page. tokens: history length, int or int64 tensor [seqs]; recent: int or int32 tensor [seqs]; tree: int32
+        tensor [nodes][words] or [seqs][nodes][words] (tree_mask), None for a chain; rows: int32 tensor [seqs], nodes
+        used. k_type / v_type: type of the pages (default: q's). Returns (out like q, lse [seqs][nodes][q_heads])."""
+        w = "kvm_tree_attention"
+        dev = self.ctx.device
+        _on_device(dev, w, q=q, tail_k=tail_k, tail_v=tail_v, out=out, lse=lse, sel_ids=sel_ids, sel_n=sel_n, tree=tree)
+        out, lse = _attention_out(w, q, tail_k, tail_v, out, lse, want_lse, _stream_on(dev, stream))
+        R, N, Hq, D = q.shape
+        t = _TORCH_QTYPE[q.dtype]
+        d = A.TreeDesc()
+        d.q_heads, d.kv_heads, d.head_dim, d.type = Hq, tail_k.shape[2], D, t
+        d.k_type, d.v_type = t if k_type is None else k_type, t if v_type is None else v_type
+        d.seqs, d.nodes, d.row0, d.row_step = R, N, row0, row_step
+        d.page_tokens, d.scale = page_tokens, scale
+        d.tokens, d.seq_tokens = _u64_arg(tokens, dev, R, w)
+        d.recent, d.seq_recent = _u32_arg(recent, dev, R, w)
+        if rows is not None:
+            d.seq_rows = _u32_arg(rows, dev, R, w)[1]
+        if sel_ids is not None:
+            if sel_n is None or sel_ids.dim() != 2 or sel_ids.shape[0] < R or sel_ids.element_size() != 4 or \
+                    (sel_ids.shape[1] > 1 and sel_ids.stride(1) != 1) or (R > 1 and sel_ids.stride(0) < sel_ids.shape[1]):
+                raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{w}: sel_ids is int32 [seqs][.] with sel_n [seqs]")
+            d.sel_ids, d.sel_n = sel_ids.data_ptr(), _u32_arg(sel_n, dev, R, w)[1]
+            d.sel_stride = sel_ids.stride(0) if R > 1 else sel_ids.shape[1]
+        if tree is not None:
+            if tree.element_size() != 4 or not tree.is_contiguous() or tree.dim() not in (2, 3) or \
+                    tree.shape[-2] != N or (tree.dim() == 3 and tree.shape[0] != R):
+                raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{w}: tree is contiguous int32 [nodes][words] or [seqs][nodes][words]")
+            d.tree, d.tree_words = tree.data_ptr(), tree.shape[-1]
+            d.tree_stride = N * tree.shape[-1] if tree.dim() == 3 else 0
+        qq, kk, vv, oo = _rows4(q, w), _dense4(tail_k, w), _dense4(tail_v, w), _rows4(out, w)
+        A.check(self.ctx.lib.kvm_tree_attention(self.ctx.h, self.h, C.byref(d), C.byref(layout), C.byref(qq), C.byref(kk),
+                                                C.byref(vv), C.byref(oo), _ptr(lse), _stream_on(dev, stream).cuda_stream), w)
+        return out, lse
+
+    # -- pages --------------------------------------------------------------
+    def tables(self):
+        """(slot_of [rows][pages], page_of [rows][slots]) int32 tensors that alias the pool's device tables: for
+        reading, while the pool lives."""
+        a, b = C.c_void_p(), C.c_void_p()
+        A.check(self.ctx.lib.kvm_pool_tables(self.h, C.byref(a), C.byref(b)), "kvm_pool_tables")
+        dev = torch.device("cuda", self.ctx.device)
+        return (torch.as_tensor(_DeviceTable(a.value, (self.rows, self.pages), self), device=dev),
+                torch.as_tensor(_DeviceTable(b.value, (self.rows, self.slots), self), device=dev))
+
+    def fork(self, layout: A.StageLayout, src_rows: Sequence[int], dst_rows: Sequence[int], *,
+             page_end: Optional[int] = None, ctas: int = 0, stream=None) -> None:
+        """Row dst_rows[i] becomes a copy of row src_rows[i]: its resident pages below page_end (default: all), in
+        the same slots (kvm_pool_fork)."""
+        n = len(dst_rows)
+        if len(src_rows) != n:
+            raise A.KvmError(A.ERR_INVALID_ARGUMENT, "kvm_pool_fork: as many sources as destinations")
+        src, dst = (C.c_uint32 * max(1, n))(*src_rows), (C.c_uint32 * max(1, n))(*dst_rows)
+        A.check(self.ctx.lib.kvm_pool_fork(self.ctx.h, self.h, C.byref(layout), src, dst, n,
+                                           self.pages if page_end is None else page_end, ctas,
+                                           _stream_on(self.ctx.device, stream).cuda_stream), "kvm_pool_fork")
+
+    def copy_pages(self, layout: A.StageLayout, items, *, ctas: int = 0, stream=None) -> None:
+        """items: (src_row, src_page, dst_row, dst_page) tuples, or a contiguous int32 CPU tensor [n][4]
+        (kvm_pool_copy)."""
+        if isinstance(items, torch.Tensor):
+            if items.device.type != "cpu" or items.dtype != torch.int32 or items.dim() != 2 or items.shape[1] != 4 or \
+                    not items.is_contiguous():
+                raise A.KvmError(A.ERR_INVALID_ARGUMENT, "kvm_pool_copy: items is a contiguous int32 CPU tensor [n][4]")
+            n, ptr = items.shape[0], items.data_ptr()
+        else:
+            arr = (A.PageCopy * max(1, len(items)))(*[A.PageCopy(*x) for x in items])
+            n, ptr = len(items), C.cast(arr, C.c_void_p)
+        A.check(self.ctx.lib.kvm_pool_copy(self.ctx.h, self.h, C.byref(layout), ptr, n, ctas,
+                                           _stream_on(self.ctx.device, stream).cuda_stream), "kvm_pool_copy")
+
+    def free(self, rows: Sequence[int], ids: torch.Tensor, counts: torch.Tensor, *, stream=None) -> None:
+        """Drops the pages ids[i][: counts[i]] (int32, device) of row rows[i] (kvm_pool_free)."""
+        n = len(rows)
+        w = "kvm_pool_free"
+        _on_device(self.ctx.device, w, ids=ids, counts=counts)
+        if ids.dim() != 2 or ids.shape[0] < n or ids.element_size() != 4 or not ids.is_contiguous():
+            raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{w}: ids is contiguous int32 [rows][.]")
+        arr = (C.c_uint32 * max(1, n))(*rows)
+        A.check(self.ctx.lib.kvm_pool_free(self.ctx.h, self.h, arr, n, ids.data_ptr(),
+                                           _u32_arg(counts, self.ctx.device, n, w)[1], ids.shape[1],
+                                           _stream_on(self.ctx.device, stream).cuda_stream), w)
+
+    def compact(self, layout: A.StageLayout, rows: Optional[Sequence[int]] = None, *, used: Optional[torch.Tensor] = None,
+                ctas: int = 0, stream=None) -> None:
+        """Brings the resident pages of `rows` (default: all) into their first slots (kvm_pool_compact); used: int32
+        tensor [rows], receives the number of resident pages."""
+        rows = range(self.rows) if rows is None else rows
+        n = len(rows)
+        w = "kvm_pool_compact"
+        arr = (C.c_uint32 * max(1, n))(*rows)
+        ptr = None if used is None else _u32_arg(used, self.ctx.device, n, w)[1]
+        A.check(self.ctx.lib.kvm_pool_compact(self.ctx.h, self.h, C.byref(layout), arr, n, ptr, ctas,
+                                              _stream_on(self.ctx.device, stream).cuda_stream), w)
+
+
 class Transfer:
     """A working-set transfer over a ResidencyPool (kvm_transfer): the GPU side of
     kvmem::MemoryTransfer (kvmem/include/kvmem/memory_contract.hpp:171-185). The
@@ -548,6 +754,49 @@ class StageOut:
 
     def clear(self) -> None:
         A.check(self.lib.kvm_stageout_clear(self.h), "kvm_stageout_clear")
+
+
+def _attention_out(where, q, k, v, out, lse, want_lse, stream):
+    """Shape and type checks of an attention call, and its outputs (allocated for `stream` where not given)."""
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or q.dtype not in (torch.float16, torch.bfloat16):
+        raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{where}: q, k, v are 4-D, q fp16 or bf16")
+    if k.dtype != q.dtype or v.dtype != q.dtype or k.shape != v.shape or k.shape[0] != q.shape[0] or \
+            k.shape[3] != q.shape[3]:
+        raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{where}: k and v do not match q")
+    with torch.cuda.stream(stream):
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        if lse is None and want_lse:
+            lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
+    if out.shape != q.shape or out.dtype != q.dtype:
+        raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{where}: out does not match q")
+    if lse is not None and (lse.shape != q.shape[:3] or lse.dtype != torch.float32 or not lse.is_contiguous()):
+        raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{where}: lse is contiguous float32 [seqs][rows][q_heads]")
+    return out, lse
+
+
+def tree_mask(parents: Sequence[int]) -> torch.Tensor:
+    """The visibility words int32 [nodes][words] (CPU) of a tree of drafted tokens given by parents, -1 for a root
+    (kvm_tree_mask)."""
+    n = len(parents)
+    words = max(1, -(-n // 32))
+    out = torch.zeros((n, words), dtype=torch.int32)
+    arr = (C.c_int32 * max(1, n))(*parents)
+    A.check(A.load().kvm_tree_mask(arr, n, words, out.data_ptr()), "kvm_tree_mask")
+    return out
+
+
+def cache_layout(*planes: torch.Tensor) -> A.StageLayout:
+    """Layout of a paged cache alone (no host records): one or two device tensors [rows][slots][...] whose slots are
+    contiguous."""
+    out = []
+    for t in planes:
+        if t.dim() < 3 or not t[0, 0].is_contiguous():
+            raise A.KvmError(A.ERR_INVALID_ARGUMENT, "cache_layout: [rows][slots][...] with contiguous slots")
+        es = t.element_size()
+        out.append(dict(host_base=None, host_row_stride=0, host_page_stride=0, dev_base=t.data_ptr(),
+                        dev_row_stride=t.stride(0) * es, dev_slot_stride=t.stride(1) * es, bytes=t[0, 0].numel() * es))
+    return stage_layout(out)
 
 
 def ipc_export(t: torch.Tensor) -> bytes:
