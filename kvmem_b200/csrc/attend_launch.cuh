@@ -27,16 +27,29 @@ int launch_attend_m(kvm_ctx* c, const AttendParams& p, int mode, bool quant, cud
 
 template <int D, bool BF16>
 int launch_attend_t(kvm_ctx* c, const AttendParams& p, int mode, bool quant, int wm, cudaStream_t s) {
-    int rc = wm == 1   ? launch_attend_m<D, 1, BF16>(c, p, mode, quant, s)
-             : wm == 2 ? launch_attend_m<D, 2, BF16>(c, p, mode, quant, s)
-                       : launch_attend_m<D, 4, BF16>(c, p, mode, quant, s);
-    if (rc != KVM_OK || p.splits == 1) return rc;
+    return wm == 1   ? launch_attend_m<D, 1, BF16>(c, p, mode, quant, s)
+           : wm == 2 ? launch_attend_m<D, 2, BF16>(c, p, mode, quant, s)
+                     : launch_attend_m<D, 4, BF16>(c, p, mode, quant, s);
+}
+
+template <int D, bool BF16>
+int launch_attend_combine_t(kvm_ctx* c, const AttendParams& p, cudaStream_t s) {
     const uint64_t rows = uint64_t(p.seqs) * p.width * p.q_heads;
     if (rows > 0x7fffffffull) return KVM_ERR_LENGTH;
     const uint32_t warps = p.splits < 8 ? (p.splits < 4 ? 2 : 4) : 8;
     attend_combine_kernel<D, BF16><<<uint32_t(rows), warps * 32, 0, s>>>(p);
     ++c->launches;
     return cudaGetLastError() == cudaSuccess ? KVM_OK : KVM_ERR_CUDA;
+}
+
+// The joining pass, where the keys were split.
+inline int launch_attend_combine(kvm_ctx* c, const AttendParams& p, uint32_t dim, bool bf16, cudaStream_t s) {
+    if (p.splits == 1) return KVM_OK;
+    switch (dim) {
+        case 64: return bf16 ? launch_attend_combine_t<64, true>(c, p, s) : launch_attend_combine_t<64, false>(c, p, s);
+        case 128: return bf16 ? launch_attend_combine_t<128, true>(c, p, s) : launch_attend_combine_t<128, false>(c, p, s);
+        default: return bf16 ? launch_attend_combine_t<256, true>(c, p, s) : launch_attend_combine_t<256, false>(c, p, s);
+    }
 }
 
 extern template int launch_attend_t<64, false>(kvm_ctx*, const AttendParams&, int, bool, int, cudaStream_t);

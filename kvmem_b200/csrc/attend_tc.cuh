@@ -1,0 +1,638 @@
+// Attention of many rows over a cache on the 5th-generation tensor cores: the
+// same operators as attend.cuh (window with sinks, tree over pages), for packed row
+// counts where the products and not the reading of K and V bound the time.
+//
+// One CTA per (sequence, KV head, 128 * MT packed rows, key chunk), one per SM:
+//  * warp 0 (one thread): TMA loads of 128-key tiles into one ring of 16 KiB
+//    units, K and V in the order in which the products take them. A K unit is 128
+//    keys x 64 dims (the B operand of S, K-major); a V unit is 32 / 64 / 128 keys x
+//    256 / 128 / 64 dims (the B operand of O, MN-major). Small units let the ring
+//    hold two and a half 64 KiB tiles at head_dim 256. Pages come as boxes of
+//    gcd(page_tokens, 128) tokens, each from its slot;
+//  * warp 1 (one thread): tcgen05.mma kind::f16, S = Q K^T (M = 128, N = 128, Q in
+//    shared memory), then O += P V (N = head_dim, P from tensor memory, where it
+//    replaces its S). Two S accumulators are in flight: the two M tiles of a CTA
+//    (MT = 2, head_dim 64 / 128: K and V are read once for 256 rows), or two
+//    successive key tiles of one (MT = 1, head_dim 256, where O takes half of the
+//    tensor memory). S of step w + 2 is issued right behind P V of step w;
+//  * four softmax warps per M tile: thread = packed row = tensor-memory lane.
+//    Masks are four words of bits per row and tile, made only for tiles that some
+//    row sees in part. The running max moves lazily: O is rescaled only when it
+//    grows by more than 2^8, so P stays below 2^8 and sums stay in 32 bits.
+// A V tile behind a mask may hold infinities or NaN, which 0 * x would spread to
+// rows that do not see them: masked tiles are scanned, such values are taken out of
+// the product and added by hand to the rows that do see them.
+// Every wait is bounded: on expiry the kernel records KVM_ERR_TIMEOUT, raises the
+// CTA's abort flag, lets copies and MMAs in flight finish and frees its TMEM.
+#pragma once
+#include "attend.cuh"
+#include "prefill_attn.cuh"
+
+namespace kvmb {
+
+constexpr int kAcKeys = 128;             // keys per tile
+constexpr uint32_t kAcUnit = 16384;      // bytes per ring unit
+constexpr uint32_t kAcTable = 512;       // page entries of one CTA's key chunk
+constexpr uint32_t kAcMaxUnits = 12;
+
+__host__ __device__ constexpr int ac_mt(int D) { return D == 256 ? 1 : 2; }
+__host__ __device__ constexpr int ac_threads(int D) { return 128 + 128 * ac_mt(D); }
+__host__ __device__ constexpr uint32_t ac_units(int D, int mode) {
+    // What is left of 227 KiB beside the query tiles (and the page table).
+    return (D == 64 ? 12u : 10u) - (mode == kAtTree ? 1u : 0u);
+}
+__host__ __device__ constexpr uint32_t ac_smem_bytes(int D, int mode) {
+    return 1024u + uint32_t(ac_mt(D)) * 128u * uint32_t(D) * 2u + ac_units(D, mode) * kAcUnit +
+           (mode == kAtTree ? kAcTable * 8u : 0u) + 512u;
+}
+
+static_assert(ac_smem_bytes(64, kAtTree) <= 227 * 1024 && ac_smem_bytes(64, kAtWindow) <= 227 * 1024 &&
+              ac_smem_bytes(128, kAtTree) <= 227 * 1024 && ac_smem_bytes(256, kAtWindow) <= 227 * 1024, "shared memory");
+
+struct AttendTcMaps {
+    CUtensorMap dk, dv;  // dense keys: (D, kv_heads, tokens, sequences), boxes (64, 1, 128 | V unit keys, 1)
+    CUtensorMap pk, pv;  // pages: (D, kv_heads, page_tokens, slots, rows), boxes (64, 1, box | min(box, V unit keys), 1, 1)
+};
+
+__device__ __forceinline__ void ac_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
+            "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        : "memory");
+}
+__device__ __forceinline__ void ac_load_5d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, int v,
+                                           uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// Max of 128 values by three-input maxes.
+__device__ __forceinline__ float ac_max128(const float* x) { return fmaxf(pf_max64(x), pf_max64(x + 64)); }
+
+template <int D, bool BF16, int MODE>
+__global__ void __launch_bounds__(ac_threads(D), 1)
+    attend_tc_kernel(const __grid_constant__ AttendTcMaps maps, const __grid_constant__ AttendParams P,
+                     const uint32_t box) {
+    constexpr int MT = ac_mt(D);
+    constexpr uint32_t U = D / 64;               // units of a K tile, and of a V tile
+    constexpr uint32_t VK = kAcUnit / (D * 2);   // keys of a V unit
+    constexpr uint32_t NU = ac_units(D, MODE);
+    constexpr uint32_t kQTile = 128 * D * 2;
+    constexpr uint32_t kColO = 256;              // S / P: columns 0-127 and 128-255; O of M tile m: 256 + m * D
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* qsm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* ring = qsm + MT * kQTile;
+    int2* table = reinterpret_cast<int2*>(ring + NU * kAcUnit);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(table) + (MODE == kAtTree ? kAcTable * 8 : 0));
+    uint64_t* full = bars;                 // [NU]
+    uint64_t* empty = bars + kAcMaxUnits;  // [NU]
+    uint64_t* s_full = bars + 2 * kAcMaxUnits;      // [2]
+    uint64_t* p_full = bars + 2 * kAcMaxUnits + 2;  // [2]
+    uint64_t* pv_done = bars + 2 * kAcMaxUnits + 4; // [2]
+    uint64_t* q_full = bars + 2 * kAcMaxUnits + 6;
+    uint64_t* fin = bars + 2 * kAcMaxUnits + 7;
+    uint64_t* together = bars + 2 * kAcMaxUnits + 8;  // all softmax threads (a barrier whose wait is bounded)
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kAcMaxUnits + 9);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    uint32_t* bad_flag = tmem_slot + 2;  // [2], by tile parity
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint32_t un = blockIdx.x;
+    const uint32_t mt = un % P.m_tiles;
+    un /= P.m_tiles;
+    const uint32_t split = un % P.splits;
+    un /= P.splits;
+    const uint32_t h = un % P.kv_heads, b = un / P.kv_heads;
+    const uint32_t G = P.group;
+    const uint32_t rows = P.seq_rows ? min(__ldg(P.seq_rows + b), P.width) : P.width;
+    const uint32_t m0 = mt * 128 * MT, m_end = rows * G;
+    if (m0 >= m_end) return;
+    const uint32_t i0 = m0 / G, i1 = min(m0 + 128 * MT - 1, m_end - 1) / G;
+
+    // ---- this unit's keys (as attend_mma_kernel, tiles of 128) ----
+    uint32_t nt, n_first;
+    uint32_t p0 = 0, p1 = 0, lo = 0, hi = 0, few = 0;
+    uint32_t n_keys = 0, recent = 0, prow = 0;
+    uint32_t e0 = 0;
+    if constexpr (MODE == kAtWindow) {
+        const uint64_t base = P.seq_base ? __ldg(reinterpret_cast<const unsigned long long*>(P.seq_base + b)) : P.base;
+        if (base > P.capacity || rows > P.capacity - base) {
+            if (tid == 0) record_error(P.status, KVM_ERR_LENGTH, 120);
+            return;
+        }
+        p0 = uint32_t(base) + i0;
+        p1 = uint32_t(base) + i1;
+        hi = p1 + 1;
+        lo = P.window == 0 ? hi : (p0 + 1 > P.window ? p0 + 1 - P.window : 0);
+        few = min(P.sinks, lo);
+        n_first = (few + kAcKeys - 1) / kAcKeys;
+        nt = n_first + (hi - lo + kAcKeys - 1) / kAcKeys;
+    } else {
+        recent = P.seq_recent ? __ldg(P.seq_recent + b) : P.recent;
+        if (recent > P.capacity || rows > P.capacity - recent) {
+            if (tid == 0) record_error(P.status, KVM_ERR_LENGTH, 121);
+            return;
+        }
+        prow = P.row0 + b * P.row_step;
+        uint32_t n_list = P.pool_slots;
+        if (P.sel_ids) {
+            n_list = __ldg(P.sel_n + b);
+            if (n_list > P.sel_stride) {
+                if (tid == 0) record_error(P.status, KVM_ERR_INVALID_ARGUMENT, 122);
+                n_list = P.sel_stride;
+            }
+        }
+        n_keys = n_list * P.page_tokens;
+        n_first = (n_keys + kAcKeys - 1) / kAcKeys;
+        nt = n_first + (recent + rows + kAcKeys - 1) / kAcKeys;
+    }
+    const uint32_t tb = uint32_t(uint64_t(nt) * split / P.splits), te = uint32_t(uint64_t(nt) * (split + 1) / P.splits);
+    const uint32_t n = te - tb;  // tiles of this CTA
+    auto page_div = [&](uint32_t x) { return uint32_t((uint64_t(x) * P.pt_magic) >> P.pt_shift); };
+    if constexpr (MODE == kAtTree) {
+        // {slot, tokens held} of the chunk's pages; the host's chunks touch at most kAcTable of them.
+        e0 = page_div(tb * kAcKeys);
+        const uint32_t last = min(te, n_first) * kAcKeys;
+        const uint32_t n_ent = tb < min(te, n_first) ? min(page_div(min(last, n_keys) - 1) + 1 - e0, kAcTable) : 0;
+        const uint64_t tokens = P.seq_tokens ? __ldg(reinterpret_cast<const unsigned long long*>(P.seq_tokens + b)) : P.tokens;
+        for (uint32_t i = tid; i < n_ent; i += ac_threads(D)) {
+            const uint32_t e = e0 + i;
+            int page, slot;
+            if (P.sel_ids) {
+                const uint32_t id = __ldg(P.sel_ids + uint64_t(b) * P.sel_stride + e);
+                page = id < P.pool_pages ? int(id) : -1;
+                slot = page >= 0 ? P.slot_of[uint64_t(prow) * P.pool_pages + page] : -1;
+                if (page < 0) record_error(P.status, KVM_ERR_INVALID_ARGUMENT, 123);
+                else if (slot < 0 || slot >= int(P.pool_slots)) {
+                    record_error(P.status, KVM_ERR_STALE, 124);
+                    page = -1;
+                }
+            } else {
+                slot = int(e);
+                page = P.page_of[uint64_t(prow) * P.pool_slots + e];
+            }
+            int2 ent = make_int2(0, 0);
+            if (page >= 0) {
+                const uint64_t start = uint64_t(page) * P.page_tokens;
+                const uint64_t held = tokens > start ? tokens - start : 0;
+                ent = make_int2(slot, int(min(held, uint64_t(P.page_tokens))));
+            }
+            table[i] = ent;
+        }
+    }
+
+    if (tid == 0) {
+        for (uint32_t i = 0; i < NU; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 128);
+            mbar_init(&pv_done[i], 1);
+        }
+        mbar_init(q_full, 128 * MT);
+        mbar_init(fin, 1);
+        mbar_init(together, 128 * MT);
+        *abort_flag = 0;
+        bad_flag[0] = bad_flag[1] = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    // Ring order of the units: the order in which the products take the tiles.
+    // MT = 2: K0 V0 K1 V1 ..; MT = 1: K0 K1 V0 K2 V1 .. V(n - 1).
+    auto k_unit = [&](uint32_t j) { return MT == 2 ? 2 * j * U : (j ? (2 * j - 1) * U : 0); };
+    auto v_unit = [&](uint32_t j) { return MT == 2 ? (2 * j + 1) * U : (j + 1 == n ? (2 * n - 1) * U : (2 * j + 2) * U); };
+
+    // MT = 2: registers go to the softmax warps, 4 x 32 x 72 + 8 x 32 x 216 = 384 x 168.
+    if (warp < 4) {
+        if constexpr (MT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 0) {
+            // ---- TMA producer ----
+            if (lane == 0) {
+                uint32_t issued = 0;
+                // Unit `sub` of K (or V) tile j of this CTA.
+                auto load = [&](uint32_t idx, uint32_t j, bool is_v, uint32_t sub) -> bool {
+                    const uint32_t s = idx % NU;
+                    if (idx >= NU && !mbar_wait(&empty[s], ((idx - NU) / NU) & 1)) {
+                        record_error(P.status, KVM_ERR_TIMEOUT, 125);
+                        return false;
+                    }
+                    const uint32_t dst = smem_u32(ring + s * kAcUnit), t = tb + j;
+                    const uint32_t keys = is_v ? VK : uint32_t(kAcKeys), key0 = is_v ? sub * VK : 0;
+                    const uint32_t d0 = is_v ? 0 : sub, d1 = is_v ? U : sub + 1;  // 64-dim blocks
+                    issued = idx + 1;
+                    if (MODE == kAtWindow || t >= n_first) {
+                        const uint32_t tok = MODE == kAtWindow
+                                                 ? (t < n_first ? t * kAcKeys : lo + (t - n_first) * kAcKeys) + key0
+                                                 : (t - n_first) * kAcKeys + key0;
+                        mbar_arrive_expect_tx(&full[s], kAcUnit);
+                        for (uint32_t a = d0; a < d1; ++a)
+                            ac_load_4d(dst + (a - d0) * keys * 128, is_v ? &maps.dv : &maps.dk, int(a * 64), int(h), int(tok),
+                                       int(b), &full[s]);
+                    } else {
+                        const uint32_t bh = min(box, keys), nb = keys / bh;
+                        uint32_t live = 0;
+                        for (uint32_t i = 0; i < nb; ++i) {
+                            const uint32_t x = t * kAcKeys + key0 + i * bh, en = page_div(x);
+                            if (x < n_keys && int(x - en * P.page_tokens) < table[en - e0].y) ++live;
+                        }
+                        if (live) mbar_arrive_expect_tx(&full[s], live * bh * 128 * (d1 - d0));
+                        else mbar_arrive(&full[s]);
+                        if (live)
+                            for (uint32_t i = 0; i < nb; ++i) {
+                                const uint32_t x = t * kAcKeys + key0 + i * bh, en = page_div(x), o = x - en * P.page_tokens;
+                                if (x >= n_keys || int(o) >= table[en - e0].y) continue;
+                                for (uint32_t a = d0; a < d1; ++a)
+                                    ac_load_5d(dst + (a - d0) * keys * 128 + i * bh * 128, is_v ? &maps.pv : &maps.pk,
+                                               int(a * 64), int(h), int(o), table[en - e0].x, int(prow), &full[s]);
+                            }
+                    }
+                    return true;
+                };
+                bool ok = true;
+                auto load_k = [&](uint32_t j) {
+                    for (uint32_t i = 0; i < U && ok && !*abort_flag; ++i) ok = load(k_unit(j) + i, j, false, i);
+                };
+                auto load_v = [&](uint32_t j) {
+                    for (uint32_t i = 0; i < U && ok && !*abort_flag; ++i) ok = load(v_unit(j) + i, j, true, i);
+                };
+                if (n) {
+                    load_k(0);
+                    if (MT == 1 && n > 1) load_k(1);
+                    for (uint32_t j = 0; j < n && ok && !*abort_flag; ++j) {
+                        load_v(j);
+                        if (j + (3 - MT) < n) load_k(j + (3 - MT));
+                    }
+                }
+                if (!ok) *abort_flag = 1;
+                // Every issued copy lands before the CTA frees its shared memory.
+                for (uint32_t i = issued > NU ? issued - NU : 0; i < issued; ++i)
+                    if (!mbar_wait(&full[i % NU], (i / NU) & 1)) record_error(P.status, KVM_ERR_TIMEOUT, 126);
+            }
+        } else if (warp == 1) {
+            // ---- MMA issue: one thread; step w = (tile w / MT, M tile w % MT), S slot w & 1 ----
+            if (lane == 0) {
+                constexpr uint32_t idesc_s = pf_idesc(128, kAcKeys, BF16, false);
+                constexpr uint32_t idesc_o = pf_idesc(128, D, BF16, true);
+                int err = 0;
+                auto issue_s = [&](uint32_t w) -> bool {
+                    const uint32_t j = w / MT, m = w % MT, at = k_unit(j);
+                    const uint32_t qb = smem_u32(qsm + m * kQTile);
+                    for (uint32_t a = 0; a < U; ++a) {
+                        const uint32_t s = (at + a) % NU;
+                        if (!mbar_wait(&full[s], ((at + a) / NU) & 1)) return false;
+                        tc_fence_after();
+                        const uint32_t kb = smem_u32(ring + s * kAcUnit);
+    #pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            tc_mma(tmem + (w & 1) * 128, tc_desc_sw128(qb + a * 16384 + kk * 32), tc_desc_sw128(kb + kk * 32),
+                                   idesc_s, (a | kk) != 0);
+                        if (m == MT - 1) tc_commit(&empty[s]);
+                    }
+                    tc_commit(&s_full[w & 1]);
+                    return true;
+                };
+                const uint32_t steps = n * MT;
+                if (!mbar_wait(q_full, 0)) err = 130;
+                tc_fence_after();
+                for (uint32_t w = 0; w < 2 && w < steps && !err; ++w)
+                    if (!issue_s(w)) err = 131;
+                for (uint32_t w = 0; w < steps && !err; ++w) {
+                    if (*abort_flag) {
+                        err = -1;
+                        break;
+                    }
+                    const uint32_t j = w / MT, m = w % MT, at = v_unit(j);
+                    if (!mbar_wait(&p_full[w & 1], (w >> 1) & 1)) {
+                        err = 132;
+                        break;
+                    }
+                    tc_fence_after();
+                    for (uint32_t a = 0; a < U; ++a) {
+                        const uint32_t s = (at + a) % NU;
+                        if (!mbar_wait(&full[s], ((at + a) / NU) & 1)) {
+                            err = 133;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t vb = smem_u32(ring + s * kAcUnit);
+    #pragma unroll
+                        for (uint32_t kk = 0; kk < VK / 16; ++kk)  // P: 16 keys = 8 tensor-memory columns
+                            tc_mma_ts(tmem + kColO + m * D, tmem + (w & 1) * 128 + (a * (VK / 16) + kk) * 8,
+                                      pf_desc_mn_sw128(vb + kk * 2048, VK * 128), idesc_o, j > 0 || (a | kk) != 0);
+                        if (m == MT - 1) tc_commit(&empty[s]);
+                    }
+                    if (err) break;
+                    tc_commit(&pv_done[w & 1]);
+                    if (w + 2 < steps && !issue_s(w + 2)) err = 131;
+                }
+                if (err > 0) {
+                    record_error(P.status, KVM_ERR_TIMEOUT, err);
+                    *abort_flag = 1;
+                }
+                tc_commit(fin);
+                if (!mbar_wait(fin, 0)) record_error(P.status, KVM_ERR_TIMEOUT, 134);
+            }
+        }
+    } else {
+        if constexpr (MT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        // ---- softmax: thread = packed row = tensor-memory lane ----
+        const uint32_t m = uint32_t(tid - 128) / 128, row = uint32_t(tid - 128) % 128;
+        const uint32_t lane_addr = tmem + ((32u * uint32_t(warp & 3)) << 16);
+        const uint32_t r = m0 + m * 128 + row;  // packed row
+        const uint32_t ri = min(r, m_end - 1) / G;
+        const uint32_t qh = h * G + (min(r, m_end - 1) - ri * G);
+        {
+            const uint4* qp = reinterpret_cast<const uint4*>(P.q + uint64_t(b) * P.q_seq + uint64_t(ri) * P.q_row +
+                                                             uint64_t(qh) * P.q_head);
+            uint8_t* qd = qsm + m * kQTile + row * 128;
+#pragma unroll 8
+            for (uint32_t c = 0; c < D / 8; ++c) {
+                const uint4 x = r < m_end ? __ldg(qp + c) : make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(qd + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4)) = x;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive(q_full);
+        }
+        const float c2 = P.scale_log2;
+        float m_used = -1e30f, l = 0.f;
+        bool ok = true;
+        uint32_t meet_phase = 0;
+        auto meet = [&] {
+            mbar_arrive(together);
+            ok = pf_warp_wait(together, meet_phase) && ok;
+            meet_phase ^= 1;
+        };
+        auto below = [](int x, int q4) -> uint32_t {  // bits of the keys < x in word q4
+            const int y = min(max(x - q4 * 32, 0), 32);
+            return y == 32 ? ~0u : (1u << y) - 1u;
+        };
+        const uint32_t col_o = lane_addr + kColO + m * D;
+        for (uint32_t j = 0; j < n; ++j) {
+            const uint32_t w = j * MT + m, slot = w & 1, t = tb + j;
+            if (__shfl_sync(0xffffffffu, *abort_flag, 0)) {
+                ok = false;
+                break;
+            }
+            // Which of the tile's keys this row sees; `part`: some row of the CTA does not see all.
+            uint32_t see[4] = {~0u, ~0u, ~0u, ~0u};
+            bool part;
+            if constexpr (MODE == kAtWindow) {
+                const uint32_t a = t < n_first ? t * kAcKeys : lo + (t - n_first) * kAcKeys;
+                const uint32_t end = t < n_first ? few : hi;
+                part = !(a + kAcKeys <= end && a + kAcKeys - 1 <= p0 && (a + kAcKeys <= P.sinks || p1 - a < P.window));
+                if (part) {
+                    // Keys [0, s1) u [w0, u1) of the tile: sinks, and the window up to the row's position.
+                    const uint32_t p = p0 + (ri - i0);
+                    const int u1 = int(min(end, p + 1)) - int(a);
+                    const int s1 = min(P.sinks > a ? int(min(P.sinks - a, 256u)) : 0, u1);
+                    const int w0 = P.window == 0 ? 256 : (p + 1 > P.window ? int(p + 1 - P.window) - int(a) : 0);
+#pragma unroll
+                    for (int q4 = 0; q4 < 4; ++q4) see[q4] = below(s1, q4) | (below(u1, q4) & ~below(w0, q4));
+                }
+            } else if (t >= n_first) {
+                const uint32_t a = (t - n_first) * kAcKeys;
+                part = a + kAcKeys > recent;
+                if (part) {
+const int rec = int(recent) - int(a);  // keys below are recent tokens, key rec + x is node x
+                    const uint32_t* tw = P.tree ? P.tree + uint64_t(b) * P.tree_seq + uint64_t(ri) * P.tree_words : nullptr;
+                    auto word = [&](int i) { return i >= 0 && i < int(P.tree_words) ? __ldg(tw + i) : 0u; };
+#pragma unroll
+                    for (int q4 = 0; q4 < 4; ++q4) {
+                        uint32_t bits;
+                        if (tw) {
+                            const int nd = q4 * 32 - rec;
+                            bits = __funnelshift_r(word(nd >> 5), word((nd >> 5) + 1), nd & 31) & below(rec + int(rows), q4);
+                        } else {
+                            bits = below(rec + int(ri) + 1, q4);
+                        }
+                        see[q4] = bits | below(rec, q4);
+                    }
+                }
+            } else {
+                part = t * kAcKeys + kAcKeys > n_keys;
+                const uint32_t first = page_div(t * kAcKeys), last = page_div(min(t * kAcKeys + kAcKeys, n_keys) - 1);
+                for (uint32_t e = first; e <= last; ++e) part = part || table[e - e0].y != int(P.page_tokens);
+                if (part) {
+                    see[0] = see[1] = see[2] = see[3] = 0;
+                    for (uint32_t e = first; e <= last; ++e) {
+                        const int at = int(e * P.page_tokens) - int(t * kAcKeys), end = at + table[e - e0].y;
+#pragma unroll
+                        for (int q4 = 0; q4 < 4; ++q4) see[q4] |= below(end, q4) & ~below(at, q4);
+                    }
+                }
+            }
+            if (!pf_warp_wait(&s_full[slot], (w >> 1) & 1)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            float x[kAcKeys];
+            {
+                uint32_t* u = reinterpret_cast<uint32_t*>(x);
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4) tc_ld32(lane_addr + slot * 128 + q4 * 32, u + q4 * 32);
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4) tc_wait_ld(u + q4 * 32);
+            }
+            if (part) {
+#pragma unroll
+                for (int k = 0; k < kAcKeys; ++k)
+                    if (!((see[k >> 5] >> (k & 31)) & 1)) x[k] = -INFINITY;
+            }
+            const float mx = ac_max128(x) * c2;
+            const bool need = mx > m_used + kPfRescale;
+            if (j == 0) {
+                m_used = fmaxf(mx, -1e30f);
+            } else if (__any_sync(0xffffffffu, need)) {
+                float alpha = 1.f;
+                if (need) {
+                    alpha = fast_exp2(m_used - mx);
+                    m_used = mx;
+                    l *= alpha;
+                }
+                // O holds the products of the tiles before once the last of them is done.
+                const uint32_t wp = w - MT;
+                if (!pf_warp_wait(&pv_done[wp & 1], (wp >> 1) & 1)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+#pragma unroll 1
+                for (uint32_t cc = 0; cc < D; cc += 32) {
+                    uint32_t o[32];
+                    tc_ld32(col_o + cc, o);
+                    tc_wait_ld(o);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                    tc_st32(col_o + cc, o);
+                }
+                tc_wait_st();
+            }
+            const float mneg = -m_used;
+            float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < kAcKeys; k += 2) {
+                pf_fma2(x[k], x[k + 1], x[k], x[k + 1], c2, mneg);
+                x[k] = fast_exp2(x[k]);
+                x[k + 1] = fast_exp2(x[k + 1]);
+                pf_add2(s4[k & 2], s4[(k & 2) + 1], x[k], x[k + 1]);
+            }
+            l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+            bool bad = false;
+            if (part) {
+                // Infinite or NaN values in a V tile that some row does not see in full.
+                const uint32_t at = v_unit(j);
+                for (uint32_t a = 0; a < U && ok; ++a) {
+                    ok = pf_warp_wait(&full[(at + a) % NU], ((at + a) / NU) & 1);
+                    const uint4* v4 = reinterpret_cast<const uint4*>(ring + ((at + a) % NU) * kAcUnit);
+                    for (uint32_t e = row; e < kAcUnit / 16; e += 128) {
+                        const uint4 y = v4[e];
+                        bad = bad || at_nonfinite<BF16>(y.x) || at_nonfinite<BF16>(y.y) || at_nonfinite<BF16>(y.z) ||
+                              at_nonfinite<BF16>(y.w);
+                    }
+                }
+                if (bad) atomicOr(&bad_flag[j & 1], 1u);
+                meet();
+                bad = *reinterpret_cast<volatile uint32_t*>(&bad_flag[j & 1]) != 0;
+                meet();
+                if (!ok) break;
+                if (row == 0 && m == 0) bad_flag[j & 1] = 0;  // read by all; set again two tiles on at the earliest
+            }
+            // P over its S, 16-bit, two per column.
+#pragma unroll
+            for (int q4 = 0; q4 < 2; ++q4) {
+                uint32_t pk[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) pk[i] = pf_pack2<BF16>(x[q4 * 64 + 2 * i], x[q4 * 64 + 2 * i + 1]);
+                tc_st32(lane_addr + slot * 128 + q4 * 32, pk);
+            }
+            if (bad) {
+                // sums of p * v over the infinite and NaN values this row sees, which leave the product
+                float fix[D], pl[kAcKeys];
+#pragma unroll
+                for (int k = 0; k < kAcKeys; ++k) pl[k] = x[k];
+                const uint32_t at = v_unit(j);
+#pragma unroll 1
+                for (uint32_t d = 0; d < D; ++d) {
+                    float f = 0.f;
+#pragma unroll 1
+                    for (uint32_t k = 0; k < uint32_t(kAcKeys); ++k) {
+                        const uint32_t kr = k % VK;
+                        const uint16_t bits = *reinterpret_cast<const uint16_t*>(
+                            ring + ((at + k / VK) % NU) * kAcUnit + (d / 64) * VK * 128 + kr * 128 +
+                            ((((d % 64) / 8) ^ (kr & 7)) << 4) + (d % 8) * 2);
+                        if (at_nonfinite<BF16>(bits)) {
+                            const uint32_t sw = k >> 5 == 0 ? see[0] : k >> 5 == 1 ? see[1] : k >> 5 == 2 ? see[2] : see[3];
+                            if ((sw >> (k & 31)) & 1) f += pl[k] * at_unpack<BF16>(bits).x;
+                        }
+                    }
+                    fix[d] = f;
+                }
+                meet();
+                for (uint32_t a = m; a < U; a += MT) {
+                    uint16_t* v2 = reinterpret_cast<uint16_t*>(ring + ((at + a) % NU) * kAcUnit);
+                    for (uint32_t e = row; e < kAcUnit / 2; e += 128)
+                        if (at_nonfinite<BF16>(v2[e])) v2[e] = 0;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                meet();
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive(&p_full[slot]);
+                if (!ok || !pf_warp_wait(&pv_done[slot], (w >> 1) & 1)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+#pragma unroll 1
+                for (uint32_t cc = 0; cc < D; cc += 32) {
+                    uint32_t o[32];
+                    tc_ld32(col_o + cc, o);
+                    tc_wait_ld(o);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) + fix[cc + i]);
+                    tc_st32(col_o + cc, o);
+                }
+                tc_wait_st();
+                tc_fence_before();
+            } else {
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive(&p_full[slot]);
+            }
+        }
+        const bool go = __shfl_sync(0xffffffffu, (ok && !*abort_flag) ? 1 : 0, 0) != 0;
+        if (go) {
+            const uint32_t wl = (n - 1) * MT + m;
+            if (n == 0 || pf_warp_wait(&pv_done[wl & 1], (wl >> 1) & 1)) {
+                tc_fence_after();
+                const bool valid = r < m_end;
+                const uint64_t row_id = (uint64_t(b) * P.width + ri) * P.q_heads + qh;
+                const uint64_t id = uint64_t(split) * P.seqs * P.width * P.q_heads + row_id;
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                float* prow_o = P.part_o + id * D;
+                uint8_t* orow = P.out + uint64_t(b) * P.o_seq + uint64_t(ri) * P.o_row + uint64_t(qh) * P.o_head;
+                if (n) {
+#pragma unroll 1
+                    for (uint32_t cc = 0; cc < D; cc += 32) {
+                        uint32_t o[32];
+                        tc_ld32(col_o + cc, o);
+                        tc_wait_ld(o);
+                        if (!valid) continue;
+                        if (P.splits > 1) {
+                            float4* dst = reinterpret_cast<float4*>(prow_o + cc);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                dst[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                                     __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+                        } else {
+                            uint4* dst = reinterpret_cast<uint4*>(orow + cc * 2);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                uint32_t y[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    // A row that sees no key has a zero sum; its product is 0.
+                                    y[e] = pf_pack2<BF16>(__uint_as_float(o[8 * i + 2 * e]) * inv,
+                                                          __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
+                                }
+                                dst[i] = make_uint4(y[0], y[1], y[2], y[3]);
+                            }
+                        }
+                    }
+                }
+                if (n == 0 && valid && P.splits == 1)  // nothing to see
+                    for (uint32_t c = 0; c < D / 8; ++c) reinterpret_cast<uint4*>(orow)[c] = make_uint4(0, 0, 0, 0);
+                if (valid && P.splits > 1) P.part_ml[id] = make_float2(l == 0.f ? -INFINITY : m_used, l);
+                if (valid && P.splits == 1 && P.lse) P.lse[row_id] = l == 0.f ? -INFINITY : (m_used + log2f(l)) * kAtLn2;
+            } else {
+                ok = false;
+            }
+        }
+        if (!ok) {
+            record_error(P.status, KVM_ERR_TIMEOUT, 135);
+            *abort_flag = 1;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+}  // namespace kvmb

@@ -10,6 +10,7 @@
 #include <vector>
 
 #include "attend_launch.cuh"
+#include "attend_tc_launch.cuh"
 #include "common.cuh"
 #include "layerwise.cuh"
 #include "lse_launch.cuh"
@@ -2297,50 +2298,142 @@ int attend_common(const kvm_ctx* c, uint32_t q_heads, uint32_t kv_heads, uint32_
     return KVM_OK;
 }
 
-// Chooses the M tile and the key chunks, takes the scratch and launches. `tiles`:
-// key tiles of the longest unit.
-int attend_launch(kvm_ctx* c, AttendParams& p, uint32_t head_dim, bool bf16, int mode, bool quant, uint64_t tiles,
-                  cudaStream_t s) {
-    const uint32_t packed = p.width * p.group;
-    const int wm = packed <= 16 ? 1 : packed <= 32 ? 2 : 4;
-    p.m_tiles = (packed + 16 * wm - 1) / (16 * wm);
-    // Key chunks: the modelled time of `waves` waves of CTAs, each of its tiles' copies at
-    // the SM's share of HBM plus its start and end, and the joining of the chunks.
-    const uint32_t smem = at_smem_bytes(int(head_dim), wm, quant);
-    const uint32_t occ = std::max(1u, 227u * 1024u / (smem + 1024u));
-    const double tile_us = double(kAtKeys) * 4 * head_dim * c->num_sms * occ / 6.4e6;
-    const uint64_t units = uint64_t(p.seqs) * p.kv_heads * p.m_tiles;
-    const uint64_t rows = uint64_t(p.seqs) * p.width * p.q_heads;
-    const size_t row_bytes = size_t(head_dim) * 4 + 8;
-    const uint64_t slots = uint64_t(c->num_sms) * occ;
-    uint32_t splits = 1;
+bool attend_is(const char* name) {
+    const char* e = std::getenv("KVM_ATTEND");
+    return e && std::strcmp(e, name) == 0;
+}
+
+// Tensor maps of the tcgen05 kernel. False where TMA cannot express the operands: a
+// zero stride (one tensor for all sequences), or pages that are no multiple of 16 tokens.
+bool attend_tc_maps(const AttendParams& p, uint32_t head_dim, bool bf16, int mode, uint32_t pool_rows, AttendTcMaps* maps,
+                    uint32_t* box) {
+    TensorMapEncodeFn enc = tensor_map_encoder();
+    if (!enc) return false;
+    const CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+    const uint32_t vk = kAcUnit / (head_dim * 2);
+    auto encode = [&](CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+                      const cuuint32_t* boxes) {
+        for (int i = 0; i < rank - 1; ++i)
+            if (!strides[i] || strides[i] >= (1ull << 40)) return false;
+        return enc(m, dt, cuuint32_t(rank), const_cast<void*>(base), dims, strides, boxes, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    };
+    for (int v = 0; v < 2; ++v) {
+        const uint64_t tok = v ? p.v_tok : p.k_tok;
+        const cuuint64_t dims[4] = {head_dim, p.kv_heads, p.capacity, p.seqs};
+        const cuuint64_t strides[3] = {p.kv_heads > 1 ? (v ? p.v_head : p.k_head) : tok, tok,
+                                       p.seqs > 1 ? (v ? p.v_seq : p.k_seq) : tok};
+        const cuuint32_t boxes[4] = {64, 1, v ? vk : uint32_t(kAcKeys), 1};
+        if (!encode(v ? &maps->dv : &maps->dk, v ? p.v : p.k, 4, dims, strides, boxes)) return false;
+    }
+    if (mode == kAtWindow) return true;
+    uint32_t b = 128;
+    while (p.page_tokens % b) b >>= 1;
+    if (b < 16) return false;
+    *box = b;
+    for (int v = 0; v < 2; ++v) {
+        const cuuint64_t dims[5] = {head_dim, p.kv_heads, p.page_tokens, p.pool_slots, pool_rows};
+        const uint64_t slot = v ? p.pv_slot : p.pk_slot;
+        const cuuint64_t strides[4] = {v ? p.pv_head : p.pk_head, v ? p.pv_tok : p.pk_tok, slot,
+                                       pool_rows > 1 ? (v ? p.pv_row : p.pk_row) : slot};
+        const cuuint32_t boxes[5] = {64, 1, v ? std::min(b, vk) : b, 1, 1};
+        if (!encode(v ? &maps->pv : &maps->pk, v ? p.pv : p.pk, 5, dims, strides, boxes)) return false;
+    }
+    return true;
+}
+
+// Key chunks of a launch: the split whose modelled time is least. A wave of CTAs takes
+// its tiles' time plus the start and end of a CTA; a split adds the joining pass over
+// its partial rows.
+uint32_t attend_splits(const kvm_ctx* c, uint64_t units, uint64_t slots, uint64_t tiles, double tile_us, double cta_us,
+                       uint64_t rows, size_t row_bytes, uint32_t least) {
+    uint32_t splits = least;
     double best = 0;
-    for (uint32_t sp = 1; sp <= std::min<uint64_t>(tiles, 256); ++sp) {
-        if (sp > 1 && (units * (sp - 1) >= 4 * slots || rows * sp * row_bytes > (size_t(1) << 30))) break;
+    for (uint32_t sp = least; sp <= std::max<uint64_t>(least, std::min<uint64_t>(tiles, 256)); ++sp) {
+        if (sp > least && (units * (sp - 1) >= 4 * slots || rows * sp * row_bytes > (size_t(1) << 30))) break;
         const uint64_t waves = (units * sp + slots - 1) / slots;
-        const double t = double(waves) * (double((tiles + sp - 1) / sp) * tile_us + 3.0) +
+        const double t = double(waves) * (double((tiles + sp - 1) / sp) * tile_us + cta_us) +
                          (sp > 1 ? 3.0 + double(rows * sp * row_bytes) / 3e6 : 0.0);
-        if (sp == 1 || t < best) best = t, splits = sp;
+        if (sp == least || t < best) best = t, splits = sp;
     }
     if (const char* e = std::getenv("KVM_ATTEND_SPLITS")) {  // the tests reach the joining pass on small problems with it
         const long v = std::strtol(e, nullptr, 10);
-        if (v >= 1 && v <= 256) splits = uint32_t(v);
+        if (v >= 1 && v <= 256) splits = std::max(least, uint32_t(v));
     }
     if (c->ws_borrowed)
-        while (splits > 1 && rows * splits * row_bytes + 256 > c->ws_bytes) --splits;
-    p.splits = splits;
-    if (splits > 1) {
-        const size_t po = align256(rows * splits * head_dim * 4);
-        void* ws = nullptr;
-        KVM_TRY(ensure_attn_ws(c, po + rows * splits * 8, s, &ws));
-        p.part_o = static_cast<float*>(ws);
-        p.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(ws) + po);
+        while (splits > least && rows * splits * row_bytes + 256 > c->ws_bytes) --splits;
+    return splits;
+}
+
+int attend_scratch(kvm_ctx* c, AttendParams& p, uint32_t head_dim, cudaStream_t s) {
+    if (p.splits == 1) return KVM_OK;
+    const uint64_t rows = uint64_t(p.seqs) * p.width * p.q_heads;
+    const size_t po = align256(rows * p.splits * head_dim * 4);
+    void* ws = nullptr;
+    KVM_TRY(ensure_attn_ws(c, po + rows * p.splits * 8, s, &ws));
+    p.part_o = static_cast<float*>(ws);
+    p.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(ws) + po);
+    return KVM_OK;
+}
+
+// Chooses the kernel, its M tile and the key chunks, takes the scratch and launches.
+// `keys`: keys of the longest unit; `list_keys`: those of its page list; `tail_most`:
+// a bound on those of its tail.
+// KVM_ATTEND=mma and KVM_ATTEND=tc force a kernel (tc: KVM_ERR_UNSUPPORTED where it
+// cannot run); the tests use them.
+int attend_launch(kvm_ctx* c, AttendParams& p, uint32_t head_dim, bool bf16, int mode, bool quant, uint64_t keys,
+                  uint64_t list_keys, uint64_t tail_most, uint32_t pool_rows, cudaStream_t s) {
+    const uint32_t packed = p.width * p.group;
+    const uint64_t rows = uint64_t(p.seqs) * p.width * p.q_heads;
+    const size_t row_bytes = size_t(head_dim) * 4 + 8;
+    const bool force_tc = attend_is("tc");
+    if (!quant && (packed > 64 || force_tc) && !attend_is("mma")) {
+        AttendTcMaps maps;
+        std::memset(&maps, 0, sizeof maps);
+        uint32_t box = 0;
+        if (attend_tc_maps(p, head_dim, bf16, mode, pool_rows, &maps, &box)) {
+            const uint32_t m = 128u * ac_mt(int(head_dim));
+            p.m_tiles = (packed + m - 1) / m;
+            // One CTA's chunk touches at most kAcTable pages
+            uint32_t least = 1;
+            bool too_many = false;
+            if (mode == kAtTree) {
+                // (chunks are even shares of all tiles, the longest tail's among them).
+                const uint64_t most = uint64_t(kAcTable - 2) * p.page_tokens / kAcKeys;
+                const uint64_t all = (list_keys + kAcKeys - 1) / kAcKeys + (tail_most + kAcKeys - 1) / kAcKeys;
+                if (all / most >= 256) too_many = true;
+                least = uint32_t(all / most + 1);
+            }
+            if (!too_many) {
+                const uint64_t tiles = (keys + kAcKeys - 1) / kAcKeys + 1;
+                p.splits = attend_splits(c, uint64_t(p.seqs) * p.kv_heads * p.m_tiles, uint64_t(c->num_sms), tiles, 1.6, 5.0,
+                                         rows, row_bytes, least);
+                KVM_TRY(attend_scratch(c, p, head_dim, s));
+                KVM_TRY(bf16 ? launch_attend_tc_t<true>(c, maps, p, head_dim, mode, box, s)
+                             : launch_attend_tc_t<false>(c, maps, p, head_dim, mode, box, s));
+                return launch_attend_combine(c, p, head_dim, bf16, s);
+            }
+        }
     }
+    if (force_tc) return KVM_ERR_UNSUPPORTED;
+    const int wm = packed <= 16 ? 1 : packed <= 32 ? 2 : 4;
+    p.m_tiles = (packed + 16 * wm - 1) / (16 * wm);
+    const uint32_t smem = at_smem_bytes(int(head_dim), wm, quant);
+    const uint32_t occ = std::max(1u, 227u * 1024u / (smem + 1024u));
+    const double tile_us = double(kAtKeys) * 4 * head_dim * c->num_sms * occ / 6.4e6;
+    p.splits = attend_splits(c, uint64_t(p.seqs) * p.kv_heads * p.m_tiles, uint64_t(c->num_sms) * occ,
+                             (keys + kAtKeys - 1) / kAtKeys + 1, tile_us, 3.0, rows, row_bytes, 1);
+    KVM_TRY(attend_scratch(c, p, head_dim, s));
+    int rc;
     switch (head_dim) {
-        case 64: return bf16 ? launch_attend_t<64, true>(c, p, mode, quant, wm, s) : launch_attend_t<64, false>(c, p, mode, quant, wm, s);
-        case 128: return bf16 ? launch_attend_t<128, true>(c, p, mode, quant, wm, s) : launch_attend_t<128, false>(c, p, mode, quant, wm, s);
-        default: return bf16 ? launch_attend_t<256, true>(c, p, mode, quant, wm, s) : launch_attend_t<256, false>(c, p, mode, quant, wm, s);
+        case 64: rc = bf16 ? launch_attend_t<64, true>(c, p, mode, quant, wm, s) : launch_attend_t<64, false>(c, p, mode, quant, wm, s); break;
+        case 128: rc = bf16 ? launch_attend_t<128, true>(c, p, mode, quant, wm, s) : launch_attend_t<128, false>(c, p, mode, quant, wm, s); break;
+        default: rc = bf16 ? launch_attend_t<256, true>(c, p, mode, quant, wm, s) : launch_attend_t<256, false>(c, p, mode, quant, wm, s); break;
     }
+    if (rc != KVM_OK) return rc;
+    return launch_attend_combine(c, p, head_dim, bf16, s);
 }
 
 // Device side of a layout's planes (host fields unused).
@@ -2378,12 +2471,11 @@ int kvm_window_attention(kvm_ctx* c, const kvm_window_desc* d, const kvm_rows* q
     p.seq_rows = d->seq_rows;
     p.window = d->window;
     p.sinks = d->sinks;
-    // Keys of the longest M tile (at most 64 packed rows).
-    const uint64_t reach = std::min<uint64_t>(uint64_t(d->window) + 64, p.capacity);
-    const uint64_t tiles = (std::min<uint64_t>(d->sinks, p.capacity) + kAtKeys - 1) / kAtKeys + (reach + kAtKeys - 1) / kAtKeys;
-    const uint64_t most = (uint64_t(p.capacity) + kAtKeys - 1) / kAtKeys + 1;
+    // Keys of the longest unit: the sinks, the window and the rows of an M tile (at most 256 packed).
+    const uint64_t reach = uint64_t(d->window) + std::min<uint64_t>(d->width, 256 / p.group + 2);
+    const uint64_t keys = std::min<uint64_t>(std::min<uint64_t>(d->sinks, p.capacity) + reach, p.capacity);
     DeviceGuard guard(c->device);
-    return attend_launch(c, p, d->head_dim, d->type == KVM_BF16, kAtWindow, false, std::min(tiles, most),
+    return attend_launch(c, p, d->head_dim, d->type == KVM_BF16, kAtWindow, false, keys, 0, 0, 0,
                          static_cast<cudaStream_t>(stream));
 }
 
@@ -2446,9 +2538,9 @@ int kvm_tree_attention(kvm_ctx* c, const kvm_pool* pool, const kvm_tree_desc* d,
     p.seq_rows = d->seq_rows;
     p.tree = d->tree, p.tree_seq = d->tree_stride, p.tree_words = d->tree_words;
     const uint64_t dense = d->seq_recent ? std::min<uint64_t>(p.capacity, uint64_t(d->page_tokens) + d->nodes) : uint64_t(d->recent) + d->nodes;
-    const uint64_t tiles = (list * d->page_tokens + kAtKeys - 1) / kAtKeys + (dense + kAtKeys - 1) / kAtKeys;
     DeviceGuard guard(c->device);
-    return attend_launch(c, p, d->head_dim, d->type == KVM_BF16, kAtTree, quant, tiles, static_cast<cudaStream_t>(stream));
+    return attend_launch(c, p, d->head_dim, d->type == KVM_BF16, kAtTree, quant, list * d->page_tokens + dense,
+                         list * d->page_tokens, d->seq_recent ? p.capacity : dense, view.rows, static_cast<cudaStream_t>(stream));
 }
 
 int kvm_tree_mask(const int32_t* parents, uint32_t nodes, uint32_t tree_words, uint32_t* words) {

@@ -142,7 +142,11 @@ CASES = [
 
 @pytest.mark.parametrize("case", CASES)
 @pytest.mark.parametrize("splits", ["", "1", "4"])
-def test_tree(ctx, monkeypatch, case, splits):
+@pytest.mark.parametrize("kernel", ["", "mma", "tc"])
+def test_tree(ctx, monkeypatch, case, splits, kernel):
+    if kernel == "tc" and case[5] % 16:
+        pytest.skip("the tcgen05 kernel takes pages of a multiple of 16 tokens")
+    monkeypatch.setenv("KVM_ATTEND", kernel)
     if splits:
         monkeypatch.setenv("KVM_ATTEND_SPLITS", splits)
     p = Problem(ctx, 11, *case, garbage=True)
@@ -197,7 +201,9 @@ def test_rows_that_see_nothing(ctx):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-def test_a_poisoned_node_stays_with_those_that_see_it(ctx, dtype):
+@pytest.mark.parametrize("kernel", ["mma", "tc"])
+def test_a_poisoned_node_stays_with_those_that_see_it(ctx, monkeypatch, dtype, kernel):
+    monkeypatch.setenv("KVM_ATTEND", kernel)
     p = Problem(ctx, 16, 1, 40, 6, 2, 64, 32, 10, 4, [300], [9], dtype)
     j = 17
     for x in p.tail_d + p.tail:

@@ -60,7 +60,9 @@ CASES = [
 
 @pytest.mark.parametrize("case", CASES)
 @pytest.mark.parametrize("splits", ["", "1", "3"])
-def test_window(ctx, monkeypatch, case, splits):
+@pytest.mark.parametrize("kernel", ["", "mma", "tc"])
+def test_window(ctx, monkeypatch, case, splits, kernel):
+    monkeypatch.setenv("KVM_ATTEND", kernel)
     seqs, width, hq, hkv, dim, bases, window, sinks, dtype = case
     if splits:
         monkeypatch.setenv("KVM_ATTEND_SPLITS", splits)
@@ -72,9 +74,11 @@ def test_window(ctx, monkeypatch, case, splits):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("dim,hq,hkv,width", [(64, 12, 2, 19), (128, 16, 4, 1), (128, 8, 2, 40), (256, 6, 1, 3)])
-def test_masked_garbage_does_not_reach_rows(ctx, dtype, dim, hq, hkv, width):
+@pytest.mark.parametrize("dim,hq,hkv,width", [(64, 12, 2, 19), (128, 16, 4, 1), (128, 8, 2, 40), (256, 6, 1, 3), (256, 24, 4, 30)])
+@pytest.mark.parametrize("kernel", ["mma", "tc"])
+def test_masked_garbage_does_not_reach_rows(ctx, monkeypatch, dtype, dim, hq, hkv, width, kernel):
     """NaN and infinities in keys that no row sees, and in keys that only some rows of a tile see."""
+    monkeypatch.setenv("KVM_ATTEND", kernel)
     base, window, sinks, cap = 150, 40, 2, 260
     q, k, v = make(2, 1, width, hq, hkv, dim, cap, dtype)
     see = visible(base, width, cap, window, sinks)
