@@ -217,10 +217,9 @@ SIGNATURES = {
     "kvm_ipc_close": ([_i, _vp], _i),
     "kvm_prefill_attention": ([_vp, C.POINTER(PrefillDesc), _vp, _u64, _u64, C.POINTER(KCache), C.POINTER(KCache),
                                _vp, _u64, _u64, _vp, _vp], _i),
-    "kvm_window_attention": ([_vp, C.POINTER(WindowDesc), C.POINTER(Rows), C.POINTER(KCache), C.POINTER(KCache),
-                              C.POINTER(Rows), _vp, _vp], _i),
-    "kvm_tree_attention": ([_vp, _vp, C.POINTER(TreeDesc), C.POINTER(StageLayout), C.POINTER(Rows), C.POINTER(KCache),
-                            C.POINTER(KCache), C.POINTER(Rows), _vp, _vp], _i),
+    # descriptors as bytes or ctypes.byref(structure): WindowDesc / TreeDesc, Rows, KCache, KCache, Rows
+    "kvm_window_attention": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp], _i),
+    "kvm_tree_attention": ([_vp, _vp, _vp, C.POINTER(StageLayout), _vp, _vp, _vp, _vp, _vp, _vp], _i),
     "kvm_tree_mask": ([_vp, _u32, _u32, _vp], _i),
     "kvm_pool_fork": ([_vp, _vp, C.POINTER(StageLayout), _vp, _vp, _u32, _u32, _u32, _vp], _i),
     "kvm_pool_copy": ([_vp, _vp, C.POINTER(StageLayout), _vp, _u32, _u32, _vp], _i),

@@ -693,6 +693,7 @@ __global__ void __launch_bounds__(kAtThreads) attend_mma_kernel(const __grid_con
         }
     }
     at_wait<0>();
+    grid_release();
     __syncthreads();
 
     // ---- the warps' parts of each row, merged through shared memory ----
@@ -765,6 +766,7 @@ template <int D, bool BF16>
 __global__ void __launch_bounds__(256) attend_combine_kernel(const __grid_constant__ AttendParams P) {
     __shared__ float acc_s[8][D];
     __shared__ float2 ml_s[8];
+    grid_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
     const uint64_t row_id = blockIdx.x, stride = uint64_t(P.seqs) * P.width * P.q_heads;
     const uint32_t qh = uint32_t(row_id % P.q_heads);
@@ -787,7 +789,7 @@ __global__ void __launch_bounds__(256) attend_combine_kernel(const __grid_consta
     float m = -INFINITY, l = 0.f;
 #pragma unroll 4
     for (uint32_t c = warp; c < P.splits; c += nw) {
-        const float2 ml = __ldg(P.part_ml + c * stride + row_id);
+        const float2 ml = P.part_ml[c * stride + row_id];
         const float* src = P.part_o + (c * stride + row_id) * D + lane * E;
         float x[E];
         if constexpr (E == 2) {

@@ -37,9 +37,10 @@ int launch_attend_combine_t(kvm_ctx* c, const AttendParams& p, cudaStream_t s) {
     const uint64_t rows = uint64_t(p.seqs) * p.width * p.q_heads;
     if (rows > 0x7fffffffull) return KVM_ERR_LENGTH;
     const uint32_t warps = p.splits < 8 ? (p.splits < 4 ? 2 : 4) : 8;
-    attend_combine_kernel<D, BF16><<<uint32_t(rows), warps * 32, 0, s>>>(p);
     ++c->launches;
-    return cudaGetLastError() == cudaSuccess ? KVM_OK : KVM_ERR_CUDA;
+    if (launch_early(attend_combine_kernel<D, BF16>, uint32_t(rows), warps * 32, 0, s, p) == cudaSuccess) return KVM_OK;
+    cudaGetLastError();
+    return KVM_ERR_CUDA;
 }
 
 // The joining pass, where the keys were split.

@@ -575,6 +575,7 @@ const int rec = int(recent) - int(a);  // keys below are recent tokens, key rec 
                 mbar_arrive(&p_full[slot]);
             }
         }
+        grid_release();
         const bool go = __shfl_sync(0xffffffffu, (ok && !*abort_flag) ? 1 : 0, 0) != 0;
         if (go) {
             const uint32_t wl = (n - 1) * MT + m;

@@ -31,6 +31,29 @@ inline cudaError_t smem_attr(const void* fn, int bytes) {
     return e;
 }
 
+// Waits until the kernel before it in the stream is done (its launch allowed this one
+// to start early), and lets the next one start early.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Launches `fn` so that it may start before the kernel ahead of it in the stream has
+// ended (programmatic dependent launch); `fn` waits with griddepcontrol.wait before it
+// touches what that kernel writes.
+template <typename... P, typename... A>
+inline cudaError_t launch_early(void (*fn)(P...), uint32_t grid, uint32_t block, size_t smem, cudaStream_t s, const A&... args) {
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, fn, args...);
+}
+
 // Upper bound on polls of one mbarrier / flag before a kernel gives up,
 // records KVM_ERR_TIMEOUT and unwinds (a few seconds at the longest).
 constexpr uint32_t kSpinLimit = 1u << 22;

@@ -2597,10 +2597,10 @@ int copy_pages(kvm_ctx* c, const kvm_pool* pool, const PageGroups& gr, const Gat
     if (bulk) {
         KVM_CUDA(smem_attr(reinterpret_cast<const void*>(page_copy_kernel), int(kPcSmem)));
         const uint32_t grid = uint32_t(std::min<uint64_t>(most, ctas ? ctas : uint32_t(c->num_sms)));
-        page_copy_kernel<<<grid, 32, kPcSmem, s>>>(gr, pc);
+        KVM_CUDA(launch_early(page_copy_kernel, grid, kPcThreads, kPcSmem, s, gr, pc));
     } else {
         const uint32_t grid = uint32_t(std::min<uint64_t>(most, ctas ? ctas : uint32_t(c->num_sms) * 8));
-        page_copy_plain_kernel<<<grid, kPcPlainThreads, 0, s>>>(gr, pc);
+        KVM_CUDA(launch_early(page_copy_plain_kernel, grid, kPcPlainThreads, 0, s, gr, pc));
     }
     ++c->launches;
     KVM_CUDA(cudaGetLastError());

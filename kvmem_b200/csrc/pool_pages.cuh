@@ -19,6 +19,7 @@ constexpr uint32_t kPcChunk = 16384;
 constexpr uint32_t kPcStages = 12;
 constexpr int kPcPlanThreads = 256;
 constexpr int kPcPlainThreads = 256;
+constexpr int kPcThreads = int(kPcStages) * 32;
 constexpr uint32_t kPcSmem = kPcStages * kPcChunk + kPcStages * 8 + (kPcGroups + 1) * 4;
 
 struct PageGroups {
@@ -43,6 +44,7 @@ struct PageRows {
 // destination): the source's slots whose page is below page_end.
 __global__ void __launch_bounds__(kPcPlanThreads) fork_plan_kernel(PoolView pool, const __grid_constant__ PageGroups gr,
                                                                    uint32_t page_end, int2* moves, uint32_t* n_moves) {
+    grid_release();
     __shared__ uint32_t warp_sums[32];
     const int tid = threadIdx.x;
     const uint32_t d = blockIdx.x, dst = gr.dst_row[d];
@@ -81,6 +83,7 @@ __global__ void __launch_bounds__(kPcPlanThreads) fork_plan_kernel(PoolView pool
 // slot, destination slot}, n_moves[i] = 1, or 0 where it is left out.
 __global__ void __launch_bounds__(kPcPlanThreads) copy_plan_kernel(PoolView pool, const __grid_constant__ PageItems it,
                                                                    int2* moves, uint32_t* n_moves, DeviceStatus* status) {
+    grid_release();
     __shared__ uint32_t warp_sums[32];
     __shared__ uint32_t free_slot[kPcPlanThreads];
     const int tid = threadIdx.x;
@@ -169,6 +172,7 @@ __global__ void __launch_bounds__(kPcPlanThreads) free_kernel(PoolView pool, con
 // With c resident pages, the k-th resident slot >= c goes to the k-th free slot < c.
 __global__ void __launch_bounds__(kPcPlanThreads) compact_plan_kernel(PoolView pool, const __grid_constant__ PageGroups gr,
                                                                       int2* moves, uint32_t* n_moves, uint32_t* used) {
+    grid_release();
     __shared__ uint32_t warp_sums[32];
     __shared__ uint32_t sh_n;
     const int tid = threadIdx.x;
@@ -272,49 +276,52 @@ __device__ __forceinline__ uint8_t* page_at(const GatherLayout& lay, uint32_t pl
     return lay.dev_base[plane] + uint64_t(row) * lay.dev_row_stride[plane] + uint64_t(slot) * lay.dev_slot_stride[plane];
 }
 
-__global__ void __launch_bounds__(32) page_copy_kernel(const __grid_constant__ PageGroups gr,
-                                                       const __grid_constant__ PageCopy pc) {
+// One thread of each warp owns a stage: load, store to every destination, next chunk.
+// The address of a chunk (a search in shared memory and a load of its move) is worked
+// out while the chunk before it is on its way.
+__global__ void __launch_bounds__(kPcThreads) page_copy_kernel(const __grid_constant__ PageGroups gr,
+                                                               const __grid_constant__ PageCopy pc) {
     extern __shared__ __align__(128) uint8_t ring[];
     uint64_t* full = reinterpret_cast<uint64_t*>(ring + kPcStages * kPcChunk);
     uint32_t* sums = reinterpret_cast<uint32_t*>(full + kPcStages);
-    page_prefix(gr, pc.n_moves, sums);
+    const uint32_t warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < kPcStages; ++s) mbar_init(&full[s], 1);
         mbar_fence_init();
     }
-    __syncwarp();
-    if (threadIdx.x != 0) return;
+    grid_wait();
+    if (warp == 0) page_prefix(gr, pc.n_moves, sums);
+    __syncthreads();
+    if (threadIdx.x & 31) return;
+    // The plan's tables and lists are generic-proxy writes of another kernel; the pages are
+    // read and written by the async proxy only.
+    asm volatile("fence.proxy.async;" ::: "memory");
     const uint64_t items = uint64_t(sums[gr.n]) * (pc.chunks[0] + pc.chunks[1]);
-    const uint64_t n = items > blockIdx.x ? (items - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
+    const uint64_t step = uint64_t(gridDim.x) * kPcStages;
     const uint64_t policy = policy_evict_first();
-    constexpr uint32_t kLag = kPcStages / 2;  // loads in flight; the other stages are being stored
-    for (uint64_t k = 0; k < n + kLag; ++k) {
-        if (k < n) {
-            // The stage's previous chunk was stored kPcStages - kLag store groups ago.
-            asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kPcStages - kLag - 1) : "memory");
-            const uint32_t s = uint32_t(k % kPcStages);
-            const PageChunk x = page_chunk(gr, pc, sums, blockIdx.x + k * gridDim.x);
-            mbar_arrive_expect_tx(&full[s], x.bytes);
-            bulk_g2s(ring + s * kPcChunk, page_at(pc.lay, x.plane, gr.src_row[x.g], uint32_t(x.move.x)) + x.offset, x.bytes,
-                     &full[s], policy);
+    uint8_t* stage = ring + warp * kPcChunk;
+    uint64_t i = blockIdx.x + uint64_t(warp) * gridDim.x;
+    if (i >= items) return;
+    PageChunk x = page_chunk(gr, pc, sums, i);
+    for (uint32_t phase = 0;; phase ^= 1) {
+        mbar_arrive_expect_tx(&full[warp], x.bytes);
+        bulk_g2s(stage, page_at(pc.lay, x.plane, gr.src_row[x.g], uint32_t(x.move.x)) + x.offset, x.bytes, &full[warp], policy);
+        const PageChunk y = x;
+        i += step;
+        if (i < items) x = page_chunk(gr, pc, sums, i);
+        if (!mbar_wait(&full[warp], phase)) {
+            record_error(pc.status, KVM_ERR_TIMEOUT, 114);
+            mbar_wait(&full[warp], phase);  // the load lands before the shared memory is freed
+            break;
         }
-        if (k >= kLag) {
-            const uint64_t j = k - kLag;
-            const uint32_t s = uint32_t(j % kPcStages);
-            if (!mbar_wait(&full[s], uint32_t(j / kPcStages) & 1)) {
-                record_error(pc.status, KVM_ERR_TIMEOUT, 114);
-                // The loads already started land before the shared memory is freed.
-                for (uint64_t r = j; r < min(n, k + 1); ++r) mbar_wait(&full[r % kPcStages], uint32_t(r / kPcStages) & 1);
-                break;
-            }
-            const PageChunk x = page_chunk(gr, pc, sums, blockIdx.x + j * gridDim.x);
-            for (uint32_t d = gr.first[x.g]; d < gr.first[x.g + 1]; ++d)
-                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(
-                                 page_at(pc.lay, x.plane, gr.dst_row[d], uint32_t(x.move.y)) + x.offset),
-                             "r"(smem_u32(ring + s * kPcChunk)), "r"(x.bytes)
-                             : "memory");
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-        }
+        for (uint32_t d = gr.first[y.g]; d < gr.first[y.g + 1]; ++d)
+            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(
+                             page_at(pc.lay, y.plane, gr.dst_row[d], uint32_t(y.move.y)) + y.offset),
+                         "r"(smem_u32(stage)), "r"(y.bytes)
+                         : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        if (i >= items) break;
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     }
     asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
@@ -323,6 +330,7 @@ __global__ void __launch_bounds__(32) page_copy_kernel(const __grid_constant__ P
 __global__ void __launch_bounds__(kPcPlainThreads) page_copy_plain_kernel(const __grid_constant__ PageGroups gr,
                                                                           const __grid_constant__ PageCopy pc) {
     __shared__ uint32_t sums[kPcGroups + 1];
+    grid_wait();
     if (threadIdx.x < 32) page_prefix(gr, pc.n_moves, sums);
     __syncthreads();
     const uint64_t items = uint64_t(sums[gr.n]) * (pc.chunks[0] + pc.chunks[1]);

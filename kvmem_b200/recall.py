@@ -14,7 +14,9 @@ Two layers:
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
+import struct
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -22,6 +24,7 @@ import torch
 
 from . import _abi as A
 
+_ATTN_TYPES = {torch.float16: A.F16, torch.bfloat16: A.BF16}
 _TORCH_QTYPE = {torch.float32: A.F32, torch.float16: A.F16, torch.bfloat16: A.BF16}
 
 
@@ -31,60 +34,79 @@ def _stream_ptr(stream) -> int:
     return stream.cuda_stream
 
 
-def _stream_on(device: int, stream) -> "torch.cuda.Stream":
+def _stream_on(device: int, stream) -> int:
     """The given stream, else the current stream of `device` (whichever device is current)."""
-    return stream if stream is not None else torch.cuda.current_stream(device)
+    return (stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream
 
 
-def _on_device(device: int, where: str, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and (t.device.type != "cuda" or t.device.index != device):
-            raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{where}: {name} is on {t.device}, the context on cuda:{device}")
+def _bad(where: str, what: str, code: int = A.ERR_INVALID_ARGUMENT) -> A.KvmError:
+    return A.KvmError(code, f"{where}: {what}")
 
 
-def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
-    return None if t is None else t.data_ptr()
+def _on_device(device: int, where: str, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise _bad(where, f"a tensor is on {t.device}, the context on cuda:{device}")
 
 
-def _u64_arg(x, device: int, n: int, where: str):
-    """(scalar, device pointer) of a per-sequence argument: an int, or an int64 tensor [n]."""
-    return _seq_arg(x, device, n, where, torch.int64)
-
-
-def _u32_arg(x, device: int, n: int, where: str):
-    """(scalar, device pointer) of a per-sequence argument: an int, or an int32 tensor [n]."""
-    return _seq_arg(x, device, n, where, torch.int32)
-
-
-def _seq_arg(x, device, n, where, dtype):
+def _seq_arg(x, device: int, n: int, where: str, dtype):
+    """(scalar, device address) of a per-sequence argument: an int, or a tensor [n] of `dtype` on the device."""
     if isinstance(x, torch.Tensor):
-        _on_device(device, where, argument=x)
-        if x.dtype != dtype or x.dim() != 1 or x.shape[0] < n or not x.is_contiguous():
-            raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{where}: a per-sequence tensor is contiguous {dtype} [{n}]")
+        if x.dtype is not dtype or x.get_device() != device or x.dim() != 1 or len(x) < n or not x.is_contiguous():
+            raise _bad(where, f"a per-sequence tensor is contiguous {dtype} [{n}] on cuda:{device}")
         return 0, x.data_ptr()
     if x < 0:
-        raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{where}: negative argument")
-    return int(x), None
+        raise _bad(where, "negative argument")
+    return int(x), 0
 
 
-def _rows4(t: torch.Tensor, where: str) -> A.Rows:
-    """kvm_rows of a [sequence][row][head][dim] tensor (dim contiguous)."""
-    if t.stride(3) != 1 and t.shape[3] != 1:
-        raise A.KvmError(A.ERR_UNSUPPORTED, f"{where}: the last dimension must be contiguous")
-    es = t.element_size()
-    # The stride of a dimension of one element says nothing: it is taken as one row.
-    st = [(t.stride(i) if t.shape[i] > 1 else t.shape[3]) * es for i in range(3)]
-    return A.Rows(t.data_ptr(), *st)
+# The attention calls' C structures, packed in one go (native alignment, as ctypes lays them out; a ctypes.Structure of
+# as many fields takes several times as long to fill, and a decode step makes this call once per layer).
+_ROWS = struct.Struct("@PQQQ")
+_KCACHE = struct.Struct("@PiIQQQQ")
+_WINDOW = struct.Struct("@3Ii4IQPPfI")
+_TREE = struct.Struct("@3I3i6IQ5P2IPQfI")
+assert [x.size for x in (_ROWS, _KCACHE, _WINDOW, _TREE)] == [C.sizeof(x) for x in (A.Rows, A.KCache, A.WindowDesc, A.TreeDesc)]
 
 
-def _dense4(t: torch.Tensor, where: str) -> A.KCache:
-    """kvm_kcache of a [sequence][token][head][dim] tensor (dim contiguous)."""
-    r = _rows4(t, where)
-    kc = A.KCache()
-    kc.data, kc.type = r.data, _TORCH_QTYPE[t.dtype]
-    kc.layer_stride, kc.token_stride, kc.head_stride = r.seq_stride, r.row_stride, r.head_stride
-    kc.capacity_tokens = t.shape[1]
-    return kc
+def _view4(t: torch.Tensor, shape, where: str):
+    """(address, byte strides of sequence, row and head) of a 16-bit [sequence][row][head][dim] tensor (dim contiguous).
+    The stride of a dimension of one element says nothing: it is taken as one row."""
+    a, b, c, d = t.stride()
+    n0, n1, n2, dim = shape
+    if d != 1 and dim != 1:
+        raise _bad(where, "the last dimension must be contiguous", A.ERR_UNSUPPORTED)
+    return t.data_ptr(), 2 * (a if n0 > 1 else dim), 2 * (b if n1 > 1 else dim), 2 * (c if n2 > 1 else dim)
+
+
+def _attention_args(where: str, device: int, q, k, v, out, lse, want_lse, stream):
+    """Checks of an attention call and its tensors as C structures: (out, lse, its address, type, q shape, KV heads,
+    q, k, v, out). Outputs that are not given are allocated for the stream of the call."""
+    dtype = q.dtype
+    t = _ATTN_TYPES.get(dtype)
+    qs, ks = q.shape, k.shape
+    if t is None or len(qs) != 4 or len(ks) != 4:
+        raise _bad(where, "q, k, v are 4-D, q fp16 or bf16")
+    if k.dtype is not dtype or v.dtype is not dtype or v.shape != ks or ks[0] != qs[0] or ks[3] != qs[3]:
+        raise _bad(where, "k and v do not match q")
+    if q.get_device() != device or k.get_device() != device or v.get_device() != device:
+        raise _bad(where, f"q, k and v are on cuda:{device}")
+    if out is None or (want_lse and lse is None):
+        with torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext():
+            if out is None:
+                out = q.new_empty(qs)
+            if lse is None and want_lse:
+                lse = q.new_empty(qs[:3], dtype=torch.float32)
+    if out.shape != qs or out.dtype is not dtype or out.get_device() != device:
+        raise _bad(where, "out does not match q")
+    if lse is not None and (lse.shape != qs[:3] or lse.dtype is not torch.float32 or not lse.is_contiguous() or
+                            lse.get_device() != device):
+        raise _bad(where, "lse is contiguous float32 [seqs][rows][q_heads]")
+    kp, k0, k1, k2 = _view4(k, ks, where)
+    vp, v0, v1, v2 = _view4(v, ks, where)
+    return (out, lse, None if lse is None else lse.data_ptr(), t, qs, ks[2], _ROWS.pack(*_view4(q, qs, where)),
+            _KCACHE.pack(kp, t, 0, k0, k1, k2, ks[1]), _KCACHE.pack(vp, t, 0, v0, v1, v2, ks[1]),
+            _ROWS.pack(*_view4(out, qs, where)))
 
 
 class _DeviceTable:
@@ -258,24 +280,20 @@ class RecallContext:
         are multiples of 16 bytes. base: int, or int64 tensor [seqs] on the device; rows: int32 tensor [seqs], the
         rows used per sequence (the others keep what `out` and `lse` hold).
         Returns (out like q, lse [seqs][width][q_heads] f32 or None)."""
-        w = "kvm_window_attention"
+        w, dev = "kvm_window_attention", self.device
         flat = q.dim() == 3
         if flat:
             q, k, v = q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0)
             out = None if out is None else out.unsqueeze(0)
             lse = None if lse is None else lse.unsqueeze(0)
-        _on_device(self.device, w, q=q, k=k, v=v, out=out, lse=lse)
-        out, lse = _attention_out(w, q, k, v, out, lse, want_lse, _stream_on(self.device, stream))
-        B, W, Hq, D = q.shape
-        d = A.WindowDesc()
-        d.q_heads, d.kv_heads, d.head_dim, d.type = Hq, k.shape[2], D, _TORCH_QTYPE[q.dtype]
-        d.seqs, d.width, d.window, d.sinks, d.scale = B, W, min(window, 0xFFFFFFFF), min(sinks, 0xFFFFFFFF), scale
-        d.base, d.seq_base = _u64_arg(base, self.device, B, w)
-        if rows is not None:
-            d.seq_rows = _u32_arg(rows, self.device, B, w)[1]
-        qq, kk, vv, oo = _rows4(q, w), _dense4(k, w), _dense4(v, w), _rows4(out, w)
-        A.check(self.lib.kvm_window_attention(self.h, C.byref(d), C.byref(qq), C.byref(kk), C.byref(vv), C.byref(oo),
-                                              _ptr(lse), _stream_on(self.device, stream).cuda_stream), w)
+        out, lse, lse_p, t, (B, W, Hq, D), hkv, qq, kk, vv, oo = _attention_args(w, dev, q, k, v, out, lse, want_lse, stream)
+        base, seq_base = _seq_arg(base, dev, B, w, torch.int64)
+        seq_rows = 0 if rows is None else _seq_arg(rows, dev, B, w, torch.int32)[1]
+        d = _WINDOW.pack(Hq, hkv, D, t, B, W, min(window, 0xFFFFFFFF), min(sinks, 0xFFFFFFFF), base, seq_base, seq_rows,
+                         scale, 0)
+        rc = self.lib.kvm_window_attention(self.h, d, qq, kk, vv, oo, lse_p, _stream_on(dev, stream))
+        if rc:
+            A.check(rc, w)
         if flat:
             return out[0], (None if lse is None else lse[0])
         return out, lse
@@ -539,36 +557,33 @@ class ResidencyPool:
         page. tokens: history length, int or int64 tensor [seqs]; recent: int or int32 tensor [seqs]; tree: int32
         tensor [nodes][words] or [seqs][nodes][words] (tree_mask), None for a chain; rows: int32 tensor [seqs], nodes
         used. k_type / v_type: type of the pages (default: q's). Returns (out like q, lse [seqs][nodes][q_heads])."""
-        w = "kvm_tree_attention"
-        dev = self.ctx.device
-        _on_device(dev, w, q=q, tail_k=tail_k, tail_v=tail_v, out=out, lse=lse, sel_ids=sel_ids, sel_n=sel_n, tree=tree)
-        out, lse = _attention_out(w, q, tail_k, tail_v, out, lse, want_lse, _stream_on(dev, stream))
-        R, N, Hq, D = q.shape
-        t = _TORCH_QTYPE[q.dtype]
-        d = A.TreeDesc()
-        d.q_heads, d.kv_heads, d.head_dim, d.type = Hq, tail_k.shape[2], D, t
-        d.k_type, d.v_type = t if k_type is None else k_type, t if v_type is None else v_type
-        d.seqs, d.nodes, d.row0, d.row_step = R, N, row0, row_step
-        d.page_tokens, d.scale = page_tokens, scale
-        d.tokens, d.seq_tokens = _u64_arg(tokens, dev, R, w)
-        d.recent, d.seq_recent = _u32_arg(recent, dev, R, w)
-        if rows is not None:
-            d.seq_rows = _u32_arg(rows, dev, R, w)[1]
+        w, dev = "kvm_tree_attention", self.ctx.device
+        out, lse, lse_p, t, (R, N, Hq, D), hkv, qq, kk, vv, oo = _attention_args(w, dev, q, tail_k, tail_v, out, lse, want_lse,
+                                                                                 stream)
+        tokens, seq_tokens = _seq_arg(tokens, dev, R, w, torch.int64)
+        recent, seq_recent = _seq_arg(recent, dev, R, w, torch.int32)
+        ids = ns = stride = words = tree_p = tree_stride = 0
         if sel_ids is not None:
-            if sel_n is None or sel_ids.dim() != 2 or sel_ids.shape[0] < R or sel_ids.element_size() != 4 or \
-                    (sel_ids.shape[1] > 1 and sel_ids.stride(1) != 1) or (R > 1 and sel_ids.stride(0) < sel_ids.shape[1]):
-                raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{w}: sel_ids is int32 [seqs][.] with sel_n [seqs]")
-            d.sel_ids, d.sel_n = sel_ids.data_ptr(), _u32_arg(sel_n, dev, R, w)[1]
-            d.sel_stride = sel_ids.stride(0) if R > 1 else sel_ids.shape[1]
+            n0, width = sel_ids.shape if sel_ids.dim() == 2 else (0, 0)
+            stride = sel_ids.stride(0) if n0 > 1 else width
+            if sel_n is None or n0 < R or sel_ids.element_size() != 4 or stride < width or \
+                    (width > 1 and sel_ids.stride(1) != 1) or sel_ids.get_device() != dev:
+                raise _bad(w, "sel_ids is int32 [seqs][.] on the device, with sel_n [seqs]")
+            ids, ns = sel_ids.data_ptr(), _seq_arg(sel_n, dev, R, w, torch.int32)[1]
         if tree is not None:
-            if tree.element_size() != 4 or not tree.is_contiguous() or tree.dim() not in (2, 3) or \
-                    tree.shape[-2] != N or (tree.dim() == 3 and tree.shape[0] != R):
-                raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{w}: tree is contiguous int32 [nodes][words] or [seqs][nodes][words]")
-            d.tree, d.tree_words = tree.data_ptr(), tree.shape[-1]
-            d.tree_stride = N * tree.shape[-1] if tree.dim() == 3 else 0
-        qq, kk, vv, oo = _rows4(q, w), _dense4(tail_k, w), _dense4(tail_v, w), _rows4(out, w)
-        A.check(self.ctx.lib.kvm_tree_attention(self.ctx.h, self.h, C.byref(d), C.byref(layout), C.byref(qq), C.byref(kk),
-                                                C.byref(vv), C.byref(oo), _ptr(lse), _stream_on(dev, stream).cuda_stream), w)
+            shape = tree.shape
+            if tree.element_size() != 4 or not tree.is_contiguous() or tree.get_device() != dev or \
+                    shape[:-1] not in ((N,), (R, N)):
+                raise _bad(w, "tree is contiguous int32 [nodes][words] or [seqs][nodes][words] on the device")
+            words = shape[-1]
+            tree_p, tree_stride = tree.data_ptr(), (N * words if len(shape) == 3 else 0)
+        seq_rows = 0 if rows is None else _seq_arg(rows, dev, R, w, torch.int32)[1]
+        d = _TREE.pack(Hq, hkv, D, t, t if k_type is None else k_type, t if v_type is None else v_type, R, N, row0, row_step,
+                       page_tokens, recent, tokens, seq_tokens, seq_recent, seq_rows, ids, ns, stride, words, tree_p,
+                       tree_stride, scale, 0)
+        rc = self.ctx.lib.kvm_tree_attention(self.ctx.h, self.h, d, layout, qq, kk, vv, oo, lse_p, _stream_on(dev, stream))
+        if rc:
+            A.check(rc, w)
         return out, lse
 
     # -- pages --------------------------------------------------------------
@@ -591,7 +606,7 @@ class ResidencyPool:
         src, dst = (C.c_uint32 * max(1, n))(*src_rows), (C.c_uint32 * max(1, n))(*dst_rows)
         A.check(self.ctx.lib.kvm_pool_fork(self.ctx.h, self.h, C.byref(layout), src, dst, n,
                                            self.pages if page_end is None else page_end, ctas,
-                                           _stream_on(self.ctx.device, stream).cuda_stream), "kvm_pool_fork")
+                                           _stream_on(self.ctx.device, stream)), "kvm_pool_fork")
 
     def copy_pages(self, layout: A.StageLayout, items, *, ctas: int = 0, stream=None) -> None:
         """items: (src_row, src_page, dst_row, dst_page) tuples, or a contiguous int32 CPU tensor [n][4]
@@ -605,19 +620,19 @@ class ResidencyPool:
             arr = (A.PageCopy * max(1, len(items)))(*[A.PageCopy(*x) for x in items])
             n, ptr = len(items), C.cast(arr, C.c_void_p)
         A.check(self.ctx.lib.kvm_pool_copy(self.ctx.h, self.h, C.byref(layout), ptr, n, ctas,
-                                           _stream_on(self.ctx.device, stream).cuda_stream), "kvm_pool_copy")
+                                           _stream_on(self.ctx.device, stream)), "kvm_pool_copy")
 
     def free(self, rows: Sequence[int], ids: torch.Tensor, counts: torch.Tensor, *, stream=None) -> None:
         """Drops the pages ids[i][: counts[i]] (int32, device) of row rows[i] (kvm_pool_free)."""
         n = len(rows)
         w = "kvm_pool_free"
-        _on_device(self.ctx.device, w, ids=ids, counts=counts)
+        _on_device(self.ctx.device, w, ids)
         if ids.dim() != 2 or ids.shape[0] < n or ids.element_size() != 4 or not ids.is_contiguous():
             raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{w}: ids is contiguous int32 [rows][.]")
         arr = (C.c_uint32 * max(1, n))(*rows)
         A.check(self.ctx.lib.kvm_pool_free(self.ctx.h, self.h, arr, n, ids.data_ptr(),
-                                           _u32_arg(counts, self.ctx.device, n, w)[1], ids.shape[1],
-                                           _stream_on(self.ctx.device, stream).cuda_stream), w)
+                                           _seq_arg(counts, self.ctx.device, n, w, torch.int32)[1], ids.shape[1],
+                                           _stream_on(self.ctx.device, stream)), w)
 
     def compact(self, layout: A.StageLayout, rows: Optional[Sequence[int]] = None, *, used: Optional[torch.Tensor] = None,
                 ctas: int = 0, stream=None) -> None:
@@ -627,9 +642,9 @@ class ResidencyPool:
         n = len(rows)
         w = "kvm_pool_compact"
         arr = (C.c_uint32 * max(1, n))(*rows)
-        ptr = None if used is None else _u32_arg(used, self.ctx.device, n, w)[1]
+        ptr = None if used is None else _seq_arg(used, self.ctx.device, n, w, torch.int32)[1]
         A.check(self.ctx.lib.kvm_pool_compact(self.ctx.h, self.h, C.byref(layout), arr, n, ptr, ctas,
-                                              _stream_on(self.ctx.device, stream).cuda_stream), w)
+                                              _stream_on(self.ctx.device, stream)), w)
 
 
 class Transfer:
@@ -754,25 +769,6 @@ class StageOut:
 
     def clear(self) -> None:
         A.check(self.lib.kvm_stageout_clear(self.h), "kvm_stageout_clear")
-
-
-def _attention_out(where, q, k, v, out, lse, want_lse, stream):
-    """Shape and type checks of an attention call, and its outputs (allocated for `stream` where not given)."""
-    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or q.dtype not in (torch.float16, torch.bfloat16):
-        raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{where}: q, k, v are 4-D, q fp16 or bf16")
-    if k.dtype != q.dtype or v.dtype != q.dtype or k.shape != v.shape or k.shape[0] != q.shape[0] or \
-            k.shape[3] != q.shape[3]:
-        raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{where}: k and v do not match q")
-    with torch.cuda.stream(stream):
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        if lse is None and want_lse:
-            lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
-    if out.shape != q.shape or out.dtype != q.dtype:
-        raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{where}: out does not match q")
-    if lse is not None and (lse.shape != q.shape[:3] or lse.dtype != torch.float32 or not lse.is_contiguous()):
-        raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{where}: lse is contiguous float32 [seqs][rows][q_heads]")
-    return out, lse
 
 
 def tree_mask(parents: Sequence[int]) -> torch.Tensor:

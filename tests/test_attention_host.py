@@ -37,8 +37,8 @@ def test_null_handles_are_refused_before_any_cuda_call():
     import kvmem_b200 as K
     A, lib = K._abi, K._abi.load()
     r, kc, lay = A.Rows(), A.KCache(), A.StageLayout()
-    assert lib.kvm_window_attention(None, A.WindowDesc(), r, kc, kc, r, None, None) == A.ERR_INVALID_ARGUMENT
-    assert lib.kvm_tree_attention(None, None, A.TreeDesc(), lay, r, kc, kc, r, None, None) == A.ERR_INVALID_ARGUMENT
+    assert lib.kvm_window_attention(None, C.byref(A.WindowDesc()), C.byref(r), C.byref(kc), C.byref(kc), C.byref(r), None, None) == A.ERR_INVALID_ARGUMENT
+    assert lib.kvm_tree_attention(None, None, C.byref(A.TreeDesc()), lay, C.byref(r), C.byref(kc), C.byref(kc), C.byref(r), None, None) == A.ERR_INVALID_ARGUMENT
     assert lib.kvm_pool_fork(None, None, lay, None, None, 1, 1, 0, None) == A.ERR_INVALID_ARGUMENT
     assert lib.kvm_pool_copy(None, None, lay, None, 1, 0, None) == A.ERR_INVALID_ARGUMENT
     assert lib.kvm_pool_free(None, None, None, 1, None, None, 1, None) == A.ERR_INVALID_ARGUMENT
