@@ -33,7 +33,8 @@ namespace kvmb {
 constexpr int kAcKeys = 128;             // keys per tile
 constexpr uint32_t kAcUnit = 16384;      // bytes per ring unit
 constexpr uint32_t kAcTable = 512;       // page entries of one CTA's key chunk
-constexpr uint32_t kAcMaxUnits = 12;
+constexpr uint32_t kAcScans = 8;          // V tiles that the scan may be ahead of the softmax, and one
+constexpr uint32_t kAcMaxTiles = 14;      // K and V tiles that the ring's barriers tell apart
 
 __host__ __device__ constexpr int ac_mt(int D) { return D == 256 ? 1 : 2; }
 __host__ __device__ constexpr int ac_threads(int D) { return 128 + 128 * ac_mt(D); }
@@ -41,6 +42,9 @@ __host__ __device__ constexpr uint32_t ac_units(int D, int mode) {
     // What is left of 227 KiB beside the query tiles (and the page table).
     return (D == 64 ? 12u : 10u) - (mode == kAtTree ? 1u : 0u);
 }
+// A K or V tile (D / 64 units) has one pair of barriers; those of tile q serve tile
+// q + ac_tiles again, whose first unit waits for a unit of a tile behind q.
+__host__ __device__ constexpr uint32_t ac_tiles(int D, int mode) { return ac_units(D, mode) / uint32_t(D / 64) + 2u; }
 __host__ __device__ constexpr uint32_t ac_smem_bytes(int D, int mode) {
     return 1024u + uint32_t(ac_mt(D)) * 128u * uint32_t(D) * 2u + ac_units(D, mode) * kAcUnit +
            (mode == kAtTree ? kAcTable * 8u : 0u) + 512u;
@@ -53,6 +57,33 @@ struct AttendTcMaps {
     CUtensorMap dk, dv;  // dense keys: (D, kv_heads, tokens, sequences), boxes (64, 1, 128 | V unit keys, 1)
     CUtensorMap pk, pv;  // pages: (D, kv_heads, page_tokens, slots, rows), boxes (64, 1, box | min(box, V unit keys), 1, 1)
 };
+
+__device__ __forceinline__ void ac_complete_tx(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+
+// The instructions of the MMA warp are executed by all its lanes, so that descriptors
+// stay in uniform registers; one elected lane issues (the same one every time).
+__device__ __forceinline__ void ac_mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t.reg .b32 t;\n\telect.sync t|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void ac_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t.reg .b32 t;\n\telect.sync t|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void ac_commit(uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t.reg .b32 t;\n\telect.sync t|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
+        : "memory");
+}
 
 __device__ __forceinline__ void ac_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
     asm volatile(
@@ -69,6 +100,21 @@ __device__ __forceinline__ void ac_load_5d(uint32_t dst, const CUtensorMap* map,
         : "memory");
 }
 
+// 0 * x + acc on two packed 16-bit values: stays 0 while every x is finite, NaN from then on.
+template <bool BF16>
+__device__ __forceinline__ uint32_t ac_zero_times(uint32_t x, uint32_t acc) {
+    const uint32_t zero = 0;
+    if constexpr (BF16) {
+        const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&zero),
+                                         *reinterpret_cast<const __nv_bfloat162*>(&acc));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    } else {
+        const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&zero),
+                                  *reinterpret_cast<const __half2*>(&acc));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+}
+
 // Max of 128 values by three-input maxes.
 __device__ __forceinline__ float ac_max128(const float* x) { return fmaxf(pf_max64(x), pf_max64(x + 64)); }
 
@@ -80,6 +126,8 @@ __global__ void __launch_bounds__(ac_threads(D), 1)
     constexpr uint32_t U = D / 64;               // units of a K tile, and of a V tile
     constexpr uint32_t VK = kAcUnit / (D * 2);   // keys of a V unit
     constexpr uint32_t NU = ac_units(D, MODE);
+    constexpr uint32_t NB = ac_tiles(D, MODE);
+    static_assert(NB <= kAcMaxTiles, "tile barriers");
     constexpr uint32_t kQTile = 128 * D * 2;
     constexpr uint32_t kColO = 256;              // S / P: columns 0-127 and 128-255; O of M tile m: 256 + m * D
     extern __shared__ uint8_t smem_raw[];
@@ -87,17 +135,19 @@ __global__ void __launch_bounds__(ac_threads(D), 1)
     uint8_t* ring = qsm + MT * kQTile;
     int2* table = reinterpret_cast<int2*>(ring + NU * kAcUnit);
     uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(table) + (MODE == kAtTree ? kAcTable * 8 : 0));
-    uint64_t* full = bars;                 // [NU]
-    uint64_t* empty = bars + kAcMaxUnits;  // [NU]
-    uint64_t* s_full = bars + 2 * kAcMaxUnits;      // [2]
-    uint64_t* p_full = bars + 2 * kAcMaxUnits + 2;  // [2]
-    uint64_t* pv_done = bars + 2 * kAcMaxUnits + 4; // [2]
-    uint64_t* q_full = bars + 2 * kAcMaxUnits + 6;
-    uint64_t* fin = bars + 2 * kAcMaxUnits + 7;
-    uint64_t* together = bars + 2 * kAcMaxUnits + 8;  // all softmax threads (a barrier whose wait is bounded)
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kAcMaxUnits + 9);
+    uint64_t* full = bars;                 // [NB] tile loaded
+    uint64_t* empty = bars + kAcMaxTiles;  // [NB] tile used up
+    uint64_t* s_full = bars + 2 * kAcMaxTiles;       // [2]
+    uint64_t* p_full = bars + 2 * kAcMaxTiles + 2;   // [2] keys 0 .. 63 of P
+    uint64_t* p_half = bars + 2 * kAcMaxTiles + 4;   // [2] keys 64 .. 127 of P
+    uint64_t* pv_done = bars + 2 * kAcMaxTiles + 6;  // [2]
+    uint64_t* q_full = bars + 2 * kAcMaxTiles + 8;
+    uint64_t* fin = bars + 2 * kAcMaxTiles + 9;
+    uint64_t* together = bars + 2 * kAcMaxTiles + 10;  // all softmax threads (a barrier whose wait is bounded)
+    uint64_t* scanned = bars + 2 * kAcMaxTiles + 11;   // [kAcScans] V tile looked through
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kAcMaxTiles + 11 + kAcScans);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    uint32_t* bad_flag = tmem_slot + 2;  // [2], by tile parity
+    volatile uint32_t* bad_flag = tmem_slot + 2;     // [kAcScans][2] by the two scanning warps
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint32_t un = blockIdx.x;
@@ -185,20 +235,21 @@ __global__ void __launch_bounds__(ac_threads(D), 1)
     }
 
     if (tid == 0) {
-        for (uint32_t i = 0; i < NU; ++i) {
+        for (uint32_t i = 0; i < NB; ++i) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
+        for (uint32_t i = 0; i < kAcScans; ++i) mbar_init(&scanned[i], 2);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 128);
+            mbar_init(&p_half[i], 128);
             mbar_init(&pv_done[i], 1);
         }
         mbar_init(q_full, 128 * MT);
         mbar_init(fin, 1);
         mbar_init(together, 128 * MT);
         *abort_flag = 0;
-        bad_flag[0] = bad_flag[1] = 0;
         mbar_fence_init();
     }
     if (warp == 1) {
@@ -211,10 +262,24 @@ __global__ void __launch_bounds__(ac_threads(D), 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    // Ring order of the units: the order in which the products take the tiles.
+    // Ring order of the tiles, the order in which the products take them.
     // MT = 2: K0 V0 K1 V1 ..; MT = 1: K0 K1 V0 K2 V1 .. V(n - 1).
-    auto k_unit = [&](uint32_t j) { return MT == 2 ? 2 * j * U : (j ? (2 * j - 1) * U : 0); };
-    auto v_unit = [&](uint32_t j) { return MT == 2 ? (2 * j + 1) * U : (j + 1 == n ? (2 * n - 1) * U : (2 * j + 2) * U); };
+    auto k_seq = [&](uint32_t j) { return MT == 2 ? 2 * j : (j ? 2 * j - 1 : 0); };
+    auto v_seq = [&](uint32_t j) { return MT == 2 ? 2 * j + 1 : (j + 1 == n ? 2 * n - 1 : 2 * j + 2); };
+    // Whether some row of the CTA does not see all of tile t.
+    auto in_part = [&](uint32_t t) -> bool {
+        if constexpr (MODE == kAtWindow) {
+            const uint32_t a = t < n_first ? t * kAcKeys : lo + (t - n_first) * kAcKeys;
+            return !(a + kAcKeys <= (t < n_first ? few : hi) && a + kAcKeys - 1 <= p0 &&
+                     (a + kAcKeys <= P.sinks || p1 - a < P.window));
+        } else {
+            if (t >= n_first) return (t - n_first + 1) * kAcKeys > recent;
+            bool part = t * kAcKeys + kAcKeys > n_keys;
+            const uint32_t first = page_div(t * kAcKeys), last = page_div(min(t * kAcKeys + kAcKeys, n_keys) - 1);
+            for (uint32_t e = first; e <= last; ++e) part = part || table[e - e0].y != int(P.page_tokens);
+            return part;
+        }
+    };
 
     // MT = 2: registers go to the softmax warps, 4 x 32 x 72 + 8 x 32 x 216 = 384 x 168.
     if (warp < 4) {
@@ -222,129 +287,192 @@ __global__ void __launch_bounds__(ac_threads(D), 1)
         if (warp == 0) {
             // ---- TMA producer ----
             if (lane == 0) {
-                uint32_t issued = 0;
-                // Unit `sub` of K (or V) tile j of this CTA.
-                auto load = [&](uint32_t idx, uint32_t j, bool is_v, uint32_t sub) -> bool {
-                    const uint32_t s = idx % NU;
-                    if (idx >= NU && !mbar_wait(&empty[s], ((idx - NU) / NU) & 1)) {
-                        record_error(P.status, KVM_ERR_TIMEOUT, 125);
-                        return false;
+                uint32_t tiles_issued = 0, freed = 0;  // tiles issued; tiles known to be used up
+                // K (or V) tile j of this CTA, the q-th of the ring.
+                auto load = [&](uint32_t j, bool is_v) -> bool {
+                    const uint32_t q = is_v ? v_seq(j) : k_seq(j), t = tb + j;
+                    const uint32_t keys = is_v ? VK : uint32_t(kAcKeys), bh = min(box, keys);
+                    uint64_t* bar = &full[q % NB];
+                    const bool dense = MODE == kAtWindow || t >= n_first;
+                    const uint32_t tok = MODE == kAtWindow ? (t < n_first ? t * kAcKeys : lo + (t - n_first) * kAcKeys)
+                                                           : (t - n_first) * kAcKeys;
+                    auto held = [&](uint32_t x) { return x < n_keys && int(x - page_div(x) * P.page_tokens) < table[page_div(x) - e0].y; };
+                    uint32_t bytes = U * kAcUnit, sent = 0;
+                    if (!dense) {
+                        bytes = 0;
+                        for (uint32_t x = 0; x < uint32_t(kAcKeys); x += bh)
+                            if (held(t * kAcKeys + x)) bytes += bh * D * 2;
                     }
-                    const uint32_t dst = smem_u32(ring + s * kAcUnit), t = tb + j;
-                    const uint32_t keys = is_v ? VK : uint32_t(kAcKeys), key0 = is_v ? sub * VK : 0;
-                    const uint32_t d0 = is_v ? 0 : sub, d1 = is_v ? U : sub + 1;  // 64-dim blocks
-                    issued = idx + 1;
-                    if (MODE == kAtWindow || t >= n_first) {
-                        const uint32_t tok = MODE == kAtWindow
-                                                 ? (t < n_first ? t * kAcKeys : lo + (t - n_first) * kAcKeys) + key0
-                                                 : (t - n_first) * kAcKeys + key0;
-                        mbar_arrive_expect_tx(&full[s], kAcUnit);
-                        for (uint32_t a = d0; a < d1; ++a)
-                            ac_load_4d(dst + (a - d0) * keys * 128, is_v ? &maps.dv : &maps.dk, int(a * 64), int(h), int(tok),
-                                       int(b), &full[s]);
-                    } else {
-                        const uint32_t bh = min(box, keys), nb = keys / bh;
-                        uint32_t live = 0;
-                        for (uint32_t i = 0; i < nb; ++i) {
-                            const uint32_t x = t * kAcKeys + key0 + i * bh, en = page_div(x);
-                            if (x < n_keys && int(x - en * P.page_tokens) < table[en - e0].y) ++live;
-                        }
-                        if (live) mbar_arrive_expect_tx(&full[s], live * bh * 128 * (d1 - d0));
-                        else mbar_arrive(&full[s]);
-                        if (live)
-                            for (uint32_t i = 0; i < nb; ++i) {
-                                const uint32_t x = t * kAcKeys + key0 + i * bh, en = page_div(x), o = x - en * P.page_tokens;
-                                if (x >= n_keys || int(o) >= table[en - e0].y) continue;
-                                for (uint32_t a = d0; a < d1; ++a)
-                                    ac_load_5d(dst + (a - d0) * keys * 128 + i * bh * 128, is_v ? &maps.pv : &maps.pk,
-                                               int(a * 64), int(h), int(o), table[en - e0].x, int(prow), &full[s]);
+                    for (uint32_t sub = 0; sub < U; ++sub) {
+                        const uint32_t idx = q * U + sub, s = idx % NU;
+                        while (idx >= NU && freed <= (idx - NU) / U) {  // the tile whose unit this one replaces
+                            if (!mbar_wait(&empty[freed % NB], (freed / NB) & 1)) {
+                                record_error(P.status, KVM_ERR_TIMEOUT, 125);
+                                if (sub) ac_complete_tx(bar, bytes - sent);  // copies of this tile that are not started
+                                return false;
                             }
+                            ++freed;
+                        }
+                        if (sub == 0) {
+                            if (bytes) mbar_arrive_expect_tx(bar, bytes);
+                            else mbar_arrive(bar);
+                            tiles_issued = q + 1;
+                        }
+                        const uint32_t dst = smem_u32(ring + s * kAcUnit), key0 = is_v ? sub * VK : 0;
+                        const uint32_t d0 = is_v ? 0 : sub, d1 = is_v ? U : sub + 1;  // 64-dim blocks
+                        if (dense) {
+                            sent += kAcUnit;
+                            for (uint32_t a = d0; a < d1; ++a)
+                                ac_load_4d(dst + (a - d0) * keys * 128, is_v ? &maps.dv : &maps.dk, int(a * 64), int(h),
+                                           int(tok + key0), int(b), bar);
+                        } else {
+                            for (uint32_t i = 0; i < keys; i += bh) {
+                                const uint32_t x = t * kAcKeys + key0 + i;
+                                if (!held(x)) continue;
+                                const uint32_t en = page_div(x);
+                                sent += bh * 128 * (d1 - d0);
+                                for (uint32_t a = d0; a < d1; ++a)
+                                    ac_load_5d(dst + (a - d0) * keys * 128 + i * 128, is_v ? &maps.pv : &maps.pk, int(a * 64),
+                                               int(h), int(x - en * P.page_tokens), table[en - e0].x, int(prow), bar);
+                            }
+                        }
                     }
                     return true;
                 };
                 bool ok = true;
-                auto load_k = [&](uint32_t j) {
-                    for (uint32_t i = 0; i < U && ok && !*abort_flag; ++i) ok = load(k_unit(j) + i, j, false, i);
-                };
-                auto load_v = [&](uint32_t j) {
-                    for (uint32_t i = 0; i < U && ok && !*abort_flag; ++i) ok = load(v_unit(j) + i, j, true, i);
-                };
                 if (n) {
-                    load_k(0);
-                    if (MT == 1 && n > 1) load_k(1);
+                    ok = load(0, false);
+                    if (MT == 1 && n > 1) ok = ok && load(1, false);
                     for (uint32_t j = 0; j < n && ok && !*abort_flag; ++j) {
-                        load_v(j);
-                        if (j + (3 - MT) < n) load_k(j + (3 - MT));
+                        ok = load(j, true);
+                        if (ok && j + (3 - MT) < n) ok = load(j + (3 - MT), false);
                     }
                 }
                 if (!ok) *abort_flag = 1;
                 // Every issued copy lands before the CTA frees its shared memory.
-                for (uint32_t i = issued > NU ? issued - NU : 0; i < issued; ++i)
-                    if (!mbar_wait(&full[i % NU], (i / NU) & 1)) record_error(P.status, KVM_ERR_TIMEOUT, 126);
+                for (uint32_t q = tiles_issued > NB ? tiles_issued - NB : 0; q < tiles_issued; ++q)
+                        if (!mbar_wait(&full[q % NB], (q / NB) & 1)) record_error(P.status, KVM_ERR_TIMEOUT, 126);
             }
         } else if (warp == 1) {
-            // ---- MMA issue: one thread; step w = (tile w / MT, M tile w % MT), S slot w & 1 ----
-            if (lane == 0) {
-                constexpr uint32_t idesc_s = pf_idesc(128, kAcKeys, BF16, false);
-                constexpr uint32_t idesc_o = pf_idesc(128, D, BF16, true);
-                int err = 0;
-                auto issue_s = [&](uint32_t w) -> bool {
-                    const uint32_t j = w / MT, m = w % MT, at = k_unit(j);
-                    const uint32_t qb = smem_u32(qsm + m * kQTile);
-                    for (uint32_t a = 0; a < U; ++a) {
-                        const uint32_t s = (at + a) % NU;
-                        if (!mbar_wait(&full[s], ((at + a) / NU) & 1)) return false;
-                        tc_fence_after();
-                        const uint32_t kb = smem_u32(ring + s * kAcUnit);
-    #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)
-                            tc_mma(tmem + (w & 1) * 128, tc_desc_sw128(qb + a * 16384 + kk * 32), tc_desc_sw128(kb + kk * 32),
-                                   idesc_s, (a | kk) != 0);
-                        if (m == MT - 1) tc_commit(&empty[s]);
-                    }
-                    tc_commit(&s_full[w & 1]);
-                    return true;
-                };
-                const uint32_t steps = n * MT;
-                if (!mbar_wait(q_full, 0)) err = 130;
+            // ---- MMA issue; step w = (tile w / MT, M tile w % MT), S slot w & 1 ----
+            // The warp only adds constants to descriptors and ring positions.
+            constexpr uint32_t idesc_s = pf_idesc(128, kAcKeys, BF16, false);
+            constexpr uint32_t idesc_o = pf_idesc(128, D, BF16, true);
+            const uint64_t qdesc = tc_desc_sw128(smem_u32(qsm)), kdesc = tc_desc_sw128(smem_u32(ring));
+            const uint64_t vdesc = pf_desc_mn_sw128(smem_u32(ring), VK * 128);
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            struct Pos {  // a unit of the ring; a tile's barrier and the parity of its pass
+                uint32_t s, b, ph;
+                __device__ __forceinline__ void unit() { s = s + 1 == NU ? 0 : s + 1; }
+                __device__ __forceinline__ void tile() {
+                    if (++b == NB) b = 0, ph ^= 1;
+                }
+                __device__ __forceinline__ void skip() {  // a whole tile
+                    s += U;
+                    if (s >= NU) s -= NU;
+                    tile();
+                }
+            };
+            Pos kp{0, 0, 0}, vp{0, 0, 0};
+            vp.skip();
+            if (MT == 1 && n > 1) vp.skip();
+            int err = 0;
+            // S of M tile m from the K tile at kp; the last M tile moves kp on.
+            auto issue_s = [&](uint32_t slot, uint32_t m, bool first) -> bool {
+                if (!pf_warp_wait(&full[kp.b], kp.ph)) return false;
                 tc_fence_after();
-                for (uint32_t w = 0; w < 2 && w < steps && !err; ++w)
-                    if (!issue_s(w)) err = 131;
-                for (uint32_t w = 0; w < steps && !err; ++w) {
-                    if (*abort_flag) {
-                        err = -1;
-                        break;
-                    }
-                    const uint32_t j = w / MT, m = w % MT, at = v_unit(j);
-                    if (!mbar_wait(&p_full[w & 1], (w >> 1) & 1)) {
-                        err = 132;
-                        break;
-                    }
-                    tc_fence_after();
-                    for (uint32_t a = 0; a < U; ++a) {
-                        const uint32_t s = (at + a) % NU;
-                        if (!mbar_wait(&full[s], ((at + a) / NU) & 1)) {
-                            err = 133;
-                            break;
+                Pos k = kp;
+                const uint64_t qd = qdesc + m * (kQTile >> 4);
+#pragma unroll
+                for (uint32_t a = 0; a < U; ++a) {
+                    const uint64_t kd = kdesc + k.s * (kAcUnit >> 4);
+#pragma unroll
+                    for (uint32_t kk = 0; kk < 4; ++kk)
+                        ac_mma(tm + slot * 128, qd + a * (16384 >> 4) + kk * 2, kd + kk * 2, idesc_s, (a | kk) != 0);
+                    k.unit();
+                }
+                ac_commit(&s_full[slot]);
+                if (m == MT - 1) {
+                    ac_commit(&empty[k.b]);
+                    k.tile();
+                    kp = k;
+                    if (MT == 2 || !first) kp.skip();  // over the V tile in between
+                }
+                return true;
+            };
+            const uint32_t steps = __shfl_sync(0xffffffffu, n * MT, 0);
+            if (!pf_warp_wait(q_full, 0)) err = 130;
+            tc_fence_after();
+            for (uint32_t w = 0; w < 2 && w < steps && !err; ++w)
+                if (!issue_s(w, w % MT, w == 0)) err = 131;
+            uint32_t ph = 0;  // parity of P's barriers
+            for (uint32_t w = 0; w < steps && !err; ++w) {
+                const uint32_t slot = w & 1, m = w % MT;
+                const bool more = w >= uint32_t(MT);  // O holds something
+                if (!pf_warp_wait(&full[vp.b], vp.ph)) err = 133;
+                if (!err && !pf_warp_wait(&p_full[slot], ph)) err = 132;
+                if (err || __shfl_sync(0xffffffffu, *abort_flag, 0)) {
+                    if (!err) err = -1;
+                    break;
+                }
+                tc_fence_after();
+                Pos v = vp;
+#pragma unroll
+                for (uint32_t a = 0; a < U; ++a) {
+                    const uint64_t vd = vdesc + v.s * (kAcUnit >> 4);
+#pragma unroll
+                    for (uint32_t kk = 0; kk < VK / 16; ++kk) {  // P: 16 keys = 8 tensor-memory columns
+                        if (a * VK + kk * 16 == 64) {
+                            if (!pf_warp_wait(&p_half[slot], ph)) err = 136;
+                            tc_fence_after();
                         }
-                        tc_fence_after();
-                        const uint32_t vb = smem_u32(ring + s * kAcUnit);
-    #pragma unroll
-                        for (uint32_t kk = 0; kk < VK / 16; ++kk)  // P: 16 keys = 8 tensor-memory columns
-                            tc_mma_ts(tmem + kColO + m * D, tmem + (w & 1) * 128 + (a * (VK / 16) + kk) * 8,
-                                      pf_desc_mn_sw128(vb + kk * 2048, VK * 128), idesc_o, j > 0 || (a | kk) != 0);
-                        if (m == MT - 1) tc_commit(&empty[s]);
+                        ac_mma_ts(tm + kColO + m * D, tm + slot * 128 + (a * (VK / 16) + kk) * 8, vd + kk * (2048 >> 4), idesc_o,
+                                  more || (a | kk) != 0);
                     }
-                    if (err) break;
-                    tc_commit(&pv_done[w & 1]);
-                    if (w + 2 < steps && !issue_s(w + 2)) err = 131;
+                    v.unit();
                 }
-                if (err > 0) {
-                    record_error(P.status, KVM_ERR_TIMEOUT, err);
-                    *abort_flag = 1;
+                ac_commit(&pv_done[slot]);
+                if (m == MT - 1) {
+                    ac_commit(&empty[v.b]);
+                    v.tile();
+                    vp = v;
+                    // Over the K tile in between; none stands before the last V tile of MT = 1.
+                    if (MT == 2 || w + 2 < steps) vp.skip();
                 }
-                tc_commit(fin);
-                if (!mbar_wait(fin, 0)) record_error(P.status, KVM_ERR_TIMEOUT, 134);
+                if (!err && w + 2 < steps && !issue_s(slot, m, false)) err = 131;
+                if (slot) ph ^= 1;
+            }
+            if (err > 0 && lane == 0) {
+                record_error(P.status, KVM_ERR_TIMEOUT, err);
+                *abort_flag = 1;
+            }
+            __syncwarp();
+            ac_commit(fin);
+            if (!pf_warp_wait(fin, 0) && lane == 0) record_error(P.status, KVM_ERR_TIMEOUT, 134);
+        } else {
+            // ---- warps 2 and 3: V tiles that some row does not see in full are looked through for
+            // infinities and NaN (0 * x is NaN for the rows that must not see them) ----
+            for (uint32_t j = 0; j < n; ++j) {
+                const uint32_t q = v_seq(j);
+                const bool ok = pf_warp_wait(&full[q % NB], (q / NB) & 1);
+                uint32_t acc = 0;
+                if (in_part(tb + j)) {
+#pragma unroll
+                    for (uint32_t a = 0; a < U; ++a) {
+                        const uint4* v4 = reinterpret_cast<const uint4*>(ring + ((q * U + a) % NU) * kAcUnit);
+#pragma unroll 8
+                        for (uint32_t e = uint32_t(tid - 64); e < kAcUnit / 16; e += 64) {
+                            const uint4 y = v4[e];
+                            acc = ac_zero_times<BF16>(y.x, ac_zero_times<BF16>(y.y, ac_zero_times<BF16>(y.z, ac_zero_times<BF16>(y.w, acc))));
+                        }
+                    }
+                }
+                const bool bad = __any_sync(0xffffffffu, at_nonfinite<BF16>(acc));
+                if (lane == 0) {
+                    bad_flag[(j % kAcScans) * 2 + (warp & 1)] = bad;
+                    mbar_arrive(&scanned[j % kAcScans]);
+                }
+                if (!ok || __shfl_sync(0xffffffffu, *abort_flag, 0)) break;
             }
         }
     } else {
@@ -359,11 +487,12 @@ __global__ void __launch_bounds__(ac_threads(D), 1)
             const uint4* qp = reinterpret_cast<const uint4*>(P.q + uint64_t(b) * P.q_seq + uint64_t(ri) * P.q_row +
                                                              uint64_t(qh) * P.q_head);
             uint8_t* qd = qsm + m * kQTile + row * 128;
-#pragma unroll 8
-            for (uint32_t c = 0; c < D / 8; ++c) {
-                const uint4 x = r < m_end ? __ldg(qp + c) : make_uint4(0, 0, 0, 0);
-                *reinterpret_cast<uint4*>(qd + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4)) = x;
-            }
+            uint4 x[D / 8];
+#pragma unroll
+            for (uint32_t c = 0; c < D / 8; ++c) x[c] = r < m_end ? __ldg(qp + c) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (uint32_t c = 0; c < D / 8; ++c)
+                *reinterpret_cast<uint4*>(qd + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4)) = x[c];
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             mbar_arrive(q_full);
         }
@@ -389,11 +518,10 @@ __global__ void __launch_bounds__(ac_threads(D), 1)
             }
             // Which of the tile's keys this row sees; `part`: some row of the CTA does not see all.
             uint32_t see[4] = {~0u, ~0u, ~0u, ~0u};
-            bool part;
+            const bool part = in_part(t);
             if constexpr (MODE == kAtWindow) {
                 const uint32_t a = t < n_first ? t * kAcKeys : lo + (t - n_first) * kAcKeys;
                 const uint32_t end = t < n_first ? few : hi;
-                part = !(a + kAcKeys <= end && a + kAcKeys - 1 <= p0 && (a + kAcKeys <= P.sinks || p1 - a < P.window));
                 if (part) {
                     // Keys [0, s1) u [w0, u1) of the tile: sinks, and the window up to the row's position.
                     const uint32_t p = p0 + (ri - i0);
@@ -405,7 +533,6 @@ __global__ void __launch_bounds__(ac_threads(D), 1)
                 }
             } else if (t >= n_first) {
                 const uint32_t a = (t - n_first) * kAcKeys;
-                part = a + kAcKeys > recent;
                 if (part) {
 const int rec = int(recent) - int(a);  // keys below are recent tokens, key rec + x is node x
                     const uint32_t* tw = P.tree ? P.tree + uint64_t(b) * P.tree_seq + uint64_t(ri) * P.tree_words : nullptr;
@@ -423,10 +550,8 @@ const int rec = int(recent) - int(a);  // keys below are recent tokens, key rec 
                     }
                 }
             } else {
-                part = t * kAcKeys + kAcKeys > n_keys;
-                const uint32_t first = page_div(t * kAcKeys), last = page_div(min(t * kAcKeys + kAcKeys, n_keys) - 1);
-                for (uint32_t e = first; e <= last; ++e) part = part || table[e - e0].y != int(P.page_tokens);
                 if (part) {
+                    const uint32_t first = page_div(t * kAcKeys), last = page_div(min(t * kAcKeys + kAcKeys, n_keys) - 1);
                     see[0] = see[1] = see[2] = see[3] = 0;
                     for (uint32_t e = first; e <= last; ++e) {
                         const int at = int(e * P.page_tokens) - int(t * kAcKeys), end = at + table[e - e0].y;
@@ -482,50 +607,55 @@ const int rec = int(recent) - int(a);  // keys below are recent tokens, key rec 
                 }
                 tc_wait_st();
             }
+            // P = exp2(x c2 - m), its sum, and P over its S (16-bit, two per column). The first 64 keys go
+            // to the tensor core while the others are worked out.
             const float mneg = -m_used;
             float s4[4] = {0.f, 0.f, 0.f, 0.f};
+            auto exps = [&](int q4) {
 #pragma unroll
-            for (int k = 0; k < kAcKeys; k += 2) {
-                pf_fma2(x[k], x[k + 1], x[k], x[k + 1], c2, mneg);
-                x[k] = fast_exp2(x[k]);
-                x[k + 1] = fast_exp2(x[k + 1]);
-                pf_add2(s4[k & 2], s4[(k & 2) + 1], x[k], x[k + 1]);
-            }
-            l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
-            bool bad = false;
-            if (part) {
-                // Infinite or NaN values in a V tile that some row does not see in full.
-                const uint32_t at = v_unit(j);
-                for (uint32_t a = 0; a < U && ok; ++a) {
-                    ok = pf_warp_wait(&full[(at + a) % NU], ((at + a) / NU) & 1);
-                    const uint4* v4 = reinterpret_cast<const uint4*>(ring + ((at + a) % NU) * kAcUnit);
-                    for (uint32_t e = row; e < kAcUnit / 16; e += 128) {
-                        const uint4 y = v4[e];
-                        bad = bad || at_nonfinite<BF16>(y.x) || at_nonfinite<BF16>(y.y) || at_nonfinite<BF16>(y.z) ||
-                              at_nonfinite<BF16>(y.w);
-                    }
+                for (int k = q4 * 32; k < q4 * 32 + 32; k += 2) {
+                    pf_fma2(x[k], x[k + 1], x[k], x[k + 1], c2, mneg);
+                    x[k] = fast_exp2(x[k]);
+                    x[k + 1] = fast_exp2(x[k + 1]);
+                    pf_add2(s4[k & 2], s4[(k & 2) + 1], x[k], x[k + 1]);
                 }
-                if (bad) atomicOr(&bad_flag[j & 1], 1u);
-                meet();
-                bad = *reinterpret_cast<volatile uint32_t*>(&bad_flag[j & 1]) != 0;
-                meet();
-                if (!ok) break;
-                if (row == 0 && m == 0) bad_flag[j & 1] = 0;  // read by all; set again two tiles on at the earliest
-            }
-            // P over its S, 16-bit, two per column.
-#pragma unroll
-            for (int q4 = 0; q4 < 2; ++q4) {
+            };
+            auto store = [&](int half) {
                 uint32_t pk[32];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) pk[i] = pf_pack2<BF16>(x[q4 * 64 + 2 * i], x[q4 * 64 + 2 * i + 1]);
-                tc_st32(lane_addr + slot * 128 + q4 * 32, pk);
+                for (int i = 0; i < 32; ++i) pk[i] = pf_pack2<BF16>(x[half * 64 + 2 * i], x[half * 64 + 2 * i + 1]);
+                tc_st32(lane_addr + slot * 128 + half * 32, pk);
+            };
+            auto hand_over = [&](uint64_t* bar) {
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive(bar);
+            };
+            exps(0);
+            exps(1);
+            ok = pf_warp_wait(&scanned[j % kAcScans], (j / kAcScans) & 1);
+            if (!ok) break;
+            const bool bad = bad_flag[(j % kAcScans) * 2] | bad_flag[(j % kAcScans) * 2 + 1];
+            if (!bad) {
+                store(0);
+                exps(2);
+                hand_over(&p_full[slot]);
+                exps(3);
+                store(1);
+                hand_over(&p_half[slot]);
+            } else {
+                exps(2);
+                exps(3);
+                store(0);
+                store(1);
             }
+            l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
             if (bad) {
                 // sums of p * v over the infinite and NaN values this row sees, which leave the product
                 float fix[D], pl[kAcKeys];
 #pragma unroll
                 for (int k = 0; k < kAcKeys; ++k) pl[k] = x[k];
-                const uint32_t at = v_unit(j);
+                const uint32_t at = v_seq(j) * U;
 #pragma unroll 1
                 for (uint32_t d = 0; d < D; ++d) {
                     float f = 0.f;
@@ -550,9 +680,8 @@ const int rec = int(recent) - int(a);  // keys below are recent tokens, key rec 
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 meet();
-                tc_wait_st();
-                tc_fence_before();
-                mbar_arrive(&p_full[slot]);
+                hand_over(&p_full[slot]);
+                mbar_arrive(&p_half[slot]);
                 if (!ok || !pf_warp_wait(&pv_done[slot], (w >> 1) & 1)) {
                     ok = false;
                     break;
@@ -569,10 +698,6 @@ const int rec = int(recent) - int(a);  // keys below are recent tokens, key rec 
                 }
                 tc_wait_st();
                 tc_fence_before();
-            } else {
-                tc_wait_st();
-                tc_fence_before();
-                mbar_arrive(&p_full[slot]);
             }
         }
         grid_release();
