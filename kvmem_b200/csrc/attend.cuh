@@ -38,6 +38,8 @@ struct AttendParams {
     float* lse;  // [seqs][width][q_heads] or null
     uint32_t seqs, width, q_heads, kv_heads, group;
     uint32_t m_tiles, splits;
+    uint64_t g_magic;  // m / group = (m * g_magic) >> g_shift for m < 2^31
+    uint32_t g_shift;
     float scale_log2;
     // Dense keys: the window's cache, or the tree's tail.
     const uint8_t *k, *v;

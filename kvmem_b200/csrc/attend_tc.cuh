@@ -2,26 +2,29 @@
 // same operators as attend.cuh (window with sinks, tree over pages), for packed row
 // counts where the products and not the reading of K and V bound the time.
 //
-// One CTA per (sequence, KV head, 128 * MT packed rows, key chunk), one per SM:
+// One CTA per (sequence, KV head, 128 packed rows, key chunk); one per SM at head_dim
+// 256, two at 64 / 128, so that one's start, end and softmax run beside the other's
+// products:
 //  * warp 0 (one thread): TMA loads of 128-key tiles into one ring of 16 KiB
 //    units, K and V in the order in which the products take them. A K unit is 128
 //    keys x 64 dims (the B operand of S, K-major); a V unit is 32 / 64 / 128 keys x
-//    256 / 128 / 64 dims (the B operand of O, MN-major). Small units let the ring
-//    hold two and a half 64 KiB tiles at head_dim 256. Pages come as boxes of
-//    gcd(page_tokens, 128) tokens, each from its slot;
-//  * warp 1 (one thread): tcgen05.mma kind::f16, S = Q K^T (M = 128, N = 128, Q in
-//    shared memory), then O += P V (N = head_dim, P from tensor memory, where it
-//    replaces its S). Two S accumulators are in flight: the two M tiles of a CTA
-//    (MT = 2, head_dim 64 / 128: K and V are read once for 256 rows), or two
-//    successive key tiles of one (MT = 1, head_dim 256, where O takes half of the
-//    tensor memory). S of step w + 2 is issued right behind P V of step w;
-//  * four softmax warps per M tile: thread = packed row = tensor-memory lane.
-//    Masks are four words of bits per row and tile, made only for tiles that some
-//    row sees in part. The running max moves lazily: O is rescaled only when it
-//    grows by more than 2^8, so P stays below 2^8 and sums stay in 32 bits.
-// A V tile behind a mask may hold infinities or NaN, which 0 * x would spread to
-// rows that do not see them: masked tiles are scanned, such values are taken out of
-// the product and added by hand to the rows that do see them.
+//    256 / 128 / 64 dims (the B operand of O, MN-major). Pages come as boxes of gcd(page_tokens, 128) tokens, each from its slot;
+//  * warp 1: tcgen05.mma kind::f16, S = Q K^T (M = 128, N = 128, Q in shared memory),
+//    then O += P V (N = head_dim, P from tensor memory, where it replaces its S). At
+//    head_dim 256 two S accumulators are in flight (S of tile j + 2 is issued right
+//    behind P V of tile j); at 64 / 128 each CTA has one, and the tensor core works
+//    for the SM's other CTA meanwhile. One commit per product serves the softmax and
+//    the ring (a commit costs the tensor core some 100 cycles: with one for each use
+//    and unit a tile took 4,400 cycles instead of 3,300 at head_dim 256);
+//  * softmax warps: thread = packed row = tensor-memory lane; four warps, or eight at
+//    head_dim 256, each with half of the tile's keys. Masks are words of bits per
+//    thread and tile, made only for tiles that some row sees in part. The running max
+//    moves lazily: O is rescaled only when it grows by more than 2^8, so P stays
+//    below 2^8 and sums stay in 32 bits. P goes to the tensor core in two halves;
+//  * warps 2 and 3: a V tile behind a mask may hold infinities or NaN, which 0 * x
+//    would spread to rows that do not see them. Such tiles are looked through; where
+//    one holds such values they are taken out of the product and added by hand to the
+//    rows that do see them.
 // Every wait is bounded: on expiry the kernel records KVM_ERR_TIMEOUT, raises the
 // CTA's abort flag, lets copies and MMAs in flight finish and frees its TMEM.
 #pragma once
@@ -33,25 +36,25 @@ namespace kvmb {
 constexpr int kAcKeys = 128;             // keys per tile
 constexpr uint32_t kAcUnit = 16384;      // bytes per ring unit
 constexpr uint32_t kAcTable = 512;       // page entries of one CTA's key chunk
-constexpr uint32_t kAcScans = 8;          // V tiles that the scan may be ahead of the softmax, and one
-constexpr uint32_t kAcMaxTiles = 14;      // K and V tiles that the ring's barriers tell apart
+constexpr uint32_t kAcScans = 8;         // V tiles that the scan may be ahead of the softmax, and one
+constexpr uint32_t kAcMaxTiles = 7;
 
-__host__ __device__ constexpr int ac_mt(int D) { return D == 256 ? 1 : 2; }
-__host__ __device__ constexpr int ac_threads(int D) { return 128 + 128 * ac_mt(D); }
+__host__ __device__ constexpr int ac_ctas(int D) { return D == 256 ? 1 : 2; }      // CTAs per SM
+__host__ __device__ constexpr int ac_halves(int D) { return D == 256 ? 2 : 1; }    // softmax warps per 32 rows
+__host__ __device__ constexpr int ac_threads(int D) { return 128 + 128 * ac_halves(D); }
 __host__ __device__ constexpr uint32_t ac_units(int D, int mode) {
-    // What is left of 227 KiB beside the query tiles (and the page table).
-    return (D == 64 ? 12u : 10u) - (mode == kAtTree ? 1u : 0u);
+    // What is left of the SM's 227 KiB (or half of it) beside the query tile and the page table.
+    return D == 256 ? (mode == kAtTree ? 9u : 10u) : D == 128 ? 4u : 5u;
 }
-// A K or V tile (D / 64 units) has one pair of barriers; those of tile q serve tile
-// q + ac_tiles again, whose first unit waits for a unit of a tile behind q.
+// A K or V tile (D / 64 units) has one full barrier; that of tile q serves tile q +
+// ac_tiles again, whose first unit waits for a unit of a tile behind q.
 __host__ __device__ constexpr uint32_t ac_tiles(int D, int mode) { return ac_units(D, mode) / uint32_t(D / 64) + 2u; }
 __host__ __device__ constexpr uint32_t ac_smem_bytes(int D, int mode) {
-    return 1024u + uint32_t(ac_mt(D)) * 128u * uint32_t(D) * 2u + ac_units(D, mode) * kAcUnit +
+    return 128u * uint32_t(D) * 2u + ac_units(D, mode) * kAcUnit + (ac_halves(D) == 2 ? 2048u : 0u) +
            (mode == kAtTree ? kAcTable * 8u : 0u) + 512u;
 }
-
-static_assert(ac_smem_bytes(64, kAtTree) <= 227 * 1024 && ac_smem_bytes(64, kAtWindow) <= 227 * 1024 &&
-              ac_smem_bytes(128, kAtTree) <= 227 * 1024 && ac_smem_bytes(256, kAtWindow) <= 227 * 1024, "shared memory");
+static_assert(ac_smem_bytes(256, kAtTree) <= 227 * 1024 && ac_smem_bytes(256, kAtWindow) <= 227 * 1024, "shared memory");
+static_assert(ac_smem_bytes(128, kAtTree) <= 113 * 1024 && ac_smem_bytes(64, kAtTree) <= 113 * 1024, "shared memory");
 
 struct AttendTcMaps {
     CUtensorMap dk, dv;  // dense keys: (D, kv_heads, tokens, sequences), boxes (64, 1, 128 | V unit keys, 1)
@@ -115,41 +118,42 @@ __device__ __forceinline__ uint32_t ac_zero_times(uint32_t x, uint32_t acc) {
     }
 }
 
-// Max of 128 values by three-input maxes.
-__device__ __forceinline__ float ac_max128(const float* x) { return fmaxf(pf_max64(x), pf_max64(x + 64)); }
-
 template <int D, bool BF16, int MODE>
-__global__ void __launch_bounds__(ac_threads(D), 1)
+__global__ void __launch_bounds__(ac_threads(D), ac_ctas(D))
     attend_tc_kernel(const __grid_constant__ AttendTcMaps maps, const __grid_constant__ AttendParams P,
                      const uint32_t box) {
-    constexpr int MT = ac_mt(D);
+    constexpr int HS = ac_halves(D);
+    constexpr uint32_t SB = D == 256 ? 2 : 1;    // S accumulators
     constexpr uint32_t U = D / 64;               // units of a K tile, and of a V tile
     constexpr uint32_t VK = kAcUnit / (D * 2);   // keys of a V unit
     constexpr uint32_t NU = ac_units(D, MODE);
     constexpr uint32_t NB = ac_tiles(D, MODE);
-    static_assert(NB <= kAcMaxTiles, "tile barriers");
+    static_assert(NB <= kAcMaxTiles && NU >= 2 * U, "ring");
     constexpr uint32_t kQTile = 128 * D * 2;
-    constexpr uint32_t kColO = 256;              // S / P: columns 0-127 and 128-255; O of M tile m: 256 + m * D
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* qsm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    uint8_t* ring = qsm + MT * kQTile;
-    int2* table = reinterpret_cast<int2*>(ring + NU * kAcUnit);
+    constexpr uint32_t kColO = SB * 128, kCols = D == 256 ? 512 : 256;  // S / P, then O
+    extern __shared__ __align__(1024) uint8_t ac_smem[];  // the 128-byte swizzle counts from 1,024-byte boundaries
+    uint8_t* qsm = ac_smem;
+    uint8_t* ring = qsm + kQTile;
+    float* pair_max = reinterpret_cast<float*>(ring + NU * kAcUnit);  // HS = 2: [2 (tile parity)][2 (half)][128]
+    int2* table = reinterpret_cast<int2*>(pair_max + (HS == 2 ? 512 : 0));
     uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(table) + (MODE == kAtTree ? kAcTable * 8 : 0));
     uint64_t* full = bars;                 // [NB] tile loaded
-    uint64_t* empty = bars + kAcMaxTiles;  // [NB] tile used up
-    uint64_t* s_full = bars + 2 * kAcMaxTiles;       // [2]
-    uint64_t* p_full = bars + 2 * kAcMaxTiles + 2;   // [2] keys 0 .. 63 of P
-    uint64_t* p_half = bars + 2 * kAcMaxTiles + 4;   // [2] keys 64 .. 127 of P
-    uint64_t* pv_done = bars + 2 * kAcMaxTiles + 6;  // [2]
-    uint64_t* q_full = bars + 2 * kAcMaxTiles + 8;
-    uint64_t* fin = bars + 2 * kAcMaxTiles + 9;
-    uint64_t* together = bars + 2 * kAcMaxTiles + 10;  // all softmax threads (a barrier whose wait is bounded)
-    uint64_t* scanned = bars + 2 * kAcMaxTiles + 11;   // [kAcScans] V tile looked through
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kAcMaxTiles + 11 + kAcScans);
+    uint64_t* done = full + kAcMaxTiles;   // [NB] its product is done: S is there (K), O is and P is free (V)
+    uint64_t* p_full = done + kAcMaxTiles;  // [2] keys 0 .. 63 of P
+    uint64_t* p_half = p_full + 2;          // [2] keys 64 .. 127 of P
+    uint64_t* fin = p_full + 4;
+    uint64_t* together = p_full + 5;        // all softmax threads (a barrier whose wait is bounded)
+    uint64_t* scanned = p_full + 6;         // [kAcScans] V tile looked through
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scanned + kAcScans);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    volatile uint32_t* bad_flag = tmem_slot + 2;     // [kAcScans][2] by the two scanning warps
+    volatile uint32_t* bad_flag = tmem_slot + 2;  // [kAcScans][2] by the two scanning warps
+    static_assert((2 * kAcMaxTiles + 6 + kAcScans) * 8 + 8 + kAcScans * 8 <= 512, "barriers");
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (smem_u32(ac_smem) & 1023u) {
+        if (tid == 0) record_error(P.status, KVM_ERR_CUDA, 119);
+        return;
+    }
     uint32_t un = blockIdx.x;
     const uint32_t mt = un % P.m_tiles;
     un /= P.m_tiles;
@@ -158,9 +162,10 @@ __global__ void __launch_bounds__(ac_threads(D), 1)
     const uint32_t h = un % P.kv_heads, b = un / P.kv_heads;
     const uint32_t G = P.group;
     const uint32_t rows = P.seq_rows ? min(__ldg(P.seq_rows + b), P.width) : P.width;
-    const uint32_t m0 = mt * 128 * MT, m_end = rows * G;
+    const uint32_t m0 = mt * 128, m_end = rows * G;
     if (m0 >= m_end) return;
-    const uint32_t i0 = m0 / G, i1 = min(m0 + 128 * MT - 1, m_end - 1) / G;
+    auto row_div = [&](uint32_t m) { return uint32_t((uint64_t(m) * P.g_magic) >> P.g_shift); };
+    const uint32_t i0 = row_div(m0), i1 = row_div(min(m0 + 127, m_end - 1));
 
     // ---- this unit's keys (as attend_mma_kernel, tiles of 128) ----
     uint32_t nt, n_first;
@@ -237,35 +242,63 @@ __global__ void __launch_bounds__(ac_threads(D), 1)
     if (tid == 0) {
         for (uint32_t i = 0; i < NB; ++i) {
             mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
+            mbar_init(&done[i], 1);
         }
         for (uint32_t i = 0; i < kAcScans; ++i) mbar_init(&scanned[i], 2);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 128);
             mbar_init(&p_half[i], 128);
-            mbar_init(&pv_done[i], 1);
         }
-        mbar_init(q_full, 128 * MT);
         mbar_init(fin, 1);
-        mbar_init(together, 128 * MT);
+        mbar_init(together, 128 * HS);
         *abort_flag = 0;
         mbar_fence_init();
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512)
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kCols)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    if (warp >= 4) {
+        // The query tile, a row by D / 8 lanes.
+        constexpr uint32_t kLanes = D / 8, kRows = 128 * HS / kLanes, kIts = 128 / kRows;  // rows at a time; rounds
+        constexpr uint32_t kBatch = kIts < 8 ? kIts : 8;                                   // loads in flight
+        const uint32_t base_row = uint32_t(tid - 128) / kLanes, c = uint32_t(tid) % kLanes;
+        uint8_t* qd = qsm + (c >> 3) * 16384;
+#pragma unroll
+        for (uint32_t it = 0; it < kIts; it += kBatch) {
+            uint4 x[kBatch];
+#pragma unroll
+            for (uint32_t k = 0; k < kBatch; ++k) {
+                const uint32_t r = min(m0 + base_row + (it + k) * kRows, m_end - 1), i = row_div(r);
+                x[k] = __ldg(reinterpret_cast<const uint4*>(P.q + uint64_t(b) * P.q_seq + uint64_t(i) * P.q_row +
+                                                            uint64_t(h * G + (r - i * G)) * P.q_head) + c);
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < kBatch; ++k) {
+                // (rows past the last hold copies of it: computed and not written)
+                const uint32_t row = base_row + (it + k) * kRows;
+                *reinterpret_cast<uint4*>(qd + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = x[k];
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
     tc_fence_before();
-    __syncthreads();
+    // The loads need the barriers alone, which their own thread has set up (and the page
+    // table): over a dense cache they start at once.
+    if (MODE == kAtWindow && warp == 0) {
+        __threadfence_block();
+        asm volatile("bar.arrive 1, %0;" ::"n"(ac_threads(D)) : "memory");
+    } else {
+        named_sync(1, ac_threads(D));
+    }
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = warp ? *tmem_slot : 0;
 
     // Ring order of the tiles, the order in which the products take them.
-    // MT = 2: K0 V0 K1 V1 ..; MT = 1: K0 K1 V0 K2 V1 .. V(n - 1).
-    auto k_seq = [&](uint32_t j) { return MT == 2 ? 2 * j : (j ? 2 * j - 1 : 0); };
-    auto v_seq = [&](uint32_t j) { return MT == 2 ? 2 * j + 1 : (j + 1 == n ? 2 * n - 1 : 2 * j + 2); };
+    // One S: K0 V0 K1 V1 ..; two: K0 K1 V0 K2 V1 .. V(n - 1).
+    auto k_seq = [&](uint32_t j) { return SB == 1 ? 2 * j : (j ? 2 * j - 1 : 0); };
+    auto v_seq = [&](uint32_t j) { return SB == 1 ? 2 * j + 1 : (j + 1 == n ? 2 * n - 1 : 2 * j + 2); };
     // Whether some row of the CTA does not see all of tile t.
     auto in_part = [&](uint32_t t) -> bool {
         if constexpr (MODE == kAtWindow) {
@@ -281,9 +314,9 @@ __global__ void __launch_bounds__(ac_threads(D), 1)
         }
     };
 
-    // MT = 2: registers go to the softmax warps, 4 x 32 x 72 + 8 x 32 x 216 = 384 x 168.
+    // Two CTAs per SM: registers go to the softmax warps, 4 x 32 x 56 + 4 x 32 x 200 = 256 x 128.
     if (warp < 4) {
-        if constexpr (MT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if constexpr (HS == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 0) {
             // ---- TMA producer ----
             if (lane == 0) {
@@ -306,7 +339,7 @@ __global__ void __launch_bounds__(ac_threads(D), 1)
                     for (uint32_t sub = 0; sub < U; ++sub) {
                         const uint32_t idx = q * U + sub, s = idx % NU;
                         while (idx >= NU && freed <= (idx - NU) / U) {  // the tile whose unit this one replaces
-                            if (!mbar_wait(&empty[freed % NB], (freed / NB) & 1)) {
+                            if (!mbar_wait(&done[freed % NB], (freed / NB) & 1)) {
                                 record_error(P.status, KVM_ERR_TIMEOUT, 125);
                                 if (sub) ac_complete_tx(bar, bytes - sent);  // copies of this tile that are not started
                                 return false;
@@ -342,25 +375,25 @@ __global__ void __launch_bounds__(ac_threads(D), 1)
                 bool ok = true;
                 if (n) {
                     ok = load(0, false);
-                    if (MT == 1 && n > 1) ok = ok && load(1, false);
+                    if (SB == 2 && n > 1) ok = ok && load(1, false);
                     for (uint32_t j = 0; j < n && ok && !*abort_flag; ++j) {
                         ok = load(j, true);
-                        if (ok && j + (3 - MT) < n) ok = load(j + (3 - MT), false);
+                        if (ok && j + SB < n) ok = load(j + SB, false);
                     }
                 }
                 if (!ok) *abort_flag = 1;
                 // Every issued copy lands before the CTA frees its shared memory.
                 for (uint32_t q = tiles_issued > NB ? tiles_issued - NB : 0; q < tiles_issued; ++q)
-                        if (!mbar_wait(&full[q % NB], (q / NB) & 1)) record_error(P.status, KVM_ERR_TIMEOUT, 126);
+                    if (!mbar_wait(&full[q % NB], (q / NB) & 1)) record_error(P.status, KVM_ERR_TIMEOUT, 126);
             }
         } else if (warp == 1) {
-            // ---- MMA issue; step w = (tile w / MT, M tile w % MT), S slot w & 1 ----
+            // ---- MMA issue: tile j, S accumulator j % SB ----
             // The warp only adds constants to descriptors and ring positions.
             constexpr uint32_t idesc_s = pf_idesc(128, kAcKeys, BF16, false);
             constexpr uint32_t idesc_o = pf_idesc(128, D, BF16, true);
             const uint64_t qdesc = tc_desc_sw128(smem_u32(qsm)), kdesc = tc_desc_sw128(smem_u32(ring));
             const uint64_t vdesc = pf_desc_mn_sw128(smem_u32(ring), VK * 128);
-            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), steps = __shfl_sync(0xffffffffu, n, 0);
             struct Pos {  // a unit of the ring; a tile's barrier and the parity of its pass
                 uint32_t s, b, ph;
                 __device__ __forceinline__ void unit() { s = s + 1 == NU ? 0 : s + 1; }
@@ -375,40 +408,29 @@ __global__ void __launch_bounds__(ac_threads(D), 1)
             };
             Pos kp{0, 0, 0}, vp{0, 0, 0};
             vp.skip();
-            if (MT == 1 && n > 1) vp.skip();
+            if (SB == 2 && steps > 1) vp.skip();
             int err = 0;
-            // S of M tile m from the K tile at kp; the last M tile moves kp on.
-            auto issue_s = [&](uint32_t slot, uint32_t m, bool first) -> bool {
+            // S from the K tile at kp, which moves on (over the V tile in between, but for K1 of two).
+            auto issue_s = [&](uint32_t slot, bool over) -> bool {
                 if (!pf_warp_wait(&full[kp.b], kp.ph)) return false;
                 tc_fence_after();
-                Pos k = kp;
-                const uint64_t qd = qdesc + m * (kQTile >> 4);
 #pragma unroll
                 for (uint32_t a = 0; a < U; ++a) {
-                    const uint64_t kd = kdesc + k.s * (kAcUnit >> 4);
+                    const uint64_t kd = kdesc + kp.s * (kAcUnit >> 4);
 #pragma unroll
                     for (uint32_t kk = 0; kk < 4; ++kk)
-                        ac_mma(tm + slot * 128, qd + a * (16384 >> 4) + kk * 2, kd + kk * 2, idesc_s, (a | kk) != 0);
-                    k.unit();
+                        ac_mma(tm + slot * 128, qdesc + a * (16384 >> 4) + kk * 2, kd + kk * 2, idesc_s, (a | kk) != 0);
+                    kp.unit();
                 }
-                ac_commit(&s_full[slot]);
-                if (m == MT - 1) {
-                    ac_commit(&empty[k.b]);
-                    k.tile();
-                    kp = k;
-                    if (MT == 2 || !first) kp.skip();  // over the V tile in between
-                }
+                ac_commit(&done[kp.b]);
+                kp.tile();
+                if (over) kp.skip();
                 return true;
             };
-            const uint32_t steps = __shfl_sync(0xffffffffu, n * MT, 0);
-            if (!pf_warp_wait(q_full, 0)) err = 130;
-            tc_fence_after();
-            for (uint32_t w = 0; w < 2 && w < steps && !err; ++w)
-                if (!issue_s(w, w % MT, w == 0)) err = 131;
-            uint32_t ph = 0;  // parity of P's barriers
-            for (uint32_t w = 0; w < steps && !err; ++w) {
-                const uint32_t slot = w & 1, m = w % MT;
-                const bool more = w >= uint32_t(MT);  // O holds something
+            for (uint32_t j = 0; j < SB && j < steps && !err; ++j)
+                if (!issue_s(j, SB == 1 || j > 0)) err = 131;
+            for (uint32_t j = 0; j < steps && !err; ++j) {
+                const uint32_t slot = j % SB, ph = (j / SB) & 1;
                 if (!pf_warp_wait(&full[vp.b], vp.ph)) err = 133;
                 if (!err && !pf_warp_wait(&p_full[slot], ph)) err = 132;
                 if (err || __shfl_sync(0xffffffffu, *abort_flag, 0)) {
@@ -416,31 +438,25 @@ __global__ void __launch_bounds__(ac_threads(D), 1)
                     break;
                 }
                 tc_fence_after();
-                Pos v = vp;
 #pragma unroll
                 for (uint32_t a = 0; a < U; ++a) {
-                    const uint64_t vd = vdesc + v.s * (kAcUnit >> 4);
+                    const uint64_t vd = vdesc + vp.s * (kAcUnit >> 4);
 #pragma unroll
                     for (uint32_t kk = 0; kk < VK / 16; ++kk) {  // P: 16 keys = 8 tensor-memory columns
                         if (a * VK + kk * 16 == 64) {
                             if (!pf_warp_wait(&p_half[slot], ph)) err = 136;
                             tc_fence_after();
                         }
-                        ac_mma_ts(tm + kColO + m * D, tm + slot * 128 + (a * (VK / 16) + kk) * 8, vd + kk * (2048 >> 4), idesc_o,
-                                  more || (a | kk) != 0);
+                        ac_mma_ts(tm + kColO, tm + slot * 128 + (a * (VK / 16) + kk) * 8, vd + kk * (2048 >> 4), idesc_o,
+                                  j > 0 || (a | kk) != 0);
                     }
-                    v.unit();
+                    vp.unit();
                 }
-                ac_commit(&pv_done[slot]);
-                if (m == MT - 1) {
-                    ac_commit(&empty[v.b]);
-                    v.tile();
-                    vp = v;
-                    // Over the K tile in between; none stands before the last V tile of MT = 1.
-                    if (MT == 2 || w + 2 < steps) vp.skip();
-                }
-                if (!err && w + 2 < steps && !issue_s(slot, m, false)) err = 131;
-                if (slot) ph ^= 1;
+                ac_commit(&done[vp.b]);
+                vp.tile();
+                // Over the K tile in between; of two S none stands before the last V tile.
+                if (SB == 1 || j + 2 < steps) vp.skip();
+                if (!err && j + SB < steps && !issue_s(slot, true)) err = 131;
             }
             if (err > 0 && lane == 0) {
                 record_error(P.status, KVM_ERR_TIMEOUT, err);
@@ -450,8 +466,7 @@ __global__ void __launch_bounds__(ac_threads(D), 1)
             ac_commit(fin);
             if (!pf_warp_wait(fin, 0) && lane == 0) record_error(P.status, KVM_ERR_TIMEOUT, 134);
         } else {
-            // ---- warps 2 and 3: V tiles that some row does not see in full are looked through for
-            // infinities and NaN (0 * x is NaN for the rows that must not see them) ----
+            // ---- warps 2 and 3: V tiles that some row does not see in full are looked through ----
             for (uint32_t j = 0; j < n; ++j) {
                 const uint32_t q = v_seq(j);
                 const bool ok = pf_warp_wait(&full[q % NB], (q / NB) & 1);
@@ -476,26 +491,19 @@ __global__ void __launch_bounds__(ac_threads(D), 1)
             }
         }
     } else {
-        if constexpr (MT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        // ---- softmax: thread = packed row = tensor-memory lane ----
-        const uint32_t m = uint32_t(tid - 128) / 128, row = uint32_t(tid - 128) % 128;
+        if constexpr (HS == 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        // ---- softmax: thread = packed row (tensor-memory lane), NK of the tile's keys ----
+        // With two warps per 32 rows these exchange their maxes through shared memory, behind a
+        // barrier of their own. A warp that gives up raises the abort flag and then arrives there,
+        // and its partner looks at the flag behind every such barrier: no wait stays open.
+        constexpr int NK = kAcKeys / HS, NW = NK / 32;
+        const uint32_t half = HS == 2 ? uint32_t(tid - 128) / 128 : 0, row = uint32_t(tid) & 127;
         const uint32_t lane_addr = tmem + ((32u * uint32_t(warp & 3)) << 16);
-        const uint32_t r = m0 + m * 128 + row;  // packed row
-        const uint32_t ri = min(r, m_end - 1) / G;
+        const uint32_t r = m0 + row;  // packed row
+        const uint32_t ri = row_div(min(r, m_end - 1));
         const uint32_t qh = h * G + (min(r, m_end - 1) - ri * G);
-        {
-            const uint4* qp = reinterpret_cast<const uint4*>(P.q + uint64_t(b) * P.q_seq + uint64_t(ri) * P.q_row +
-                                                             uint64_t(qh) * P.q_head);
-            uint8_t* qd = qsm + m * kQTile + row * 128;
-            uint4 x[D / 8];
-#pragma unroll
-            for (uint32_t c = 0; c < D / 8; ++c) x[c] = r < m_end ? __ldg(qp + c) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (uint32_t c = 0; c < D / 8; ++c)
-                *reinterpret_cast<uint4*>(qd + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4)) = x[c];
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(q_full);
-        }
+        const uint32_t pair = 2 + uint32_t(warp & 3);  // barrier
+        float* xch = pair_max + row;
         const float c2 = P.scale_log2;
         float m_used = -1e30f, l = 0.f;
         bool ok = true;
@@ -505,80 +513,82 @@ __global__ void __launch_bounds__(ac_threads(D), 1)
             ok = pf_warp_wait(together, meet_phase) && ok;
             meet_phase ^= 1;
         };
+        auto pair_sync = [&] {
+            if constexpr (HS == 2) named_sync(pair, 64);
+            ok = ok && !__shfl_sync(0xffffffffu, *abort_flag, 0);
+        };
         auto below = [](int x, int q4) -> uint32_t {  // bits of the keys < x in word q4
             const int y = min(max(x - q4 * 32, 0), 32);
             return y == 32 ? ~0u : (1u << y) - 1u;
         };
-        const uint32_t col_o = lane_addr + kColO + m * D;
+        const uint32_t col_o = lane_addr + kColO + half * (D / HS);  // this thread's part of the row's O
         for (uint32_t j = 0; j < n; ++j) {
-            const uint32_t w = j * MT + m, slot = w & 1, t = tb + j;
-            if (__shfl_sync(0xffffffffu, *abort_flag, 0)) {
-                ok = false;
-                break;
-            }
-            // Which of the tile's keys this row sees; `part`: some row of the CTA does not see all.
-            uint32_t see[4] = {~0u, ~0u, ~0u, ~0u};
+            const uint32_t slot = j % SB, t = tb + j;
+            // Which of its keys this row sees; `part`: some row of the CTA does not see all of the tile.
+            uint32_t see[NW];
+#pragma unroll
+            for (int q = 0; q < NW; ++q) see[q] = ~0u;
             const bool part = in_part(t);
-            if constexpr (MODE == kAtWindow) {
-                const uint32_t a = t < n_first ? t * kAcKeys : lo + (t - n_first) * kAcKeys;
-                const uint32_t end = t < n_first ? few : hi;
-                if (part) {
+            if (part) {
+                if (MODE == kAtWindow) {
                     // Keys [0, s1) u [w0, u1) of the tile: sinks, and the window up to the row's position.
-                    const uint32_t p = p0 + (ri - i0);
+                    const uint32_t a = t < n_first ? t * kAcKeys : lo + (t - n_first) * kAcKeys;
+                    const uint32_t end = t < n_first ? few : hi, p = p0 + (ri - i0);
                     const int u1 = int(min(end, p + 1)) - int(a);
                     const int s1 = min(P.sinks > a ? int(min(P.sinks - a, 256u)) : 0, u1);
                     const int w0 = P.window == 0 ? 256 : (p + 1 > P.window ? int(p + 1 - P.window) - int(a) : 0);
 #pragma unroll
-                    for (int q4 = 0; q4 < 4; ++q4) see[q4] = below(s1, q4) | (below(u1, q4) & ~below(w0, q4));
-                }
-            } else if (t >= n_first) {
-                const uint32_t a = (t - n_first) * kAcKeys;
-                if (part) {
-const int rec = int(recent) - int(a);  // keys below are recent tokens, key rec + x is node x
+                    for (int q = 0; q < NW; ++q) {
+                        const int q4 = int(half) * NW + q;
+                        see[q] = below(s1, q4) | (below(u1, q4) & ~below(w0, q4));
+                    }
+                } else if (t >= n_first) {
+                    const int rec = int(recent) - int((t - n_first) * kAcKeys);  // keys below are recent tokens, key rec + x is node x
                     const uint32_t* tw = P.tree ? P.tree + uint64_t(b) * P.tree_seq + uint64_t(ri) * P.tree_words : nullptr;
                     auto word = [&](int i) { return i >= 0 && i < int(P.tree_words) ? __ldg(tw + i) : 0u; };
 #pragma unroll
-                    for (int q4 = 0; q4 < 4; ++q4) {
-                        uint32_t bits;
-                        if (tw) {
-                            const int nd = q4 * 32 - rec;
-                            bits = __funnelshift_r(word(nd >> 5), word((nd >> 5) + 1), nd & 31) & below(rec + int(rows), q4);
-                        } else {
-                            bits = below(rec + int(ri) + 1, q4);
-                        }
-                        see[q4] = bits | below(rec, q4);
+                    for (int q = 0; q < NW; ++q) {
+                        const int q4 = int(half) * NW + q, nd = q4 * 32 - rec;
+                        const uint32_t bits = tw ? __funnelshift_r(word(nd >> 5), word((nd >> 5) + 1), nd & 31) & below(rec + int(rows), q4)
+                                                 : below(rec + int(ri) + 1, q4);
+                        see[q] = bits | below(rec, q4);
                     }
-                }
-            } else {
-                if (part) {
+                } else {
                     const uint32_t first = page_div(t * kAcKeys), last = page_div(min(t * kAcKeys + kAcKeys, n_keys) - 1);
-                    see[0] = see[1] = see[2] = see[3] = 0;
+#pragma unroll
+                    for (int q = 0; q < NW; ++q) see[q] = 0;
                     for (uint32_t e = first; e <= last; ++e) {
                         const int at = int(e * P.page_tokens) - int(t * kAcKeys), end = at + table[e - e0].y;
 #pragma unroll
-                        for (int q4 = 0; q4 < 4; ++q4) see[q4] |= below(end, q4) & ~below(at, q4);
+                        for (int q = 0; q < NW; ++q) see[q] |= below(end, int(half) * NW + q) & ~below(at, int(half) * NW + q);
                     }
                 }
             }
-            if (!pf_warp_wait(&s_full[slot], (w >> 1) & 1)) {
-                ok = false;
-                break;
-            }
+            ok = pf_warp_wait(&done[k_seq(j) % NB], (k_seq(j) / NB) & 1);
+            if (!ok) break;
             tc_fence_after();
-            float x[kAcKeys];
+            float x[NK];
             {
                 uint32_t* u = reinterpret_cast<uint32_t*>(x);
 #pragma unroll
-                for (int q4 = 0; q4 < 4; ++q4) tc_ld32(lane_addr + slot * 128 + q4 * 32, u + q4 * 32);
+                for (int q = 0; q < NW; ++q) tc_ld32(lane_addr + slot * 128 + half * 64 + q * 32, u + q * 32);
 #pragma unroll
-                for (int q4 = 0; q4 < 4; ++q4) tc_wait_ld(u + q4 * 32);
+                for (int q = 0; q < NW; ++q) tc_wait_ld(u + q * 32);
             }
             if (part) {
 #pragma unroll
-                for (int k = 0; k < kAcKeys; ++k)
+                for (int k = 0; k < NK; ++k)
                     if (!((see[k >> 5] >> (k & 31)) & 1)) x[k] = -INFINITY;
             }
-            const float mx = ac_max128(x) * c2;
+            float mx = pf_max64(x);
+            if constexpr (HS == 1) mx = fmaxf(mx, pf_max64(x + 64));
+            mx *= c2;
+            if constexpr (HS == 2) xch[(j & 1) * 256 + half * 128] = mx;
+            tc_fence_before();
+            pair_sync();  // (P of one half goes over S columns that the other half has read by now)
+            if (!ok) break;
+            tc_fence_after();
+            if constexpr (HS == 2) mx = fmaxf(mx, xch[(j & 1) * 256 + (half ^ 1) * 128]);
             const bool need = mx > m_used + kPfRescale;
             if (j == 0) {
                 m_used = fmaxf(mx, -1e30f);
@@ -590,14 +600,11 @@ const int rec = int(recent) - int(a);  // keys below are recent tokens, key rec 
                     l *= alpha;
                 }
                 // O holds the products of the tiles before once the last of them is done.
-                const uint32_t wp = w - MT;
-                if (!pf_warp_wait(&pv_done[wp & 1], (wp >> 1) & 1)) {
-                    ok = false;
-                    break;
-                }
+                ok = pf_warp_wait(&done[v_seq(j - 1) % NB], (v_seq(j - 1) / NB) & 1);
+                if (!ok) break;
                 tc_fence_after();
 #pragma unroll 1
-                for (uint32_t cc = 0; cc < D; cc += 32) {
+                for (uint32_t cc = 0; cc < D / HS; cc += 32) {
                     uint32_t o[32];
                     tc_ld32(col_o + cc, o);
                     tc_wait_ld(o);
@@ -606,159 +613,194 @@ const int rec = int(recent) - int(a);  // keys below are recent tokens, key rec 
                     tc_st32(col_o + cc, o);
                 }
                 tc_wait_st();
+                tc_fence_before();
+                pair_sync();  // both halves of O are rescaled before either half of P is handed over
+                if (!ok) break;
+                tc_fence_after();
             }
-            // P = exp2(x c2 - m), its sum, and P over its S (16-bit, two per column). The first 64 keys go
-            // to the tensor core while the others are worked out.
+            // P = exp2(x c2 - m), its sum, and P over its S (16-bit, two per column). 64 keys at a time go
+            // to the tensor core.
             const float mneg = -m_used;
             float s4[4] = {0.f, 0.f, 0.f, 0.f};
-            auto exps = [&](int q4) {
+            auto exps = [&](int from, int to) {
 #pragma unroll
-                for (int k = q4 * 32; k < q4 * 32 + 32; k += 2) {
+                for (int k = from; k < to; k += 2) {
                     pf_fma2(x[k], x[k + 1], x[k], x[k + 1], c2, mneg);
                     x[k] = fast_exp2(x[k]);
                     x[k + 1] = fast_exp2(x[k + 1]);
                     pf_add2(s4[k & 2], s4[(k & 2) + 1], x[k], x[k + 1]);
                 }
             };
-            auto store = [&](int half) {
+            auto store = [&](int from, uint32_t part64) {
                 uint32_t pk[32];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) pk[i] = pf_pack2<BF16>(x[half * 64 + 2 * i], x[half * 64 + 2 * i + 1]);
-                tc_st32(lane_addr + slot * 128 + half * 32, pk);
+                for (int i = 0; i < 32; ++i) pk[i] = pf_pack2<BF16>(x[from + 2 * i], x[from + 2 * i + 1]);
+                tc_st32(lane_addr + slot * 128 + part64 * 32, pk);
             };
             auto hand_over = [&](uint64_t* bar) {
                 tc_wait_st();
                 tc_fence_before();
                 mbar_arrive(bar);
             };
-            exps(0);
-            exps(1);
+            exps(0, 64);
             ok = pf_warp_wait(&scanned[j % kAcScans], (j / kAcScans) & 1);
             if (!ok) break;
             const bool bad = bad_flag[(j % kAcScans) * 2] | bad_flag[(j % kAcScans) * 2 + 1];
-            if (!bad) {
-                store(0);
-                exps(2);
-                hand_over(&p_full[slot]);
-                exps(3);
-                store(1);
-                hand_over(&p_half[slot]);
+            store(0, half);
+            if constexpr (HS == 1) {
+                exps(64, 96);
+                if (!bad) hand_over(&p_full[slot]);
+                exps(96, 128);
+                store(64, 1);
+                if (!bad) hand_over(&p_half[slot]);
             } else {
-                exps(2);
-                exps(3);
-                store(0);
-                store(1);
+                if (!bad) hand_over(half ? &p_half[slot] : &p_full[slot]);
             }
             l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
             if (bad) {
-                // sums of p * v over the infinite and NaN values this row sees, which leave the product
-                float fix[D], pl[kAcKeys];
+                // Sums of p * v over the infinite and NaN values this row sees, which leave the product.
+                float fix[D], pl[NK];
 #pragma unroll
-                for (int k = 0; k < kAcKeys; ++k) pl[k] = x[k];
+                for (int k = 0; k < NK; ++k) pl[k] = x[k];
+                uint32_t sl[NW];
+#pragma unroll
+                for (int q = 0; q < NW; ++q) sl[q] = see[q];
                 const uint32_t at = v_seq(j) * U;
 #pragma unroll 1
                 for (uint32_t d = 0; d < D; ++d) {
                     float f = 0.f;
 #pragma unroll 1
-                    for (uint32_t k = 0; k < uint32_t(kAcKeys); ++k) {
-                        const uint32_t kr = k % VK;
+                    for (uint32_t k = 0; k < uint32_t(NK); ++k) {
+                        const uint32_t key = half * NK + k, kr = key % VK;
                         const uint16_t bits = *reinterpret_cast<const uint16_t*>(
-                            ring + ((at + k / VK) % NU) * kAcUnit + (d / 64) * VK * 128 + kr * 128 +
+                            ring + ((at + key / VK) % NU) * kAcUnit + (d / 64) * VK * 128 + kr * 128 +
                             ((((d % 64) / 8) ^ (kr & 7)) << 4) + (d % 8) * 2);
-                        if (at_nonfinite<BF16>(bits)) {
-                            const uint32_t sw = k >> 5 == 0 ? see[0] : k >> 5 == 1 ? see[1] : k >> 5 == 2 ? see[2] : see[3];
-                            if ((sw >> (k & 31)) & 1) f += pl[k] * at_unpack<BF16>(bits).x;
-                        }
+                        if (at_nonfinite<BF16>(bits) && ((sl[k >> 5] >> (k & 31)) & 1)) f += pl[k] * at_unpack<BF16>(bits).x;
                     }
                     fix[d] = f;
                 }
                 meet();
-                for (uint32_t a = m; a < U; a += MT) {
+                for (uint32_t a = 0; a < U; ++a) {
                     uint16_t* v2 = reinterpret_cast<uint16_t*>(ring + ((at + a) % NU) * kAcUnit);
-                    for (uint32_t e = row; e < kAcUnit / 2; e += 128)
+                    for (uint32_t e = uint32_t(tid - 128); e < kAcUnit / 2; e += 128 * HS)
                         if (at_nonfinite<BF16>(v2[e])) v2[e] = 0;
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 meet();
-                hand_over(&p_full[slot]);
-                mbar_arrive(&p_half[slot]);
-                if (!ok || !pf_warp_wait(&pv_done[slot], (w >> 1) & 1)) {
-                    ok = false;
-                    break;
+                if constexpr (HS == 1) {
+                    hand_over(&p_full[slot]);
+                    mbar_arrive(&p_half[slot]);
+                } else {
+                    hand_over(half ? &p_half[slot] : &p_full[slot]);
                 }
-                tc_fence_after();
+                ok = ok && pf_warp_wait(&done[v_seq(j) % NB], (v_seq(j) / NB) & 1);
+                for (uint32_t turn = 0; turn < uint32_t(HS); ++turn) {  // each part of the keys adds to the whole row
+                    tc_fence_after();
+                    if (ok && turn == half) {
 #pragma unroll 1
-                for (uint32_t cc = 0; cc < D; cc += 32) {
-                    uint32_t o[32];
-                    tc_ld32(col_o + cc, o);
-                    tc_wait_ld(o);
+                        for (uint32_t cc = 0; cc < D; cc += 32) {
+                            uint32_t o[32];
+                            tc_ld32(lane_addr + kColO + cc, o);
+                            tc_wait_ld(o);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) + fix[cc + i]);
-                    tc_st32(col_o + cc, o);
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) + fix[cc + i]);
+                            tc_st32(lane_addr + kColO + cc, o);
+                        }
+                        tc_wait_st();
+                    }
+                    tc_fence_before();
+                    meet();
                 }
-                tc_wait_st();
-                tc_fence_before();
+                if (!ok) break;
             }
         }
         grid_release();
-        const bool go = __shfl_sync(0xffffffffu, (ok && !*abort_flag) ? 1 : 0, 0) != 0;
-        if (go) {
-            const uint32_t wl = (n - 1) * MT + m;
-            if (n == 0 || pf_warp_wait(&pv_done[wl & 1], (wl >> 1) & 1)) {
-                tc_fence_after();
-                const bool valid = r < m_end;
-                const uint64_t row_id = (uint64_t(b) * P.width + ri) * P.q_heads + qh;
-                const uint64_t id = uint64_t(split) * P.seqs * P.width * P.q_heads + row_id;
-                const float inv = l == 0.f ? 0.f : 1.f / l;
-                float* prow_o = P.part_o + id * D;
-                uint8_t* orow = P.out + uint64_t(b) * P.o_seq + uint64_t(ri) * P.o_row + uint64_t(qh) * P.o_head;
-                if (n) {
+        if (ok) ok = n == 0 || pf_warp_wait(&done[v_seq(n - 1) % NB], (v_seq(n - 1) / NB) & 1);
+        if (HS == 2 && ok) {
+            xch[(n & 1) * 256 + half * 128] = l;
+            pair_sync();
+            l += xch[(n & 1) * 256 + (half ^ 1) * 128];
+        }
+        if (ok) {
+            tc_fence_after();
+            const bool valid = r < m_end;
+            const uint64_t row_id = (uint64_t(b) * P.width + ri) * P.q_heads + qh;
+            const uint64_t id = uint64_t(split) * P.seqs * P.width * P.q_heads + row_id;
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            constexpr uint32_t kCol = D / HS, kRowBytes = 2 * kCol;  // columns of this thread; bytes of a staged row
+            uint8_t* orow = P.out + uint64_t(b) * P.o_seq + uint64_t(ri) * P.o_row + uint64_t(qh) * P.o_head + half * kRowBytes;
+            // Rows go through shared memory (the warp's share of the query tile, which every S has left) so
+            // that a warp writes whole lines: 32 lanes with a row each would write 32 lines at a time.
+            uint8_t* stage = qsm + uint32_t(warp - 4) * (32 * kRowBytes);
+            uint8_t* srow = stage + lane * kRowBytes;
+            const bool parts = P.splits > 1;
+            uint64_t dst0 = parts ? reinterpret_cast<uint64_t>(P.part_o + id * D + half * kCol) : reinterpret_cast<uint64_t>(orow);
+            if (!valid) dst0 = 0;
+            constexpr uint32_t kChunks = kRowBytes / 16;  // 8, 16 or 32
+            for (uint32_t pass = 0; n && pass < (parts ? 2u : 1u); ++pass) {  // 32-bit rows in two parts
+                const uint32_t c0 = parts ? pass * (kCol / 2) : 0, c1 = parts ? c0 + kCol / 2 : kCol;
 #pragma unroll 1
-                    for (uint32_t cc = 0; cc < D; cc += 32) {
-                        uint32_t o[32];
-                        tc_ld32(col_o + cc, o);
-                        tc_wait_ld(o);
-                        if (!valid) continue;
-                        if (P.splits > 1) {
-                            float4* dst = reinterpret_cast<float4*>(prow_o + cc);
+                for (uint32_t cc = c0; cc < c1; cc += 32) {
+                    uint32_t o[32];
+                    tc_ld32(col_o + cc, o);
+                    tc_wait_ld(o);
+                    if (parts) {
 #pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                dst[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
-                                                     __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
-                        } else {
-                            uint4* dst = reinterpret_cast<uint4*>(orow + cc * 2);
+                        for (uint32_t i = 0; i < 8; ++i)
+                            *reinterpret_cast<uint4*>(srow + ((((cc - c0) / 4 + i) ^ (lane & 7)) << 4)) =
+                                make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    } else {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                uint32_t y[4];
+                        for (uint32_t i = 0; i < 4; ++i) {
+                            uint32_t y[4];
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    // A row that sees no key has a zero sum; its product is 0.
-                                    y[e] = pf_pack2<BF16>(__uint_as_float(o[8 * i + 2 * e]) * inv,
-                                                          __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
-                                }
-                                dst[i] = make_uint4(y[0], y[1], y[2], y[3]);
-                            }
+                            for (int e = 0; e < 4; ++e)  // (a row that sees no key has a zero sum; its product is 0)
+                                y[e] = pf_pack2<BF16>(__uint_as_float(o[8 * i + 2 * e]) * inv,
+                                                      __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
+                            *reinterpret_cast<uint4*>(srow + (((cc / 8 + i) ^ (lane & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
                         }
                     }
                 }
-                if (n == 0 && valid && P.splits == 1)  // nothing to see
-                    for (uint32_t c = 0; c < D / 8; ++c) reinterpret_cast<uint4*>(orow)[c] = make_uint4(0, 0, 0, 0);
-                if (valid && P.splits > 1) P.part_ml[id] = make_float2(l == 0.f ? -INFINITY : m_used, l);
-                if (valid && P.splits == 1 && P.lse) P.lse[row_id] = l == 0.f ? -INFINITY : (m_used + log2f(l)) * kAtLn2;
-            } else {
-                ok = false;
+                __syncwarp();
+                constexpr uint32_t kStep = 32 / kChunks;  // rows at a time, eight rounds in flight
+                const uint32_t c = uint32_t(lane) % kChunks;
+#pragma unroll 1
+                for (uint32_t r0 = uint32_t(lane) / kChunks; r0 < 32; r0 += 8 * kStep) {
+                    uint4 y[8];
+                    uint64_t to[8];
+#pragma unroll
+                    for (uint32_t k = 0; k < 8; ++k) {
+                        const uint32_t rr = r0 + k * kStep;
+                        to[k] = __shfl_sync(0xffffffffu, dst0, rr);
+                        y[k] = *reinterpret_cast<const uint4*>(stage + rr * kRowBytes + ((c ^ (rr & 7)) << 4));
+                    }
+#pragma unroll
+                    for (uint32_t k = 0; k < 8; ++k)
+                        if (to[k]) reinterpret_cast<uint4*>(to[k])[pass * kChunks + c] = y[k];
+                }
+                __syncwarp();
             }
-        }
-        if (!ok) {
-            record_error(P.status, KVM_ERR_TIMEOUT, 135);
-            *abort_flag = 1;
+            if (n == 0 && valid && P.splits == 1)  // nothing to see
+                for (uint32_t c = 0; c < kChunks; ++c) reinterpret_cast<uint4*>(orow)[c] = make_uint4(0, 0, 0, 0);
+            if (valid && half == 0) {
+                if (parts) P.part_ml[id] = make_float2(l == 0.f ? -INFINITY : m_used, l);
+                else if (P.lse) P.lse[row_id] = l == 0.f ? -INFINITY : (m_used + log2f(l)) * kAtLn2;
+            }
+        } else {
+            if (lane == 0) {
+                record_error(P.status, KVM_ERR_TIMEOUT, 135);
+                *abort_flag = 1;
+            }
+            __syncwarp();
+            __threadfence_block();
+            if constexpr (HS == 2) asm volatile("bar.arrive %0, 64;" ::"r"(pair) : "memory");
         }
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     if (warp == 1)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
 }
 
 }  // namespace kvmb

@@ -9,13 +9,13 @@ namespace kvmb {
 template <int D, bool BF16, int MODE>
 int launch_attend_tc_k(kvm_ctx* c, const AttendTcMaps& maps, const AttendParams& p, uint32_t box, cudaStream_t s) {
     auto fn = attend_tc_kernel<D, BF16, MODE>;
-    if constexpr (ac_mt(D) == 2) {
-        // The register split needs every register of 384 x 168: with fewer the warps would wait for more for ever.
+    if constexpr (ac_halves(D) == 1) {
+        // The register split needs every register of 256 x 128: with fewer the warps would wait for more for ever.
         static const int regs = [&] {
             cudaFuncAttributes a{};
             return cudaFuncGetAttributes(&a, fn) == cudaSuccess ? a.numRegs : 0;
         }();
-        if (regs < 168) return KVM_ERR_CUDA;
+        if (regs != 128) return KVM_ERR_CUDA;
     }
     constexpr uint32_t smem = ac_smem_bytes(D, MODE);
     if (smem_attr(reinterpret_cast<const void*>(fn), int(smem)) != cudaSuccess) return KVM_ERR_CUDA;

@@ -2257,6 +2257,14 @@ int ensure_attn_ws(kvm_ctx* c, size_t bytes, cudaStream_t s, void** out) {
     return KVM_OK;
 }
 
+// u / d = (u * magic) >> shift for u < 2^31: magic = ceil(2^shift / d) with 2^shift >= 2^32 d / 2.
+void division(uint32_t d, uint64_t* magic, uint32_t* shift) {
+    uint32_t lg = 0;
+    while ((1ull << lg) < d) ++lg;
+    *shift = 32 + lg;
+    *magic = ((1ull << *shift) + d - 1) / d;
+}
+
 // Checks and fills what both attention calls share: heads, rows, q / out, the dense keys.
 int attend_common(const kvm_ctx* c, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, int32_t type, uint32_t seqs,
                   uint32_t width, float scale, const kvm_rows* q, const kvm_kcache* k, const kvm_kcache* v,
@@ -2289,6 +2297,7 @@ int attend_common(const kvm_ctx* c, uint32_t q_heads, uint32_t kv_heads, uint32_
     p->o_seq = out->seq_stride, p->o_row = out->row_stride, p->o_head = out->head_stride;
     p->lse = lse;
     p->seqs = seqs, p->width = width, p->q_heads = q_heads, p->kv_heads = kv_heads, p->group = q_heads / kv_heads;
+    division(p->group, &p->g_magic, &p->g_shift);
     p->scale_log2 = (scale > 0.f ? scale : 1.f / std::sqrt(float(head_dim))) * 1.4426950408889634f;
     p->k = static_cast<const uint8_t*>(k->data), p->v = static_cast<const uint8_t*>(v->data);
     p->k_seq = k->layer_stride, p->k_tok = k->token_stride, p->k_head = k->head_stride;
@@ -2394,8 +2403,7 @@ int attend_launch(kvm_ctx* c, AttendParams& p, uint32_t head_dim, bool bf16, int
         std::memset(&maps, 0, sizeof maps);
         uint32_t box = 0;
         if (attend_tc_maps(p, head_dim, bf16, mode, pool_rows, &maps, &box)) {
-            const uint32_t m = 128u * ac_mt(int(head_dim));
-            p.m_tiles = (packed + m - 1) / m;
+            p.m_tiles = (packed + 127) / 128;
             // One CTA's chunk touches at most kAcTable pages
             uint32_t least = 1;
             bool too_many = false;
@@ -2408,7 +2416,7 @@ int attend_launch(kvm_ctx* c, AttendParams& p, uint32_t head_dim, bool bf16, int
             }
             if (!too_many) {
                 const uint64_t tiles = (keys + kAcKeys - 1) / kAcKeys + 1;
-                p.splits = attend_splits(c, uint64_t(p.seqs) * p.kv_heads * p.m_tiles, uint64_t(c->num_sms), tiles, 1.6, 5.0,
+                p.splits = attend_splits(c, uint64_t(p.seqs) * p.kv_heads * p.m_tiles, uint64_t(c->num_sms) * ac_ctas(int(head_dim)), tiles, 1.7, 6.0,
                                          rows, row_bytes, least);
                 KVM_TRY(attend_scratch(c, p, head_dim, s));
                 KVM_TRY(bf16 ? launch_attend_tc_t<true>(c, maps, p, head_dim, mode, box, s)
@@ -2471,8 +2479,8 @@ int kvm_window_attention(kvm_ctx* c, const kvm_window_desc* d, const kvm_rows* q
     p.seq_rows = d->seq_rows;
     p.window = d->window;
     p.sinks = d->sinks;
-    // Keys of the longest unit: the sinks, the window and the rows of an M tile (at most 256 packed).
-    const uint64_t reach = uint64_t(d->window) + std::min<uint64_t>(d->width, 256 / p.group + 2);
+    // Keys of the longest unit: the sinks, the window and the rows of an M tile (at most 128 packed).
+    const uint64_t reach = uint64_t(d->window) + std::min<uint64_t>(d->width, 128 / p.group + 2);
     const uint64_t keys = std::min<uint64_t>(std::min<uint64_t>(d->sinks, p.capacity) + reach, p.capacity);
     DeviceGuard guard(c->device);
     return attend_launch(c, p, d->head_dim, d->type == KVM_BF16, kAtWindow, false, keys, 0, 0, 0,
@@ -2529,10 +2537,7 @@ int kvm_tree_attention(kvm_ctx* c, const kvm_pool* pool, const kvm_tree_desc* d,
     p.row0 = d->row0, p.row_step = d->row_step;
     p.sel_ids = d->sel_ids, p.sel_n = d->sel_n, p.sel_stride = d->sel_stride;
     p.page_tokens = d->page_tokens;
-    uint32_t lg = 0;
-    while ((1ull << lg) < d->page_tokens) ++lg;
-    p.pt_shift = 32 + lg;
-    p.pt_magic = ((1ull << p.pt_shift) + d->page_tokens - 1) / d->page_tokens;
+    division(d->page_tokens, &p.pt_magic, &p.pt_shift);
     p.tokens = d->tokens, p.seq_tokens = d->seq_tokens;
     p.recent = d->recent, p.seq_recent = d->seq_recent;
     p.seq_rows = d->seq_rows;
