@@ -2,32 +2,35 @@
 // same operators as attend.cuh (window with sinks, tree over pages), for packed row
 // counts where the products and not the reading of K and V bound the time.
 //
-// One CTA per (sequence, KV head, 128 packed rows, key chunk); one per SM at head_dim
-// 256, two at 64 / 128, so that one's start, end and softmax run beside the other's
-// products:
-//  * warp 0 (one thread): TMA loads of 128-key tiles into one ring of 16 KiB
-//    units, K and V in the order in which the products take them. A K unit is 128
-//    keys x 64 dims (the B operand of S, K-major); a V unit is 32 / 64 / 128 keys x
-//    256 / 128 / 64 dims (the B operand of O, MN-major). Pages come as boxes of gcd(page_tokens, 128) tokens, each from its slot;
+// One CTA per (sequence, KV head, 128 packed rows, key chunk), in one of two shapes
+// (ac_wide): one CTA per SM, or two, so that one's start, end and softmax run beside the
+// other's products:
+//  * warp 0, in the wide shape also warp 2 (one thread each): TMA loads of 128-key K and V
+//    tiles into one ring of 16 KiB units, in the order in which the products take them. A
+//    K unit is 128 keys x 64 dims (the B operand of S, K-major); a V unit is 32 / 64 / 128
+//    keys x 256 / 128 / 64 dims (the B operand of O, MN-major). Pages come as boxes of
+//    gcd(page_tokens, 128) tokens, each from its slot;
 //  * warp 1: tcgen05.mma kind::f16, S = Q K^T (M = 128, N = 128, Q in shared memory),
-//    then O += P V (N = head_dim, P from tensor memory, where it replaces its S). At
-//    head_dim 256 two S accumulators are in flight (S of tile j + 2 is issued right
-//    behind P V of tile j); at 64 / 128 each CTA has one, and the tensor core works
-//    for the SM's other CTA meanwhile. One commit per product serves the softmax and
-//    the ring (a commit costs the tensor core some 100 cycles: with one for each use
-//    and unit a tile took 4,400 cycles instead of 3,300 at head_dim 256);
-//  * softmax warps: thread = packed row = tensor-memory lane; four warps, or eight at
-//    head_dim 256, each with half of the tile's keys. Masks are words of bits per
+//    then O += P V (N = head_dim, P from tensor memory, where it replaces its S). In
+//    the wide shape two S accumulators are in flight (S of tile j + 2 is issued right
+//    behind P V of tile j); in the narrow one the tensor core works for the SM's other
+//    CTA meanwhile. One commit per product serves the softmax and the ring (a commit
+//    costs the tensor core some 100 cycles: with one for each use and unit a tile took
+//    4,400 cycles instead of 3,300 at head_dim 256);
+//  * softmax warps: thread = packed row = tensor-memory lane; four warps, or eight in the
+//    wide shape, each with half of the tile's keys. Masks are words of bits per
 //    thread and tile, made only for tiles that some row sees in part. The running max
 //    moves lazily: O is rescaled only when it grows by more than 2^8, so P stays
 //    below 2^8 and sums stay in 32 bits. P goes to the tensor core in two halves;
-//  * warps 2 and 3: a V tile behind a mask may hold infinities or NaN, which 0 * x
-//    would spread to rows that do not see them. Such tiles are looked through; where
-//    one holds such values they are taken out of the product and added by hand to the
-//    rows that do see them.
+//  * warp 3 (and 2): a V tile behind a mask may hold infinities or NaN, which 0 * x
+//    would spread to rows that do not see them. Keys that no row sees become zeros; the
+//    others are looked through, and where some rows see such a value it is taken out of
+//    the product and added by hand to those rows.
 // Every wait is bounded: on expiry the kernel records KVM_ERR_TIMEOUT, raises the
 // CTA's abort flag, lets copies and MMAs in flight finish and frees its TMEM.
 #pragma once
+#include <type_traits>
+
 #include "attend.cuh"
 #include "prefill_attn.cuh"
 
@@ -35,26 +38,29 @@ namespace kvmb {
 
 constexpr int kAcKeys = 128;             // keys per tile
 constexpr uint32_t kAcUnit = 16384;      // bytes per ring unit
-constexpr uint32_t kAcTable = 512;       // page entries of one CTA's key chunk
-constexpr uint32_t kAcScans = 8;         // V tiles that the scan may be ahead of the softmax, and one
-constexpr uint32_t kAcMaxTiles = 7;
+constexpr uint32_t kAcTable = 512;       // page boxes of one CTA's key chunk
+constexpr uint32_t kAcScans = 8;         // V tiles that the scan's barriers tell apart
+constexpr uint32_t kAcMaxTiles = 14;
 
-__host__ __device__ constexpr int ac_ctas(int D) { return D == 256 ? 1 : 2; }      // CTAs per SM
-__host__ __device__ constexpr int ac_halves(int D) { return D == 256 ? 2 : 1; }    // softmax warps per 32 rows
-__host__ __device__ constexpr int ac_threads(int D) { return 128 + 128 * ac_halves(D); }
+// Two shapes. Wide: one CTA per SM, two S accumulators, eight softmax warps, a deep ring.
+// Narrow (a dense cache up to head_dim 128, whose tiles many rows share in L2): two CTAs
+// per SM, each with one S accumulator and four softmax warps.
+__host__ __device__ constexpr bool ac_wide(int D, int mode) { return D == 256 || mode == kAtTree; }
+__host__ __device__ constexpr int ac_threads(int D, int mode) { return ac_wide(D, mode) ? 384 : 256; }
 __host__ __device__ constexpr uint32_t ac_units(int D, int mode) {
     // What is left of the SM's 227 KiB (or half of it) beside the query tile and the page table.
-    return D == 256 ? (mode == kAtTree ? 9u : 10u) : D == 128 ? 4u : 5u;
+    return !ac_wide(D, mode) ? (D == 128 ? 4u : 5u) : D == 256 ? (mode == kAtTree ? 9u : 10u) : D == 128 ? 11u : 12u;
 }
 // A K or V tile (D / 64 units) has one full barrier; that of tile q serves tile q +
 // ac_tiles again, whose first unit waits for a unit of a tile behind q.
 __host__ __device__ constexpr uint32_t ac_tiles(int D, int mode) { return ac_units(D, mode) / uint32_t(D / 64) + 2u; }
 __host__ __device__ constexpr uint32_t ac_smem_bytes(int D, int mode) {
-    return 128u * uint32_t(D) * 2u + ac_units(D, mode) * kAcUnit + (ac_halves(D) == 2 ? 2048u : 0u) +
-           (mode == kAtTree ? kAcTable * 8u : 0u) + 512u;
+    return 128u * uint32_t(D) * 2u + ac_units(D, mode) * kAcUnit + (ac_wide(D, mode) ? 2048u : 0u) +
+           (mode == kAtTree ? kAcTable * 8u : 0u) + 544u;
 }
-static_assert(ac_smem_bytes(256, kAtTree) <= 227 * 1024 && ac_smem_bytes(256, kAtWindow) <= 227 * 1024, "shared memory");
-static_assert(ac_smem_bytes(128, kAtTree) <= 113 * 1024 && ac_smem_bytes(64, kAtTree) <= 113 * 1024, "shared memory");
+static_assert(ac_smem_bytes(256, kAtTree) <= 227 * 1024 && ac_smem_bytes(256, kAtWindow) <= 227 * 1024 &&
+              ac_smem_bytes(128, kAtTree) <= 227 * 1024 && ac_smem_bytes(64, kAtTree) <= 227 * 1024, "shared memory");
+static_assert(ac_smem_bytes(128, kAtWindow) <= 113 * 1024 && ac_smem_bytes(64, kAtWindow) <= 113 * 1024, "shared memory");
 
 struct AttendTcMaps {
     CUtensorMap dk, dv;  // dense keys: (D, kv_heads, tokens, sequences), boxes (64, 1, 128 | V unit keys, 1)
@@ -119,26 +125,29 @@ __device__ __forceinline__ uint32_t ac_zero_times(uint32_t x, uint32_t acc) {
 }
 
 template <int D, bool BF16, int MODE>
-__global__ void __launch_bounds__(ac_threads(D), ac_ctas(D))
+__global__ void __launch_bounds__(ac_threads(D, MODE), ac_wide(D, MODE) ? 1 : 2)
     attend_tc_kernel(const __grid_constant__ AttendTcMaps maps, const __grid_constant__ AttendParams P,
                      const uint32_t box) {
-    constexpr int HS = ac_halves(D);
-    constexpr uint32_t SB = D == 256 ? 2 : 1;    // S accumulators
+    constexpr bool kWide = ac_wide(D, MODE);
+    constexpr int HS = kWide ? 2 : 1;            // softmax warps per 32 rows
+    constexpr uint32_t SB = kWide ? 2 : 1;       // S accumulators
+    constexpr uint32_t kScanWarps = kWide ? 1 : 2;
+    constexpr int kThreads = ac_threads(D, MODE);
     constexpr uint32_t U = D / 64;               // units of a K tile, and of a V tile
     constexpr uint32_t VK = kAcUnit / (D * 2);   // keys of a V unit
     constexpr uint32_t NU = ac_units(D, MODE);
     constexpr uint32_t NB = ac_tiles(D, MODE);
     static_assert(NB <= kAcMaxTiles && NU >= 2 * U, "ring");
     constexpr uint32_t kQTile = 128 * D * 2;
-    constexpr uint32_t kColO = SB * 128, kCols = D == 256 ? 512 : 256;  // S / P, then O
+    constexpr uint32_t kColO = SB * 128, kCols = kWide ? 512 : 256;  // S / P, then O
     extern __shared__ __align__(1024) uint8_t ac_smem[];  // the 128-byte swizzle counts from 1,024-byte boundaries
     uint8_t* qsm = ac_smem;
     uint8_t* ring = qsm + kQTile;
     float* pair_max = reinterpret_cast<float*>(ring + NU * kAcUnit);  // HS = 2: [2 (tile parity)][2 (half)][128]
     int2* table = reinterpret_cast<int2*>(pair_max + (HS == 2 ? 512 : 0));
     uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(table) + (MODE == kAtTree ? kAcTable * 8 : 0));
-    uint64_t* full = bars;                 // [NB] tile loaded
-    uint64_t* done = full + kAcMaxTiles;   // [NB] its product is done: S is there (K), O is and P is free (V)
+    uint64_t* full = bars;                    // [NB][2] half of the tile's units loaded (its one unit: [0])
+    uint64_t* done = full + 2 * kAcMaxTiles;  // [NB] its product is done: S is there (K), O is and P is free (V)
     uint64_t* p_full = done + kAcMaxTiles;  // [2] keys 0 .. 63 of P
     uint64_t* p_half = p_full + 2;          // [2] keys 64 .. 127 of P
     uint64_t* fin = p_full + 4;
@@ -146,8 +155,8 @@ __global__ void __launch_bounds__(ac_threads(D), ac_ctas(D))
     uint64_t* scanned = p_full + 6;         // [kAcScans] V tile looked through
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scanned + kAcScans);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    volatile uint32_t* bad_flag = tmem_slot + 2;  // [kAcScans][2] by the two scanning warps
-    static_assert((2 * kAcMaxTiles + 6 + kAcScans) * 8 + 8 + kAcScans * 8 <= 512, "barriers");
+    volatile uint32_t* bad_flag = tmem_slot + 2;  // [kAcScans][2] what the scanning warps found
+    static_assert((3 * kAcMaxTiles + 6 + kAcScans) * 8 + 8 + kAcScans * 8 <= 544, "barriers");
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (smem_u32(ac_smem) & 1023u) {
@@ -171,7 +180,8 @@ __global__ void __launch_bounds__(ac_threads(D), ac_ctas(D))
     uint32_t nt, n_first;
     uint32_t p0 = 0, p1 = 0, lo = 0, hi = 0, few = 0;
     uint32_t n_keys = 0, recent = 0, prow = 0;
-    uint32_t e0 = 0;
+    const uint32_t bsh = MODE == kAtTree ? 31u - uint32_t(__clz(int(box))) : 0u;  // box = 1 << bsh
+    const uint32_t nb = MODE == kAtTree ? uint32_t(kAcKeys) >> bsh : 1;           // boxes of a page tile
     if constexpr (MODE == kAtWindow) {
         const uint64_t base = P.seq_base ? __ldg(reinterpret_cast<const unsigned long long*>(P.seq_base + b)) : P.base;
         if (base > P.capacity || rows > P.capacity - base) {
@@ -206,45 +216,50 @@ __global__ void __launch_bounds__(ac_threads(D), ac_ctas(D))
     }
     const uint32_t tb = uint32_t(uint64_t(nt) * split / P.splits), te = uint32_t(uint64_t(nt) * (split + 1) / P.splits);
     const uint32_t n = te - tb;  // tiles of this CTA
-    auto page_div = [&](uint32_t x) { return uint32_t((uint64_t(x) * P.pt_magic) >> P.pt_shift); };
     if constexpr (MODE == kAtTree) {
-        // {slot, tokens held} of the chunk's pages; the host's chunks touch at most kAcTable of them.
-        e0 = page_div(tb * kAcKeys);
-        const uint32_t last = min(te, n_first) * kAcKeys;
-        const uint32_t n_ent = tb < min(te, n_first) ? min(page_div(min(last, n_keys) - 1) + 1 - e0, kAcTable) : 0;
+        // The boxes of the chunk's page tiles, so that nobody divides by the page size or looks up a slot later:
+        // x = slot, y = first token in the page | (some box of the tile is not full) << 23 | tokens held << 24.
+        // The host's chunks have at most kAcTable of them.
         const uint64_t tokens = P.seq_tokens ? __ldg(reinterpret_cast<const unsigned long long*>(P.seq_tokens + b)) : P.tokens;
-        for (uint32_t i = tid; i < n_ent; i += ac_threads(D)) {
-            const uint32_t e = e0 + i;
-            int page, slot;
-            if (P.sel_ids) {
-                const uint32_t id = __ldg(P.sel_ids + uint64_t(b) * P.sel_stride + e);
-                page = id < P.pool_pages ? int(id) : -1;
-                slot = page >= 0 ? P.slot_of[uint64_t(prow) * P.pool_pages + page] : -1;
-                if (page < 0) record_error(P.status, KVM_ERR_INVALID_ARGUMENT, 123);
-                else if (slot < 0 || slot >= int(P.pool_slots)) {
-                    record_error(P.status, KVM_ERR_STALE, 124);
-                    page = -1;
+        const uint32_t page_tiles = tb < n_first ? min(te, n_first) - tb : 0;
+        for (uint32_t i = tid; i < min(page_tiles, kAcTable >> (7 - bsh)); i += kThreads) {
+            uint32_t least = box;
+            for (uint32_t k = 0; k < nb; ++k) {
+                const uint32_t x = (tb + i) * kAcKeys + k * box;
+                int2 ent = make_int2(0, 0);
+                if (x < n_keys) {
+                    const uint32_t e = uint32_t((uint64_t(x) * P.pt_magic) >> P.pt_shift), o = x - e * P.page_tokens;
+                    int page, slot;
+                    if (P.sel_ids) {
+                        const uint32_t id = __ldg(P.sel_ids + uint64_t(b) * P.sel_stride + e);
+                        page = id < P.pool_pages ? int(id) : -1;
+                        slot = page >= 0 ? P.slot_of[uint64_t(prow) * P.pool_pages + page] : -1;
+                        if (page < 0) record_error(P.status, KVM_ERR_INVALID_ARGUMENT, 123);
+                        else if (slot < 0 || slot >= int(P.pool_slots)) {
+                            record_error(P.status, KVM_ERR_STALE, 124);
+                            page = -1;
+                        }
+                    } else {
+                        slot = int(e);
+                        page = P.page_of[uint64_t(prow) * P.pool_slots + e];
+                    }
+                    const uint64_t start = uint64_t(max(page, 0)) * P.page_tokens + o;
+                    if (page >= 0 && tokens > start) ent = make_int2(slot, int(o | uint32_t(min(tokens - start, uint64_t(box))) << 24));
                 }
-            } else {
-                slot = int(e);
-                page = P.page_of[uint64_t(prow) * P.pool_slots + e];
+                least = min(least, uint32_t(ent.y) >> 24);
+                table[i * nb + k] = ent;
             }
-            int2 ent = make_int2(0, 0);
-            if (page >= 0) {
-                const uint64_t start = uint64_t(page) * P.page_tokens;
-                const uint64_t held = tokens > start ? tokens - start : 0;
-                ent = make_int2(slot, int(min(held, uint64_t(P.page_tokens))));
-            }
-            table[i] = ent;
+            if (least < box) table[i * nb].y |= 1 << 23;
         }
     }
 
     if (tid == 0) {
         for (uint32_t i = 0; i < NB; ++i) {
-            mbar_init(&full[i], 1);
+            mbar_init(&full[2 * i], 1);
+            mbar_init(&full[2 * i + 1], 1);
             mbar_init(&done[i], 1);
         }
-        for (uint32_t i = 0; i < kAcScans; ++i) mbar_init(&scanned[i], 2);
+        for (uint32_t i = 0; i < kAcScans; ++i) mbar_init(&scanned[i], kScanWarps);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&p_full[i], 128);
             mbar_init(&p_half[i], 128);
@@ -284,13 +299,13 @@ __global__ void __launch_bounds__(ac_threads(D), ac_ctas(D))
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     tc_fence_before();
-    // The loads need the barriers alone, which their own thread has set up (and the page
+    // The K loads need the barriers alone, which their own thread has set up (and the page
     // table): over a dense cache they start at once.
     if (MODE == kAtWindow && warp == 0) {
         __threadfence_block();
-        asm volatile("bar.arrive 1, %0;" ::"n"(ac_threads(D)) : "memory");
+        asm volatile("bar.arrive 1, %0;" ::"n"(kThreads) : "memory");
     } else {
-        named_sync(1, ac_threads(D));
+        named_sync(1, kThreads);
     }
     tc_fence_after();
     const uint32_t tmem = warp ? *tmem_slot : 0;
@@ -307,84 +322,97 @@ __global__ void __launch_bounds__(ac_threads(D), ac_ctas(D))
                      (a + kAcKeys <= P.sinks || p1 - a < P.window));
         } else {
             if (t >= n_first) return (t - n_first + 1) * kAcKeys > recent;
-            bool part = t * kAcKeys + kAcKeys > n_keys;
-            const uint32_t first = page_div(t * kAcKeys), last = page_div(min(t * kAcKeys + kAcKeys, n_keys) - 1);
-            for (uint32_t e = first; e <= last; ++e) part = part || table[e - e0].y != int(P.page_tokens);
-            return part;
+            return (table[(t - tb) * nb].y >> 23) & 1;
         }
     };
 
-    // Two CTAs per SM: registers go to the softmax warps, 4 x 32 x 56 + 4 x 32 x 200 = 256 x 128.
+    // Two CTAs per SM: registers go to the softmax warps, 4 x 32 x 72 + 4 x 32 x 184 = 256 x 128.
     if (warp < 4) {
-        if constexpr (HS == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 0) {
-            // ---- TMA producer ----
+        if constexpr (HS == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 0 || (kScanWarps == 1 && warp == 2)) {
+            // ---- TMA producer; in the wide shape two, warp 0 for K and warp 2 for V (one thread's 20 copies
+            // per tile of head_dim 256 took 2,600 cycles to issue, more than the tile's products) ----
             if (lane == 0) {
-                uint32_t tiles_issued = 0, freed = 0;  // tiles issued; tiles known to be used up
+                uint32_t freed = 0;  // tiles known to be used up
                 // K (or V) tile j of this CTA, the q-th of the ring.
-                auto load = [&](uint32_t j, bool is_v) -> bool {
-                    const uint32_t q = is_v ? v_seq(j) : k_seq(j), t = tb + j;
-                    const uint32_t keys = is_v ? VK : uint32_t(kAcKeys), bh = min(box, keys);
-                    uint64_t* bar = &full[q % NB];
+                auto load = [&](uint32_t j, auto v) -> bool {
+                    constexpr bool kV = decltype(v)::value;
+                    constexpr uint32_t kKeys = kV ? VK : uint32_t(kAcKeys), kBlocks = kV ? U : 1;  // keys, 64-dim blocks of a unit
+                    constexpr uint32_t kPer = U > 1 ? U / 2 : 1;                                   // units per barrier
+                    const CUtensorMap* dmap = kV ? &maps.dv : &maps.dk;
+                    const CUtensorMap* pmap = kV ? &maps.pv : &maps.pk;
+                    const uint32_t q = kV ? v_seq(j) : k_seq(j), t = tb + j, bh = min(box, kKeys);
                     const bool dense = MODE == kAtWindow || t >= n_first;
                     const uint32_t tok = MODE == kAtWindow ? (t < n_first ? t * kAcKeys : lo + (t - n_first) * kAcKeys)
                                                            : (t - n_first) * kAcKeys;
-                    auto held = [&](uint32_t x) { return x < n_keys && int(x - page_div(x) * P.page_tokens) < table[page_div(x) - e0].y; };
-                    uint32_t bytes = U * kAcUnit, sent = 0;
-                    if (!dense) {
-                        bytes = 0;
-                        for (uint32_t x = 0; x < uint32_t(kAcKeys); x += bh)
-                            if (held(t * kAcKeys + x)) bytes += bh * D * 2;
-                    }
+                    const int2* ents = table + j * nb;  // (page tiles come first: tile j of this CTA is tile tb + j)
+                    uint64_t* bar = nullptr;
+                    uint32_t left = 0;  // bytes of the barrier's copies that are not started
+#pragma unroll
                     for (uint32_t sub = 0; sub < U; ++sub) {
                         const uint32_t idx = q * U + sub, s = idx % NU;
                         while (idx >= NU && freed <= (idx - NU) / U) {  // the tile whose unit this one replaces
                             if (!mbar_wait(&done[freed % NB], (freed / NB) & 1)) {
                                 record_error(P.status, KVM_ERR_TIMEOUT, 125);
-                                if (sub) ac_complete_tx(bar, bytes - sent);  // copies of this tile that are not started
+                                if (left) ac_complete_tx(bar, left);
                                 return false;
                             }
                             ++freed;
                         }
-                        if (sub == 0) {
-                            if (bytes) mbar_arrive_expect_tx(bar, bytes);
-                            else mbar_arrive(bar);
-                            tiles_issued = q + 1;
+                        if (sub % kPer == 0) {
+                            bar = &full[(q % NB) * 2 + sub / kPer];
+                            left = kPer * kAcUnit;
+                            mbar_arrive_expect_tx(bar, left);
                         }
-                        const uint32_t dst = smem_u32(ring + s * kAcUnit), key0 = is_v ? sub * VK : 0;
-                        const uint32_t d0 = is_v ? 0 : sub, d1 = is_v ? U : sub + 1;  // 64-dim blocks
+                        left -= kAcUnit;
+                        const uint32_t dst = smem_u32(ring + s * kAcUnit), key0 = kV ? sub * VK : 0;
                         if (dense) {
-                            sent += kAcUnit;
-                            for (uint32_t a = d0; a < d1; ++a)
-                                ac_load_4d(dst + (a - d0) * keys * 128, is_v ? &maps.dv : &maps.dk, int(a * 64), int(h),
-                                           int(tok + key0), int(b), bar);
+#pragma unroll
+                            for (uint32_t a = 0; a < kBlocks; ++a)
+                                ac_load_4d(dst + a * kKeys * 128, dmap, int((kV ? a : sub) * 64), int(h), int(tok + key0), int(b), bar);
                         } else {
-                            for (uint32_t i = 0; i < keys; i += bh) {
-                                const uint32_t x = t * kAcKeys + key0 + i;
-                                if (!held(x)) continue;
-                                const uint32_t en = page_div(x);
-                                sent += bh * 128 * (d1 - d0);
-                                for (uint32_t a = d0; a < d1; ++a)
-                                    ac_load_5d(dst + (a - d0) * keys * 128 + i * 128, is_v ? &maps.pv : &maps.pk, int(a * 64),
-                                               int(h), int(x - en * P.page_tokens), table[en - e0].x, int(prow), bar);
+                            for (uint32_t i = 0; i < kKeys; i += bh) {
+                                const int2 ent = ents[(key0 + i) >> bsh];
+                                const uint32_t in = (key0 + i) & (box - 1);
+                                // A box without a token is read past the last slot: zeros.
+                                const int slot = in < uint32_t(ent.y) >> 24 ? ent.x : int(P.pool_slots);
+#pragma unroll
+                                for (uint32_t a = 0; a < kBlocks; ++a)
+                                    ac_load_5d(dst + a * kKeys * 128 + i * 128, pmap, int((kV ? a : sub) * 64), int(h),
+                                               int((uint32_t(ent.y) & 0x7FFFFFu) + in), slot, int(prow), bar);
                             }
                         }
                     }
                     return true;
                 };
-                bool ok = true;
-                if (n) {
-                    ok = load(0, false);
-                    if (SB == 2 && n > 1) ok = ok && load(1, false);
-                    for (uint32_t j = 0; j < n && ok && !*abort_flag; ++j) {
-                        ok = load(j, true);
-                        if (ok && j + SB < n) ok = load(j + SB, false);
+                // V(j) stays at most two tiles ahead of the scan (below).
+                auto load_v = [&](uint32_t j) -> bool {
+                    if (j >= 2 && !mbar_wait(&scanned[(j - 2) % kAcScans], ((j - 2) / kAcScans) & 1)) {
+                        record_error(P.status, KVM_ERR_TIMEOUT, 127);
+                        return false;
                     }
+                    return load(j, std::true_type{});
+                };
+                bool ok = true;
+                uint32_t j = 0;
+                if (kScanWarps == 2) {
+                    if (n) ok = load(0, std::false_type{});
+                    for (; j < n && ok && !*abort_flag; ++j) ok = load_v(j) && (j + 1 >= n || load(j + 1, std::false_type{}));
+                } else if (warp == 0) {
+                    for (; j < n && ok && !*abort_flag; ++j) ok = load(j, std::false_type{});
+                } else {
+                    for (; j < n && ok && !*abort_flag; ++j) ok = load_v(j);
                 }
                 if (!ok) *abort_flag = 1;
-                // Every issued copy lands before the CTA frees its shared memory.
-                for (uint32_t q = tiles_issued > NB ? tiles_issued - NB : 0; q < tiles_issued; ++q)
-                    if (!mbar_wait(&full[q % NB], (q / NB) & 1)) record_error(P.status, KVM_ERR_TIMEOUT, 126);
+                // Every issued copy lands before the CTA frees its shared memory: the tiles whose barrier has
+                // not been taken over by a later one (which its release came before).
+                for (uint32_t i = j > NB ? j - NB : 0; i < j; ++i)
+                    for (uint32_t v = kScanWarps == 2 ? 0 : warp / 2; v <= (kScanWarps == 2 ? 1u : uint32_t(warp) / 2); ++v) {
+                        const uint32_t q = v ? v_seq(i) : k_seq(i);
+                        if (ok ? q + NB < 2 * n : q < freed) continue;
+                        for (uint32_t x = 0; x < (U > 1 ? 2u : 1u); ++x)
+                            if (!mbar_wait(&full[(q % NB) * 2 + x], (q / NB) & 1)) record_error(P.status, KVM_ERR_TIMEOUT, 126);
+                    }
             }
         } else if (warp == 1) {
             // ---- MMA issue: tile j, S accumulator j % SB ----
@@ -412,10 +440,12 @@ __global__ void __launch_bounds__(ac_threads(D), ac_ctas(D))
             int err = 0;
             // S from the K tile at kp, which moves on (over the V tile in between, but for K1 of two).
             auto issue_s = [&](uint32_t slot, bool over) -> bool {
-                if (!pf_warp_wait(&full[kp.b], kp.ph)) return false;
-                tc_fence_after();
 #pragma unroll
                 for (uint32_t a = 0; a < U; ++a) {
+                    if (a == 0 || a == U / 2) {
+                        if (!pf_warp_wait(&full[kp.b * 2 + (a ? 1 : 0)], kp.ph)) return false;
+                        tc_fence_after();
+                    }
                     const uint64_t kd = kdesc + kp.s * (kAcUnit >> 4);
 #pragma unroll
                     for (uint32_t kk = 0; kk < 4; ++kk)
@@ -431,7 +461,7 @@ __global__ void __launch_bounds__(ac_threads(D), ac_ctas(D))
                 if (!issue_s(j, SB == 1 || j > 0)) err = 131;
             for (uint32_t j = 0; j < steps && !err; ++j) {
                 const uint32_t slot = j % SB, ph = (j / SB) & 1;
-                if (!pf_warp_wait(&full[vp.b], vp.ph)) err = 133;
+                if (!pf_warp_wait(&full[vp.b * 2], vp.ph)) err = 133;
                 if (!err && !pf_warp_wait(&p_full[slot], ph)) err = 132;
                 if (err || __shfl_sync(0xffffffffu, *abort_flag, 0)) {
                     if (!err) err = -1;
@@ -440,6 +470,7 @@ __global__ void __launch_bounds__(ac_threads(D), ac_ctas(D))
                 tc_fence_after();
 #pragma unroll
                 for (uint32_t a = 0; a < U; ++a) {
+                    if (U > 1 && a == U / 2 && !pf_warp_wait(&full[vp.b * 2 + 1], vp.ph)) err = 133;
                     const uint64_t vd = vdesc + vp.s * (kAcUnit >> 4);
 #pragma unroll
                     for (uint32_t kk = 0; kk < VK / 16; ++kk) {  // P: 16 keys = 8 tensor-memory columns
@@ -466,21 +497,38 @@ __global__ void __launch_bounds__(ac_threads(D), ac_ctas(D))
             ac_commit(fin);
             if (!pf_warp_wait(fin, 0) && lane == 0) record_error(P.status, KVM_ERR_TIMEOUT, 134);
         } else {
-            // ---- warps 2 and 3: V tiles that some row does not see in full are looked through ----
+            // ---- V tiles that some row does not see in full are looked through ----
+            // (It waits for every V tile, and the V loads stay at most two tiles ahead of it: were it to
+            // look at a barrier of another pass, that pass's parity could be taken for its tile's.)
             for (uint32_t j = 0; j < n; ++j) {
                 const uint32_t q = v_seq(j);
-                const bool ok = pf_warp_wait(&full[q % NB], (q / NB) & 1);
+                bool ok = pf_warp_wait(&full[(q % NB) * 2], (q / NB) & 1);
+                if (U > 1) ok = pf_warp_wait(&full[(q % NB) * 2 + 1], (q / NB) & 1) && ok;
                 uint32_t acc = 0;
-                if (in_part(tb + j)) {
-#pragma unroll
+                const uint32_t t = tb + j;
+                if (in_part(t)) {
+                    // V rows of keys that no row sees become zeros; the others are looked through.
+                    const bool paged = MODE == kAtTree && t < n_first;
+                    const uint32_t live = MODE == kAtWindow ? (t < n_first ? few - t * kAcKeys : hi - lo - (t - n_first) * kAcKeys)
+                                                            : recent + rows - (t - n_first) * kAcKeys;
+                    constexpr uint32_t kStep = 32 * kScanWarps;
+                    const uint32_t first = uint32_t(tid - (128 - 32 * int(kScanWarps)));
                     for (uint32_t a = 0; a < U; ++a) {
-                        const uint4* v4 = reinterpret_cast<const uint4*>(ring + ((q * U + a) % NU) * kAcUnit);
-#pragma unroll 8
-                        for (uint32_t e = uint32_t(tid - 64); e < kAcUnit / 16; e += 64) {
-                            const uint4 y = v4[e];
-                            acc = ac_zero_times<BF16>(y.x, ac_zero_times<BF16>(y.y, ac_zero_times<BF16>(y.z, ac_zero_times<BF16>(y.w, acc))));
+                        uint4* v4 = reinterpret_cast<uint4*>(ring + ((q * U + a) % NU) * kAcUnit);
+                        for (uint32_t e0 = 0; e0 < kAcUnit / 16; e0 += 8 * kStep) {
+                            uint4 y[8];
+#pragma unroll
+                            for (uint32_t i = 0; i < 8; ++i) y[i] = v4[e0 + i * kStep + first];
+#pragma unroll
+                            for (uint32_t i = 0; i < 8; ++i) {
+                                const uint32_t key = a * VK + ((e0 + i * kStep + first) / 8) % VK;
+                                const bool dead = paged ? (key & (box - 1)) >= uint32_t(table[j * nb + (key >> bsh)].y) >> 24 : key >= live;
+                                if (dead) v4[e0 + i * kStep + first] = make_uint4(0, 0, 0, 0);
+                                else acc = ac_zero_times<BF16>(y[i].x, ac_zero_times<BF16>(y[i].y, ac_zero_times<BF16>(y[i].z, ac_zero_times<BF16>(y[i].w, acc))));
+                            }
                         }
                     }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
                 const bool bad = __any_sync(0xffffffffu, at_nonfinite<BF16>(acc));
                 if (lane == 0) {
@@ -491,7 +539,7 @@ __global__ void __launch_bounds__(ac_threads(D), ac_ctas(D))
             }
         }
     } else {
-        if constexpr (HS == 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        if constexpr (HS == 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
         // ---- softmax: thread = packed row (tensor-memory lane), NK of the tile's keys ----
         // With two warps per 32 rows these exchange their maxes through shared memory, behind a
         // barrier of their own. A warp that gives up raises the abort flag and then arrives there,
@@ -554,11 +602,10 @@ __global__ void __launch_bounds__(ac_threads(D), ac_ctas(D))
                         see[q] = bits | below(rec, q4);
                     }
                 } else {
-                    const uint32_t first = page_div(t * kAcKeys), last = page_div(min(t * kAcKeys + kAcKeys, n_keys) - 1);
 #pragma unroll
                     for (int q = 0; q < NW; ++q) see[q] = 0;
-                    for (uint32_t e = first; e <= last; ++e) {
-                        const int at = int(e * P.page_tokens) - int(t * kAcKeys), end = at + table[e - e0].y;
+                    for (uint32_t k = 0; k < nb; ++k) {
+                        const int at = int(k * box), end = at + int(uint32_t(table[j * nb + k].y) >> 24);
 #pragma unroll
                         for (int q = 0; q < NW; ++q) see[q] |= below(end, int(half) * NW + q) & ~below(at, int(half) * NW + q);
                     }
@@ -643,9 +690,12 @@ __global__ void __launch_bounds__(ac_threads(D), ac_ctas(D))
                 mbar_arrive(bar);
             };
             exps(0, 64);
-            ok = pf_warp_wait(&scanned[j % kAcScans], (j / kAcScans) & 1);
-            if (!ok) break;
-            const bool bad = bad_flag[(j % kAcScans) * 2] | bad_flag[(j % kAcScans) * 2 + 1];
+            bool bad = false;
+            if (part) {
+                ok = pf_warp_wait(&scanned[j % kAcScans], (j / kAcScans) & 1);
+                if (!ok) break;
+                bad = (bad_flag[(j % kAcScans) * 2 + 1] | (kScanWarps == 2 ? bad_flag[(j % kAcScans) * 2] : 0u)) != 0;
+            }
             store(0, half);
             if constexpr (HS == 1) {
                 exps(64, 96);
@@ -727,61 +777,66 @@ __global__ void __launch_bounds__(ac_threads(D), ac_ctas(D))
             const uint64_t row_id = (uint64_t(b) * P.width + ri) * P.q_heads + qh;
             const uint64_t id = uint64_t(split) * P.seqs * P.width * P.q_heads + row_id;
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            constexpr uint32_t kCol = D / HS, kRowBytes = 2 * kCol;  // columns of this thread; bytes of a staged row
-            uint8_t* orow = P.out + uint64_t(b) * P.o_seq + uint64_t(ri) * P.o_row + uint64_t(qh) * P.o_head + half * kRowBytes;
-            // Rows go through shared memory (the warp's share of the query tile, which every S has left) so
-            // that a warp writes whole lines: 32 lanes with a row each would write 32 lines at a time.
-            uint8_t* stage = qsm + uint32_t(warp - 4) * (32 * kRowBytes);
-            uint8_t* srow = stage + lane * kRowBytes;
+            constexpr uint32_t kCol = D / HS;  // columns of this thread
+            uint8_t* orow = P.out + uint64_t(b) * P.o_seq + uint64_t(ri) * P.o_row + uint64_t(qh) * P.o_head + half * kCol * 2;
             const bool parts = P.splits > 1;
             uint64_t dst0 = parts ? reinterpret_cast<uint64_t>(P.part_o + id * D + half * kCol) : reinterpret_cast<uint64_t>(orow);
             if (!valid) dst0 = 0;
-            constexpr uint32_t kChunks = kRowBytes / 16;  // 8, 16 or 32
-            for (uint32_t pass = 0; n && pass < (parts ? 2u : 1u); ++pass) {  // 32-bit rows in two parts
-                const uint32_t c0 = parts ? pass * (kCol / 2) : 0, c1 = parts ? c0 + kCol / 2 : kCol;
+            // Rows go through shared memory (the ring, which every product has left) so that a warp
+            // writes whole lines: 32 lanes with a row each would write 32 lines at a time.
+            static_assert(NU * kAcUnit >= 128 * D * 4, "row staging");
+            uint8_t* stage = ring + uint32_t(warp - 4) * (32 * kCol * 4);
+            auto emit = [&](auto as_parts) {
+                constexpr bool kParts = decltype(as_parts)::value;
+                constexpr uint32_t kChunks = kCol * (kParts ? 4 : 2) / 16, kSwz = kChunks < 8 ? kChunks - 1 : 7;  // 16-byte chunks
+                uint8_t* srow = stage + lane * (kChunks * 16);
 #pragma unroll 1
-                for (uint32_t cc = c0; cc < c1; cc += 32) {
+                for (uint32_t cc = 0; cc < kCol; cc += 32) {
                     uint32_t o[32];
                     tc_ld32(col_o + cc, o);
                     tc_wait_ld(o);
-                    if (parts) {
 #pragma unroll
-                        for (uint32_t i = 0; i < 8; ++i)
-                            *reinterpret_cast<uint4*>(srow + ((((cc - c0) / 4 + i) ^ (lane & 7)) << 4)) =
-                                make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-                    } else {
+                    for (uint32_t i = 0; i < (kParts ? 8 : 4); ++i) {
+                        uint4 y;
+                        if constexpr (kParts) {
+                            y = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                        } else {  // (a row that sees no key has a zero sum; its product is 0)
+                            uint32_t z[4];
 #pragma unroll
-                        for (uint32_t i = 0; i < 4; ++i) {
-                            uint32_t y[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)  // (a row that sees no key has a zero sum; its product is 0)
-                                y[e] = pf_pack2<BF16>(__uint_as_float(o[8 * i + 2 * e]) * inv,
-                                                      __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
-                            *reinterpret_cast<uint4*>(srow + (((cc / 8 + i) ^ (lane & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+                            for (int e = 0; e < 4; ++e)
+                                z[e] = pf_pack2<BF16>(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
+                            y = make_uint4(z[0], z[1], z[2], z[3]);
                         }
+                        *reinterpret_cast<uint4*>(srow + (((cc / (kParts ? 4 : 8) + i) ^ (lane & kSwz)) << 4)) = y;
                     }
                 }
                 __syncwarp();
-                constexpr uint32_t kStep = 32 / kChunks;  // rows at a time, eight rounds in flight
-                const uint32_t c = uint32_t(lane) % kChunks;
+                constexpr uint32_t kPer = kChunks < 32 ? 32 / kChunks : 1, kWide32 = kChunks < 32 ? 1 : kChunks / 32;  // rows at a time; rounds per row
+                constexpr uint32_t kBatch = 32 / kPer < 8 ? 32 / kPer : 8;                                             // rounds in flight
+                const uint32_t c0 = uint32_t(lane) % kChunks;
 #pragma unroll 1
-                for (uint32_t r0 = uint32_t(lane) / kChunks; r0 < 32; r0 += 8 * kStep) {
-                    uint4 y[8];
-                    uint64_t to[8];
+                for (uint32_t r0 = uint32_t(lane) / kChunks; r0 < 32; r0 += kBatch * kPer) {
 #pragma unroll
-                    for (uint32_t k = 0; k < 8; ++k) {
-                        const uint32_t rr = r0 + k * kStep;
-                        to[k] = __shfl_sync(0xffffffffu, dst0, rr);
-                        y[k] = *reinterpret_cast<const uint4*>(stage + rr * kRowBytes + ((c ^ (rr & 7)) << 4));
+                    for (uint32_t part = 0; part < kWide32; ++part) {
+                        uint4 y[kBatch];
+                        uint64_t to[kBatch];
+                        const uint32_t c = c0 + part * 32;
+#pragma unroll
+                        for (uint32_t k = 0; k < kBatch; ++k) {
+                            const uint32_t rr = r0 + k * kPer;
+                            to[k] = __shfl_sync(0xffffffffu, dst0, rr);
+                            y[k] = *reinterpret_cast<const uint4*>(stage + rr * (kChunks * 16) + ((c ^ (rr & kSwz)) << 4));
+                        }
+#pragma unroll
+                        for (uint32_t k = 0; k < kBatch; ++k)
+                            if (to[k]) reinterpret_cast<uint4*>(to[k])[c] = y[k];
                     }
-#pragma unroll
-                    for (uint32_t k = 0; k < 8; ++k)
-                        if (to[k]) reinterpret_cast<uint4*>(to[k])[pass * kChunks + c] = y[k];
                 }
-                __syncwarp();
-            }
-            if (n == 0 && valid && P.splits == 1)  // nothing to see
-                for (uint32_t c = 0; c < kChunks; ++c) reinterpret_cast<uint4*>(orow)[c] = make_uint4(0, 0, 0, 0);
+            };
+            if (n && parts) emit(std::true_type{});
+            else if (n) emit(std::false_type{});
+            else if (valid && !parts)  // nothing to see
+                for (uint32_t c = 0; c < kCol / 8; ++c) reinterpret_cast<uint4*>(orow)[c] = make_uint4(0, 0, 0, 0);
             if (valid && half == 0) {
                 if (parts) P.part_ml[id] = make_float2(l == 0.f ? -INFINITY : m_used, l);
                 else if (P.lse) P.lse[row_id] = l == 0.f ? -INFINITY : (m_used + log2f(l)) * kAtLn2;

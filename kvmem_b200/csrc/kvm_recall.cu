@@ -2340,7 +2340,7 @@ bool attend_tc_maps(const AttendParams& p, uint32_t head_dim, bool bf16, int mod
     if (mode == kAtWindow) return true;
     uint32_t b = 128;
     while (p.page_tokens % b) b >>= 1;
-    if (b < 16) return false;
+    if (b < 16 || p.page_tokens >= (1u << 23)) return false;
     *box = b;
     for (int v = 0; v < 2; ++v) {
         const cuuint64_t dims[5] = {head_dim, p.kv_heads, p.page_tokens, p.pool_slots, pool_rows};
@@ -2404,19 +2404,20 @@ int attend_launch(kvm_ctx* c, AttendParams& p, uint32_t head_dim, bool bf16, int
         uint32_t box = 0;
         if (attend_tc_maps(p, head_dim, bf16, mode, pool_rows, &maps, &box)) {
             p.m_tiles = (packed + 127) / 128;
-            // One CTA's chunk touches at most kAcTable pages
+            // One CTA's chunk has at most kAcTable page boxes
             uint32_t least = 1;
             bool too_many = false;
             if (mode == kAtTree) {
                 // (chunks are even shares of all tiles, the longest tail's among them).
-                const uint64_t most = uint64_t(kAcTable - 2) * p.page_tokens / kAcKeys;
+                const uint64_t most = uint64_t(kAcTable) * box / kAcKeys;
                 const uint64_t all = (list_keys + kAcKeys - 1) / kAcKeys + (tail_most + kAcKeys - 1) / kAcKeys;
                 if (all / most >= 256) too_many = true;
                 least = uint32_t(all / most + 1);
             }
             if (!too_many) {
                 const uint64_t tiles = (keys + kAcKeys - 1) / kAcKeys + 1;
-                p.splits = attend_splits(c, uint64_t(p.seqs) * p.kv_heads * p.m_tiles, uint64_t(c->num_sms) * ac_ctas(int(head_dim)), tiles, 1.7, 6.0,
+                const bool wide = ac_wide(int(head_dim), mode);
+                p.splits = attend_splits(c, uint64_t(p.seqs) * p.kv_heads * p.m_tiles, uint64_t(c->num_sms) * (wide ? 1 : 2), tiles, wide ? 1.3 : 1.8, 7.0,
                                          rows, row_bytes, least);
                 KVM_TRY(attend_scratch(c, p, head_dim, s));
                 KVM_TRY(bf16 ? launch_attend_tc_t<true>(c, maps, p, head_dim, mode, box, s)

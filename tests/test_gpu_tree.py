@@ -289,6 +289,30 @@ def test_long_list_with_table_refills(ctx, monkeypatch):
     p.verify(out, lse, lists=p2)
 
 
+@pytest.mark.parametrize("dim,page,dtype", [(64, 16, torch.float16), (128, 64, torch.bfloat16), (256, 128, torch.float16)])
+@pytest.mark.parametrize("kernel", ["mma", "tc"])
+def test_many_tiles_in_one_chunk_with_holes(ctx, monkeypatch, dim, page, dtype, kernel):
+    """Twenty and more key tiles in one chunk, some of them partly filled or absent in the middle, garbage in all that
+    is not visible."""
+    monkeypatch.setenv("KVM_ATTEND", kernel)
+    monkeypatch.setenv("KVM_ATTEND_SPLITS", "1")
+    slots = 2816 // page
+    p = Problem(ctx, 25, 1, 5, 8, 2, dim, page, slots + 9, slots, [(slots + 8) * page + 3], [70], dtype, garbage=True)
+    # all resident pages in slot order (free slots are holes), then a list with pages past the history in the middle
+    out, lse = p.call(lists=None)
+    ctx.check_status()
+    p.verify(out, lse, lists=None)
+    half = (slots // 2) * page + 5
+    p.tokens = [half]
+    for r, s in zip(*np.nonzero(p.page_of >= 0)):
+        held = max(0, min(page, half - int(p.page_of[r, s]) * page))
+        p.cache[0][r, s, held:], p.cache[1][r, s, held:] = NAN, float("inf")
+    pages = p.lists[0][np.argsort(p.lists[0] % 3, kind="stable")]
+    out, lse = p.call(lists=[pages])
+    ctx.check_status()
+    p.verify(out, lse, lists=[pages])
+
+
 def test_per_head_rows_equal_a_shared_selection(ctx):
     """Pool rows per KV head (kv_heads = 1, one sequence per head), with q, tail and out as strided views."""
     import kvmem_b200 as K

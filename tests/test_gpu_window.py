@@ -55,6 +55,9 @@ CASES = [
     (1, 5, 4, 2, 128, [3], 0, 0, torch.bfloat16),               # nothing visible
     (1, 200, 2, 1, 128, [0], 10 ** 9, 0, torch.float16),        # plain causal attention
     (1, 70, 5, 1, 64, [900], 1, 64, torch.bfloat16),            # itself and the sinks
+    (1, 33, 6, 1, 256, [2900], 2700, 130, torch.bfloat16),      # two dozen tiles
+    (1, 300, 4, 1, 128, [2500], 2400, 1, torch.float16),
+    (2, 129, 1, 1, 64, [3000, 1700], 2990, 0, torch.float16),
 ]
 
 
