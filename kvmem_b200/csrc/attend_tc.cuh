@@ -40,27 +40,27 @@ constexpr int kAcKeys = 128;             // keys per tile
 constexpr uint32_t kAcUnit = 16384;      // bytes per ring unit
 constexpr uint32_t kAcTable = 512;       // page boxes of one CTA's key chunk
 constexpr uint32_t kAcScans = 8;         // V tiles that the scan's barriers tell apart
-constexpr uint32_t kAcMaxTiles = 14;
+constexpr uint32_t kAcMaxTiles = 7;
 
-// Two shapes. Wide: one CTA per SM, two S accumulators, eight softmax warps, a deep ring.
-// Narrow (a dense cache up to head_dim 128, whose tiles many rows share in L2): two CTAs
-// per SM, each with one S accumulator and four softmax warps.
-__host__ __device__ constexpr bool ac_wide(int D, int mode) { return D == 256 || mode == kAtTree; }
-__host__ __device__ constexpr int ac_threads(int D, int mode) { return ac_wide(D, mode) ? 384 : 256; }
+// Two shapes. Wide (head_dim 256): one CTA per SM, two S accumulators, eight softmax
+// warps, a deep ring. Narrow (64, 128): two CTAs per SM, each with one S accumulator and
+// four softmax warps; the wide shape takes 1.4 times as long there (whole prompt of
+// 16,381 rows: 562 us against 397), most of it starts and ends of CTAs in turn.
+__host__ __device__ constexpr bool ac_wide(int D) { return D == 256; }
+__host__ __device__ constexpr int ac_threads(int D) { return ac_wide(D) ? 384 : 256; }
 __host__ __device__ constexpr uint32_t ac_units(int D, int mode) {
     // What is left of the SM's 227 KiB (or half of it) beside the query tile and the page table.
-    return !ac_wide(D, mode) ? (D == 128 ? 4u : 5u) : D == 256 ? (mode == kAtTree ? 9u : 10u) : D == 128 ? 11u : 12u;
+    return D == 256 ? (mode == kAtTree ? 9u : 10u) : D == 128 ? 4u : 5u;
 }
 // A K or V tile (D / 64 units) has one full barrier; that of tile q serves tile q +
 // ac_tiles again, whose first unit waits for a unit of a tile behind q.
 __host__ __device__ constexpr uint32_t ac_tiles(int D, int mode) { return ac_units(D, mode) / uint32_t(D / 64) + 2u; }
 __host__ __device__ constexpr uint32_t ac_smem_bytes(int D, int mode) {
-    return 128u * uint32_t(D) * 2u + ac_units(D, mode) * kAcUnit + (ac_wide(D, mode) ? 2048u : 0u) +
+    return 128u * uint32_t(D) * 2u + ac_units(D, mode) * kAcUnit + (ac_wide(D) ? 2048u : 0u) +
            (mode == kAtTree ? kAcTable * 8u : 0u) + 544u;
 }
-static_assert(ac_smem_bytes(256, kAtTree) <= 227 * 1024 && ac_smem_bytes(256, kAtWindow) <= 227 * 1024 &&
-              ac_smem_bytes(128, kAtTree) <= 227 * 1024 && ac_smem_bytes(64, kAtTree) <= 227 * 1024, "shared memory");
-static_assert(ac_smem_bytes(128, kAtWindow) <= 113 * 1024 && ac_smem_bytes(64, kAtWindow) <= 113 * 1024, "shared memory");
+static_assert(ac_smem_bytes(256, kAtTree) <= 227 * 1024 && ac_smem_bytes(256, kAtWindow) <= 227 * 1024, "shared memory");
+static_assert(ac_smem_bytes(128, kAtTree) <= 113 * 1024 && ac_smem_bytes(64, kAtTree) <= 113 * 1024, "shared memory");
 
 struct AttendTcMaps {
     CUtensorMap dk, dv;  // dense keys: (D, kv_heads, tokens, sequences), boxes (64, 1, 128 | V unit keys, 1)
@@ -125,14 +125,14 @@ __device__ __forceinline__ uint32_t ac_zero_times(uint32_t x, uint32_t acc) {
 }
 
 template <int D, bool BF16, int MODE>
-__global__ void __launch_bounds__(ac_threads(D, MODE), ac_wide(D, MODE) ? 1 : 2)
+__global__ void __launch_bounds__(ac_threads(D), ac_wide(D) ? 1 : 2)
     attend_tc_kernel(const __grid_constant__ AttendTcMaps maps, const __grid_constant__ AttendParams P,
                      const uint32_t box) {
-    constexpr bool kWide = ac_wide(D, MODE);
+    constexpr bool kWide = ac_wide(D);
     constexpr int HS = kWide ? 2 : 1;            // softmax warps per 32 rows
     constexpr uint32_t SB = kWide ? 2 : 1;       // S accumulators
     constexpr uint32_t kScanWarps = kWide ? 1 : 2;
-    constexpr int kThreads = ac_threads(D, MODE);
+    constexpr int kThreads = ac_threads(D);
     constexpr uint32_t U = D / 64;               // units of a K tile, and of a V tile
     constexpr uint32_t VK = kAcUnit / (D * 2);   // keys of a V unit
     constexpr uint32_t NU = ac_units(D, MODE);

@@ -9,7 +9,7 @@ namespace kvmb {
 template <int D, bool BF16, int MODE>
 int launch_attend_tc_k(kvm_ctx* c, const AttendTcMaps& maps, const AttendParams& p, uint32_t box, cudaStream_t s) {
     auto fn = attend_tc_kernel<D, BF16, MODE>;
-    if constexpr (!ac_wide(D, MODE)) {
+    if constexpr (!ac_wide(D)) {
         // The register split needs every register of 256 x 128: with fewer the warps would wait for more for ever.
         static const int regs = [&] {
             cudaFuncAttributes a{};
@@ -21,7 +21,7 @@ int launch_attend_tc_k(kvm_ctx* c, const AttendTcMaps& maps, const AttendParams&
     if (smem_attr(reinterpret_cast<const void*>(fn), int(smem)) != cudaSuccess) return KVM_ERR_CUDA;
     const uint64_t grid = uint64_t(p.seqs) * p.kv_heads * p.m_tiles * p.splits;
     if (grid > 0x7fffffffull) return KVM_ERR_LENGTH;
-    fn<<<uint32_t(grid), ac_threads(D, MODE), smem, s>>>(maps, p, box);
+    fn<<<uint32_t(grid), ac_threads(D), smem, s>>>(maps, p, box);
     ++c->launches;
     return cudaGetLastError() == cudaSuccess ? KVM_OK : KVM_ERR_CUDA;
 }

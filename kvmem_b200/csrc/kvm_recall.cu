@@ -2416,7 +2416,7 @@ int attend_launch(kvm_ctx* c, AttendParams& p, uint32_t head_dim, bool bf16, int
             }
             if (!too_many) {
                 const uint64_t tiles = (keys + kAcKeys - 1) / kAcKeys + 1;
-                const bool wide = ac_wide(int(head_dim), mode);
+                const bool wide = ac_wide(int(head_dim));
                 p.splits = attend_splits(c, uint64_t(p.seqs) * p.kv_heads * p.m_tiles, uint64_t(c->num_sms) * (wide ? 1 : 2), tiles, wide ? 1.3 : 1.8, 7.0,
                                          rows, row_bytes, least);
                 KVM_TRY(attend_scratch(c, p, head_dim, s));
