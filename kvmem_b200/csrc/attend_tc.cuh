@@ -26,6 +26,9 @@
 //    would spread to rows that do not see them. Keys that no row sees become zeros; the
 //    others are looked through, and where some rows see such a value it is taken out of
 //    the product and added by hand to those rows.
+// Quantised pages (q8_0 / q4_0): eight more warps read the blocks as stored, decode them to
+// fp16 and write them where the copies would have put them; queries and the tail become fp16
+// too (a bf16 query row after division by a power of two).
 // Every wait is bounded: on expiry the kernel records KVM_ERR_TIMEOUT, raises the
 // CTA's abort flag, lets copies and MMAs in flight finish and frees its TMEM.
 #pragma once
@@ -40,27 +43,30 @@ constexpr int kAcKeys = 128;             // keys per tile
 constexpr uint32_t kAcUnit = 16384;      // bytes per ring unit
 constexpr uint32_t kAcTable = 512;       // page boxes of one CTA's key chunk
 constexpr uint32_t kAcScans = 8;         // V tiles that the scan's barriers tell apart
-constexpr uint32_t kAcMaxTiles = 7;
+constexpr uint32_t kAcMaxTiles = 8;
 
 // Two shapes. Wide (head_dim 256): one CTA per SM, two S accumulators, eight softmax
 // warps, a deep ring. Narrow (64, 128): two CTAs per SM, each with one S accumulator and
 // four softmax warps; the wide shape takes 1.4 times as long there (whole prompt of
 // 16,381 rows: 562 us against 397), most of it starts and ends of CTAs in turn.
 __host__ __device__ constexpr bool ac_wide(int D) { return D == 256; }
-__host__ __device__ constexpr int ac_threads(int D) { return ac_wide(D) ? 384 : 256; }
-__host__ __device__ constexpr uint32_t ac_units(int D, int mode) {
+// Quantised pages: the wide shape at every head_dim, with eight more warps that decode.
+__host__ __device__ constexpr int ac_threads(int D, bool quant) { return quant ? 640 : ac_wide(D) ? 384 : 256; }
+__host__ __device__ constexpr uint32_t ac_units(int D, int mode, bool quant) {
     // What is left of the SM's 227 KiB (or half of it) beside the query tile and the page table.
-    return D == 256 ? (mode == kAtTree ? 9u : 10u) : D == 128 ? 4u : 5u;
+    return D == 256 ? (mode == kAtTree ? 9u : 10u) : D == 128 ? (quant ? 8u : 4u) : (quant ? 6u : 5u);
 }
-// A K or V tile (D / 64 units) has one full barrier; that of tile q serves tile q +
-// ac_tiles again, whose first unit waits for a unit of a tile behind q.
-__host__ __device__ constexpr uint32_t ac_tiles(int D, int mode) { return ac_units(D, mode) / uint32_t(D / 64) + 2u; }
-__host__ __device__ constexpr uint32_t ac_smem_bytes(int D, int mode) {
-    return 128u * uint32_t(D) * 2u + ac_units(D, mode) * kAcUnit + (ac_wide(D) ? 2048u : 0u) +
-           (mode == kAtTree ? kAcTable * 8u : 0u) + 544u;
+// A K or V tile (D / 64 units) has one full barrier (per half); that of tile q serves tile
+// q + ac_tiles again, whose first unit waits for a unit of a tile behind q.
+__host__ __device__ constexpr uint32_t ac_tiles(int D, int mode, bool quant) {
+    return ac_units(D, mode, quant) / uint32_t(D / 64) + 2u;
 }
-static_assert(ac_smem_bytes(256, kAtTree) <= 227 * 1024 && ac_smem_bytes(256, kAtWindow) <= 227 * 1024, "shared memory");
-static_assert(ac_smem_bytes(128, kAtTree) <= 113 * 1024 && ac_smem_bytes(64, kAtTree) <= 113 * 1024, "shared memory");
+__host__ __device__ constexpr uint32_t ac_smem_bytes(int D, int mode, bool quant) {
+    return 128u * uint32_t(D) * 2u + ac_units(D, mode, quant) * kAcUnit + (ac_wide(D) || quant ? 2048u : 0u) +
+           (quant ? 512u : 0u) + (mode == kAtTree ? kAcTable * 8u : 0u) + 544u;
+}
+static_assert(ac_smem_bytes(256, kAtTree, true) <= 227 * 1024 && ac_smem_bytes(256, kAtWindow, false) <= 227 * 1024, "shared memory");
+static_assert(ac_smem_bytes(128, kAtTree, false) <= 113 * 1024 && ac_smem_bytes(64, kAtTree, false) <= 113 * 1024, "shared memory");
 
 struct AttendTcMaps {
     CUtensorMap dk, dv;  // dense keys: (D, kv_heads, tokens, sequences), boxes (64, 1, 128 | V unit keys, 1)
@@ -124,19 +130,65 @@ __device__ __forceinline__ uint32_t ac_zero_times(uint32_t x, uint32_t acc) {
     }
 }
 
-template <int D, bool BF16, int MODE>
-__global__ void __launch_bounds__(ac_threads(D), ac_wide(D) ? 1 : 2)
+// Words of one block of a quantised row that starts at byte 2 * (odd ? 1 : 0) of its first
+// word: {scale, codes}. The last block of a row is an odd one (rows are whole words), so
+// its last word ends with the row.
+template <int WORDS>
+struct AcBlock {
+    uint32_t w[WORDS];
+    __device__ __forceinline__ void load(const uint8_t* row, uint32_t bi) {
+        const uint32_t at = bi * (4 * WORDS - 2);  // 34 or 18 bytes per block
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(row + (at & ~3u));
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) w[i] = __ldg(p + i);
+    }
+    __device__ __forceinline__ uint32_t code(int i, bool odd) const { return odd ? w[i + 1] : __funnelshift_r(w[i], w[i + 1], 16); }
+    __device__ __forceinline__ uint32_t scale2(bool odd) const {  // the fp16 scale twice
+        return __byte_perm(w[0], 0, odd ? 0x3232 : 0x1010);
+    }
+};
+
+__device__ __forceinline__ uint32_t ac_mul2(uint32_t a, uint32_t b) {
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// 16-byte chunk c (8 values) of a decoded block: code times scale, rounded to fp16 once.
+__device__ __forceinline__ uint4 ac_decode8(const AcBlock<9>& x, int c, bool odd, uint32_t d2) {
+    const uint32_t a = x.code(2 * c, odd), b = x.code(2 * c + 1, odd);
+    return make_uint4(ac_mul2(at_codes8<false>(__byte_perm(a, 0, 0x4140)), d2), ac_mul2(at_codes8<false>(__byte_perm(a, 0, 0x4342)), d2),
+                      ac_mul2(at_codes8<false>(__byte_perm(b, 0, 0x4140)), d2), ac_mul2(at_codes8<false>(__byte_perm(b, 0, 0x4342)), d2));
+}
+__device__ __forceinline__ uint4 ac_decode8(const AcBlock<5>& x, int c, bool odd, uint32_t d2) {
+    const uint32_t sh = (c >> 1) * 4;  // chunks 0, 1: low nibbles of bytes 0-7, 8-15; 2, 3: high nibbles
+    const uint32_t a = (x.code(2 * (c & 1), odd) >> sh) & 0x0F0F0F0Fu, b = (x.code(2 * (c & 1) + 1, odd) >> sh) & 0x0F0F0F0Fu;
+    return make_uint4(ac_mul2(at_codes4<false>(__byte_perm(a, 0, 0x4140)), d2), ac_mul2(at_codes4<false>(__byte_perm(a, 0, 0x4342)), d2),
+                      ac_mul2(at_codes4<false>(__byte_perm(b, 0, 0x4140)), d2), ac_mul2(at_codes4<false>(__byte_perm(b, 0, 0x4342)), d2));
+}
+
+// Two 16-bit values of the tensors' type as fp16 (a bf16 value past fp16's range gives an infinity).
+template <bool BF16>
+__device__ __forceinline__ uint32_t ac_to_half2(uint32_t w) {
+    if constexpr (!BF16) return w;
+    const __half2 h = __floats2half2_rn(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int D, bool BF16, int MODE, bool QUANT>
+__global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 : 2)
     attend_tc_kernel(const __grid_constant__ AttendTcMaps maps, const __grid_constant__ AttendParams P,
                      const uint32_t box) {
-    constexpr bool kWide = ac_wide(D);
+    constexpr bool kWide = ac_wide(D) || QUANT;
+    constexpr bool OB = BF16 && !QUANT;          // operands of the products in bf16 (decoded pages are fp16)
     constexpr int HS = kWide ? 2 : 1;            // softmax warps per 32 rows
     constexpr uint32_t SB = kWide ? 2 : 1;       // S accumulators
     constexpr uint32_t kScanWarps = kWide ? 1 : 2;
-    constexpr int kThreads = ac_threads(D);
+    constexpr int kThreads = ac_threads(D, QUANT);
+    constexpr uint32_t kFull = QUANT ? 8 : 1;    // arrivals on a full barrier
     constexpr uint32_t U = D / 64;               // units of a K tile, and of a V tile
     constexpr uint32_t VK = kAcUnit / (D * 2);   // keys of a V unit
-    constexpr uint32_t NU = ac_units(D, MODE);
-    constexpr uint32_t NB = ac_tiles(D, MODE);
+    constexpr uint32_t NU = ac_units(D, MODE, QUANT);
+    constexpr uint32_t NB = ac_tiles(D, MODE, QUANT);
     static_assert(NB <= kAcMaxTiles && NU >= 2 * U, "ring");
     constexpr uint32_t kQTile = 128 * D * 2;
     constexpr uint32_t kColO = SB * 128, kCols = kWide ? 512 : 256;  // S / P, then O
@@ -144,7 +196,8 @@ __global__ void __launch_bounds__(ac_threads(D), ac_wide(D) ? 1 : 2)
     uint8_t* qsm = ac_smem;
     uint8_t* ring = qsm + kQTile;
     float* pair_max = reinterpret_cast<float*>(ring + NU * kAcUnit);  // HS = 2: [2 (tile parity)][2 (half)][128]
-    int2* table = reinterpret_cast<int2*>(pair_max + (HS == 2 ? 512 : 0));
+    float* row_scale = pair_max + (HS == 2 ? 512 : 0);  // QUANT: [128] what the query rows were divided by
+    int2* table = reinterpret_cast<int2*>(row_scale + (QUANT ? 128 : 0));
     uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(table) + (MODE == kAtTree ? kAcTable * 8 : 0));
     uint64_t* full = bars;                    // [NB][2] half of the tile's units loaded (its one unit: [0])
     uint64_t* done = full + 2 * kAcMaxTiles;  // [NB] its product is done: S is there (K), O is and P is free (V)
@@ -255,8 +308,8 @@ __global__ void __launch_bounds__(ac_threads(D), ac_wide(D) ? 1 : 2)
 
     if (tid == 0) {
         for (uint32_t i = 0; i < NB; ++i) {
-            mbar_init(&full[2 * i], 1);
-            mbar_init(&full[2 * i + 1], 1);
+            mbar_init(&full[2 * i], kFull);
+            mbar_init(&full[2 * i + 1], kFull);
             mbar_init(&done[i], 1);
         }
         for (uint32_t i = 0; i < kAcScans; ++i) mbar_init(&scanned[i], kScanWarps);
@@ -274,7 +327,7 @@ __global__ void __launch_bounds__(ac_threads(D), ac_wide(D) ? 1 : 2)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (warp >= 4) {
+    if (warp >= 4 && warp < 4 + 4 * HS) {
         // The query tile, a row by D / 8 lanes.
         constexpr uint32_t kLanes = D / 8, kRows = 128 * HS / kLanes, kIts = 128 / kRows;  // rows at a time; rounds
         constexpr uint32_t kBatch = kIts < 8 ? kIts : 8;                                   // loads in flight
@@ -293,6 +346,27 @@ __global__ void __launch_bounds__(ac_threads(D), ac_wide(D) ? 1 : 2)
             for (uint32_t k = 0; k < kBatch; ++k) {
                 // (rows past the last hold copies of it: computed and not written)
                 const uint32_t row = base_row + (it + k) * kRows;
+                if constexpr (QUANT && BF16) {
+                    // As fp16, divided by a power of two that brings the row's largest value to [2^13, 2^14).
+                    float v[8], top = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t w = e == 0 ? x[k].x : e == 1 ? x[k].y : e == 2 ? x[k].z : x[k].w;
+                        const float2 f = at_unpack<BF16>(w);
+                        v[2 * e] = f.x, v[2 * e + 1] = f.y;
+                        top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+                    }
+#pragma unroll
+                    for (uint32_t o = kLanes / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    int ex = int((__float_as_uint(top) >> 23) & 255) - 127 - 13;
+                    ex = top > 0.f ? min(max(ex, -120), 114) : 0;
+                    const float inv = __uint_as_float(uint32_t(127 - ex) << 23);
+                    __half2 hv[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) hv[e] = __floats2half2_rn(v[2 * e] * inv, v[2 * e + 1] * inv);
+                    x[k] = *reinterpret_cast<uint4*>(hv);
+                    if (c == 0) row_scale[row] = __uint_as_float(uint32_t(127 + ex) << 23);
+                }
                 *reinterpret_cast<uint4*>(qd + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = x[k];
             }
         }
@@ -327,9 +401,13 @@ __global__ void __launch_bounds__(ac_threads(D), ac_wide(D) ? 1 : 2)
     };
 
     // Two CTAs per SM: registers go to the softmax warps, 4 x 32 x 72 + 4 x 32 x 184 = 256 x 128.
+    // With decoding warps: 4 x 32 x 64 + 8 x 32 x 136 + 8 x 32 x 72 = 640 x 96.
     if (warp < 4) {
-        if constexpr (HS == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (warp == 0 || (kScanWarps == 1 && warp == 2)) {
+        if constexpr (QUANT) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        else if constexpr (HS == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (QUANT && (warp == 0 || warp == 2)) {
+            // (decoding warps fill the ring)
+        } else if (warp == 0 || (kScanWarps == 1 && warp == 2)) {
             // ---- TMA producer; in the wide shape two, warp 0 for K and warp 2 for V (one thread's 20 copies
             // per tile of head_dim 256 took 2,600 cycles to issue, more than the tile's products) ----
             if (lane == 0) {
@@ -417,8 +495,8 @@ __global__ void __launch_bounds__(ac_threads(D), ac_wide(D) ? 1 : 2)
         } else if (warp == 1) {
             // ---- MMA issue: tile j, S accumulator j % SB ----
             // The warp only adds constants to descriptors and ring positions.
-            constexpr uint32_t idesc_s = pf_idesc(128, kAcKeys, BF16, false);
-            constexpr uint32_t idesc_o = pf_idesc(128, D, BF16, true);
+            constexpr uint32_t idesc_s = pf_idesc(128, kAcKeys, OB, false);
+            constexpr uint32_t idesc_o = pf_idesc(128, D, OB, true);
             const uint64_t qdesc = tc_desc_sw128(smem_u32(qsm)), kdesc = tc_desc_sw128(smem_u32(ring));
             const uint64_t vdesc = pf_desc_mn_sw128(smem_u32(ring), VK * 128);
             const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), steps = __shfl_sync(0xffffffffu, n, 0);
@@ -524,13 +602,13 @@ __global__ void __launch_bounds__(ac_threads(D), ac_wide(D) ? 1 : 2)
                                 const uint32_t key = a * VK + ((e0 + i * kStep + first) / 8) % VK;
                                 const bool dead = paged ? (key & (box - 1)) >= uint32_t(table[j * nb + (key >> bsh)].y) >> 24 : key >= live;
                                 if (dead) v4[e0 + i * kStep + first] = make_uint4(0, 0, 0, 0);
-                                else acc = ac_zero_times<BF16>(y[i].x, ac_zero_times<BF16>(y[i].y, ac_zero_times<BF16>(y[i].z, ac_zero_times<BF16>(y[i].w, acc))));
+                                else acc = ac_zero_times<OB>(y[i].x, ac_zero_times<OB>(y[i].y, ac_zero_times<OB>(y[i].z, ac_zero_times<OB>(y[i].w, acc))));
                             }
                         }
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
-                const bool bad = __any_sync(0xffffffffu, at_nonfinite<BF16>(acc));
+                const bool bad = __any_sync(0xffffffffu, at_nonfinite<OB>(acc));
                 if (lane == 0) {
                     bad_flag[(j % kAcScans) * 2 + (warp & 1)] = bad;
                     mbar_arrive(&scanned[j % kAcScans]);
@@ -538,21 +616,119 @@ __global__ void __launch_bounds__(ac_threads(D), ac_wide(D) ? 1 : 2)
                 if (!ok || __shfl_sync(0xffffffffu, *abort_flag, 0)) break;
             }
         }
+    } else if (QUANT && warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        // ---- decoding warps: K and V tiles in ring order, 256 threads per tile ----
+        // A block of 32 codes per thread and round, code times scale in fp16 (each product rounded once,
+        // half a step of fp16, 2^-11; reported where a scale above 511 could leave its range). Keys
+        // without a token become zeros.
+        const uint32_t dt = uint32_t(tid) - 384;
+        constexpr uint32_t kBlk = D / 32, kHalves = U > 1 ? 2 : 1, kPerHalf = 128 * kBlk / 256 / kHalves;  // blocks
+        uint32_t freed = 0;
+        bool ok = true, wild = false;
+        // 16-byte chunk c (of the row's D / 8) of key `key` of the tile whose first unit is `at`.
+        auto place = [&](uint32_t at, bool v, uint32_t key, uint32_t c) -> uint4* {
+            const uint32_t u = v ? key / VK : c >> 3, r = v ? key % VK : key;
+            return reinterpret_cast<uint4*>(ring + ((at + u) % NU) * kAcUnit + (v ? (c >> 3) * VK * 128 : 0u) + r * 128 +
+                                            (((c & 7) ^ (r & 7)) << 4));
+        };
+        auto blocks = [&](uint32_t at, uint32_t j, uint32_t hf, bool v, auto words) {
+            constexpr int W = decltype(words)::value;
+            AcBlock<W> x[kPerHalf];
+            bool live[kPerHalf];
+            uint32_t key[kPerHalf], bi[kPerHalf];
+#pragma unroll
+            for (uint32_t i = 0; i < kPerHalf; ++i) {
+                // K: this half's 64-dim units of every key; V: every dim of this half's keys.
+                const uint32_t e = dt + i * 256;
+                constexpr uint32_t kKb = kBlk / kHalves;
+                key[i] = v ? hf * (128 / kHalves) + e / kBlk : e / kKb;
+                bi[i] = v ? e % kBlk : hf * kKb + e % kKb;
+                const int2 ent = table[j * nb + (key[i] >> bsh)];
+                const uint32_t in = key[i] & (box - 1);
+                live[i] = in < uint32_t(ent.y) >> 24;
+                const uint8_t* base = v ? P.pv + uint64_t(prow) * P.pv_row + uint64_t(h) * P.pv_head
+                                        : P.pk + uint64_t(prow) * P.pk_row + uint64_t(h) * P.pk_head;
+                const uint64_t off = uint64_t(uint32_t(ent.x)) * (v ? P.pv_slot : P.pk_slot) +
+                                     uint64_t((uint32_t(ent.y) & 0x7FFFFFu) + in) * (v ? P.pv_tok : P.pk_tok);
+                if (live[i]) x[i].load(base + off, bi[i]);
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < kPerHalf; ++i) {
+                const bool odd = bi[i] & 1;
+                const uint32_t d2 = live[i] ? x[i].scale2(odd) : 0u;
+                wild = wild || (live[i] && (d2 & 0x7FFFu) > 0x5FFCu);  // 511
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint4 y = make_uint4(0, 0, 0, 0);
+                    if (live[i]) y = ac_decode8(x[i], c, odd, d2);
+                    *place(at, v, key[i], bi[i] * 4 + c) = y;
+                }
+            }
+        };
+        auto fill = [&](uint32_t j, bool v) {
+            const uint32_t q = v ? v_seq(j) : k_seq(j), t = tb + j, at = q * U;
+            const uint32_t last = at + U - 1;  // waits for all tiles whose units this one replaces
+            while (ok && last >= NU && freed <= (last - NU) / U) {
+                ok = pf_warp_wait(&done[freed % NB], (freed / NB) & 1);
+                ++freed;
+            }
+            if (ok && v && j >= 2) ok = pf_warp_wait(&scanned[(j - 2) % kAcScans], ((j - 2) / kAcScans) & 1);
+            if (!ok) return;
+            for (uint32_t hf = 0; hf < kHalves; ++hf) {
+                if (t < n_first) {
+                    if ((v ? P.pv_type : P.pk_type) == KVM_Q8_0) blocks(at, j, hf, v, std::integral_constant<int, 9>{});
+                    else blocks(at, j, hf, v, std::integral_constant<int, 5>{});
+                } else {
+                    // The tail's 16-bit rows.
+                    const uint32_t tok0 = (t - n_first) * kAcKeys, live = recent + rows;
+                    constexpr uint32_t kCh = D / 8, kKc = kCh / kHalves;
+#pragma unroll 4
+                    for (uint32_t e = dt; e < 128 * kCh / kHalves; e += 256) {
+                        const uint32_t key = v ? hf * (128 / kHalves) + e / kCh : e / kKc, c = v ? e % kCh : hf * kKc + e % kKc;
+                        uint4 y = make_uint4(0, 0, 0, 0);
+                        if (tok0 + key < live) {
+                            const uint8_t* row = v ? P.v + uint64_t(b) * P.v_seq + uint64_t(h) * P.v_head + uint64_t(tok0 + key) * P.v_tok
+                                                   : P.k + uint64_t(b) * P.k_seq + uint64_t(h) * P.k_head + uint64_t(tok0 + key) * P.k_tok;
+                            y = __ldg(reinterpret_cast<const uint4*>(row) + c);
+                            y = make_uint4(ac_to_half2<BF16>(y.x), ac_to_half2<BF16>(y.y), ac_to_half2<BF16>(y.z), ac_to_half2<BF16>(y.w));
+                        }
+                        *place(at, v, key, c) = y;
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[(q % NB) * 2 + hf]);
+            }
+        };
+        if (n) fill(0, false);
+        if (SB == 2 && n > 1) fill(1, false);
+        for (uint32_t j = 0; j < n && ok; ++j) {
+            fill(j, true);
+            if (j + SB < n && ok) fill(j + SB, false);
+            if (__shfl_sync(0xffffffffu, *abort_flag, 0)) break;
+        }
+        if (wild) record_error(P.status, KVM_ERR_NONFINITE, 128);
+        if (!ok && lane == 0) {
+            record_error(P.status, KVM_ERR_TIMEOUT, 129);
+            *abort_flag = 1;
+        }
     } else {
-        if constexpr (HS == 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+        if constexpr (QUANT) asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+        else if constexpr (HS == 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
         // ---- softmax: thread = packed row (tensor-memory lane), NK of the tile's keys ----
         // With two warps per 32 rows these exchange their maxes through shared memory, behind a
         // barrier of their own. A warp that gives up raises the abort flag and then arrives there,
         // and its partner looks at the flag behind every such barrier: no wait stays open.
         constexpr int NK = kAcKeys / HS, NW = NK / 32;
-        const uint32_t half = HS == 2 ? uint32_t(tid - 128) / 128 : 0, row = uint32_t(tid) & 127;
+        const uint32_t half = HS == 2 ? uint32_t(tid - 128) / 128 : 0u, row = uint32_t(tid) & 127;
         const uint32_t lane_addr = tmem + ((32u * uint32_t(warp & 3)) << 16);
         const uint32_t r = m0 + row;  // packed row
         const uint32_t ri = row_div(min(r, m_end - 1));
         const uint32_t qh = h * G + (min(r, m_end - 1) - ri * G);
         const uint32_t pair = 2 + uint32_t(warp & 3);  // barrier
         float* xch = pair_max + row;
-        const float c2 = P.scale_log2;
+        const float c2 = QUANT && BF16 ? P.scale_log2 * row_scale[row] : P.scale_log2;
         float m_used = -1e30f, l = 0.f;
         bool ok = true;
         uint32_t meet_phase = 0;
@@ -681,7 +857,7 @@ __global__ void __launch_bounds__(ac_threads(D), ac_wide(D) ? 1 : 2)
             auto store = [&](int from, uint32_t part64) {
                 uint32_t pk[32];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) pk[i] = pf_pack2<BF16>(x[from + 2 * i], x[from + 2 * i + 1]);
+                for (int i = 0; i < 32; ++i) pk[i] = pf_pack2<OB>(x[from + 2 * i], x[from + 2 * i + 1]);
                 tc_st32(lane_addr + slot * 128 + part64 * 32, pk);
             };
             auto hand_over = [&](uint64_t* bar) {
@@ -725,7 +901,7 @@ __global__ void __launch_bounds__(ac_threads(D), ac_wide(D) ? 1 : 2)
                         const uint16_t bits = *reinterpret_cast<const uint16_t*>(
                             ring + ((at + key / VK) % NU) * kAcUnit + (d / 64) * VK * 128 + kr * 128 +
                             ((((d % 64) / 8) ^ (kr & 7)) << 4) + (d % 8) * 2);
-                        if (at_nonfinite<BF16>(bits) && ((sl[k >> 5] >> (k & 31)) & 1)) f += pl[k] * at_unpack<BF16>(bits).x;
+                        if (at_nonfinite<OB>(bits) && ((sl[k >> 5] >> (k & 31)) & 1)) f += pl[k] * at_unpack<OB>(bits).x;
                     }
                     fix[d] = f;
                 }
@@ -733,7 +909,7 @@ __global__ void __launch_bounds__(ac_threads(D), ac_wide(D) ? 1 : 2)
                 for (uint32_t a = 0; a < U; ++a) {
                     uint16_t* v2 = reinterpret_cast<uint16_t*>(ring + ((at + a) % NU) * kAcUnit);
                     for (uint32_t e = uint32_t(tid - 128); e < kAcUnit / 2; e += 128 * HS)
-                        if (at_nonfinite<BF16>(v2[e])) v2[e] = 0;
+                        if (at_nonfinite<OB>(v2[e])) v2[e] = 0;
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 meet();

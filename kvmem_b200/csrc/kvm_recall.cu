@@ -2312,6 +2312,15 @@ bool attend_is(const char* name) {
     return e && std::strcmp(e, name) == 0;
 }
 
+// Tokens of a page that the tcgen05 kernel takes at a time: the largest power of two up to 128
+// that divides the page, 16 at least.
+bool page_box(uint32_t page_tokens, uint32_t* box) {
+    uint32_t b = 128;
+    while (page_tokens % b) b >>= 1;
+    *box = b;
+    return b >= 16 && page_tokens < (1u << 23);
+}
+
 // Tensor maps of the tcgen05 kernel. False where TMA cannot express the operands: a
 // zero stride (one tensor for all sequences), or pages that are no multiple of 16 tokens.
 bool attend_tc_maps(const AttendParams& p, uint32_t head_dim, bool bf16, int mode, uint32_t pool_rows, AttendTcMaps* maps,
@@ -2338,10 +2347,8 @@ bool attend_tc_maps(const AttendParams& p, uint32_t head_dim, bool bf16, int mod
         if (!encode(v ? &maps->dv : &maps->dk, v ? p.v : p.k, 4, dims, strides, boxes)) return false;
     }
     if (mode == kAtWindow) return true;
-    uint32_t b = 128;
-    while (p.page_tokens % b) b >>= 1;
-    if (b < 16 || p.page_tokens >= (1u << 23)) return false;
-    *box = b;
+    if (!page_box(p.page_tokens, box)) return false;
+    const uint32_t b = *box;
     for (int v = 0; v < 2; ++v) {
         const cuuint64_t dims[5] = {head_dim, p.kv_heads, p.page_tokens, p.pool_slots, pool_rows};
         const uint64_t slot = v ? p.pv_slot : p.pk_slot;
@@ -2398,11 +2405,11 @@ int attend_launch(kvm_ctx* c, AttendParams& p, uint32_t head_dim, bool bf16, int
     const uint64_t rows = uint64_t(p.seqs) * p.width * p.q_heads;
     const size_t row_bytes = size_t(head_dim) * 4 + 8;
     const bool force_tc = attend_is("tc");
-    if (!quant && (packed > 64 || force_tc) && !attend_is("mma")) {
+    if ((quant || packed > 64 || force_tc) && !attend_is("mma")) {
         AttendTcMaps maps;
         std::memset(&maps, 0, sizeof maps);
         uint32_t box = 0;
-        if (attend_tc_maps(p, head_dim, bf16, mode, pool_rows, &maps, &box)) {
+        if (quant ? page_box(p.page_tokens, &box) : attend_tc_maps(p, head_dim, bf16, mode, pool_rows, &maps, &box)) {
             p.m_tiles = (packed + 127) / 128;
             // One CTA's chunk has at most kAcTable page boxes
             uint32_t least = 1;
@@ -2416,12 +2423,12 @@ int attend_launch(kvm_ctx* c, AttendParams& p, uint32_t head_dim, bool bf16, int
             }
             if (!too_many) {
                 const uint64_t tiles = (keys + kAcKeys - 1) / kAcKeys + 1;
-                const bool wide = ac_wide(int(head_dim));
+                const bool wide = ac_wide(int(head_dim)) || quant;
                 p.splits = attend_splits(c, uint64_t(p.seqs) * p.kv_heads * p.m_tiles, uint64_t(c->num_sms) * (wide ? 1 : 2), tiles, wide ? 1.3 : 1.8, 7.0,
                                          rows, row_bytes, least);
                 KVM_TRY(attend_scratch(c, p, head_dim, s));
-                KVM_TRY(bf16 ? launch_attend_tc_t<true>(c, maps, p, head_dim, mode, box, s)
-                             : launch_attend_tc_t<false>(c, maps, p, head_dim, mode, box, s));
+                KVM_TRY(bf16 ? launch_attend_tc_t<true>(c, maps, p, head_dim, mode, quant, box, s)
+                             : launch_attend_tc_t<false>(c, maps, p, head_dim, mode, quant, box, s));
                 return launch_attend_combine(c, p, head_dim, bf16, s);
             }
         }

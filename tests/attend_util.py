@@ -6,14 +6,18 @@ A = sum_t p_t |v_t| / l, to first order. Logits come from exact products summed 
 steps of 16 is off by at most (D / 16 + 8) 2^-22 S with S = scale * sum_d |q_d k_d| (8 more steps for the scale, the
 max and exp2), which shifts each p_t by that, relative: 2 delta A, delta the largest over the row's keys. fp16 P below
 its subnormal step lose at most 2^-25 each against a row maximum of 1: T 2^-25 max|v|; with block scales the same
-after the lift by 64. A factor 1.1 covers the second order."""
+after the lift by 64. A factor 1.1 covers the second order.
+
+Pages decoded to fp16 (the tcgen05 kernel): each K and V value code * scale is rounded to fp16 once, 2^-11 relative, which
+shifts a logit by at most 2^-11 S and o by at most 2^-11 A more; values below fp16's smallest normal number by 2^-25 each,
+which D 2^-25 scale max|q| and 2^-25 cover."""
 import numpy as np
 import torch
 
 UNIT = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
 
 
-def attend64(q, k, v, see, scale):
+def attend64(q, k, v, see, scale, decoded=False):
     """q [N][Hq][D], k, v [T][Hkv][D], see bool [N][T] -> out, lse, A, delta (float64, per row and head)."""
     q, k, v = q.double(), k.double(), v.double()
     n, hq, dim = q.shape
@@ -29,10 +33,14 @@ def attend64(q, k, v, see, scale):
         for h in range(hq):
             kk, vv = k[t, h // g], v[t, h // g]
             s = kk @ q[i, h] * scale
-            delta[i, h] = (dim / 16 + 8) * 2.0 ** -22 * float((kk.abs() @ q[i, h].abs()).max()) * scale
+            delta[i, h] = ((dim / 16 + 8) * 2.0 ** -22 + (2.0 ** -11 if decoded else 0)) * float((kk.abs() @ q[i, h].abs()).max()) * scale
+            if decoded:
+                delta[i, h] += dim * 2.0 ** -25 * scale * float(q[i, h].abs().max())
             lse[i, h] = torch.logsumexp(s, 0)
             p = torch.exp(s - lse[i, h])
             out[i, h], size[i, h] = p @ vv, p @ vv.abs()
+            if decoded:  # u (A + |o|) + 2^-11 A + 2^-25 with u the output type's, so at most twice u A where u = 2^-11
+                size[i, h] = 2 * size[i, h] + 2.0 ** -13
     return out, lse, size, delta
 
 

@@ -104,7 +104,7 @@ class Problem:
         a.update(kw)
         return self.pool.tree_attention(self.q.to(DEV), *self.tail_d, **a)
 
-    def verify(self, out, lse, lists="own", see=None, rows=None, scale=None):
+    def verify(self, out, lse, lists="own", see=None, rows=None, scale=None, decoded=None):
         see = self.see if see is None else see
         for i in range(self.seqs):
             r = self.row0 + i * self.step
@@ -119,7 +119,8 @@ class Problem:
                 planes.append(torch.cat(parts + [tail[i, :self.recent[i] + n].double()]))
             held = planes[0].shape[0] - n
             vis = torch.cat([torch.ones(n, held, dtype=torch.bool), torch.from_numpy(see[i][:n, :n].copy())], 1)
-            exp = attend64(self.q[i, :n], planes[0], planes[1], vis, scale or 1 / math.sqrt(self.dim))
+            exp = attend64(self.q[i, :n], planes[0], planes[1], vis, scale or 1 / math.sqrt(self.dim),
+                           decoded=bool(self.kinds) if decoded is None else decoded)
             vmax = float(planes[1].abs().max()) if planes[1].numel() else 0.0
             check(out[i, :n], None if lse is None else lse[i, :n], exp, self.dtype, held + n, vmax)
 
@@ -162,14 +163,45 @@ def test_tree(ctx, monkeypatch, case, splits, kernel):
     (2, 5, 16, 8, 128, 48, 30, 11, [1440, 1000], [47, 0], torch.float16),
     (1, 33, 12, 3, 64, 16, 40, 25, [601], [3], torch.bfloat16),      # rows of 68 and 36 bytes
 ])
-@pytest.mark.parametrize("splits", ["", "3"])
-def test_quantised_pages(ctx, monkeypatch, kinds, case, splits):
+@pytest.mark.parametrize("splits", ["", "1", "3"])
+@pytest.mark.parametrize("kernel", ["mma", "tc"])
+def test_quantised_pages(ctx, monkeypatch, kinds, case, splits, kernel):
+    if kernel == "tc" and case[5] % 16:
+        pytest.skip("the tcgen05 kernel takes pages of a multiple of 16 tokens")
+    monkeypatch.setenv("KVM_ATTEND", kernel)
     if splits:
         monkeypatch.setenv("KVM_ATTEND_SPLITS", splits)
     p = Problem(ctx, 12, *case, kinds=kinds)
     out, lse = p.call()
     ctx.check_status()
-    p.verify(out, lse)
+    p.verify(out, lse, decoded=kernel == "tc")
+
+
+def test_quantised_holes_and_poisoned_nodes(ctx, monkeypatch):
+    """All resident pages with free slots between them over many tiles, garbage behind the tail, NaN in a drafted node."""
+    monkeypatch.setenv("KVM_ATTEND", "tc")
+    monkeypatch.setenv("KVM_ATTEND_SPLITS", "1")
+    p = Problem(ctx, 26, 1, 9, 16, 2, 128, 32, 90, 70, [89 * 32 + 3], [50], torch.bfloat16, kinds=(U.Q8_0, U.Q4_0), garbage=True)
+    out, lse = p.call(lists=None)
+    ctx.check_status()
+    p.verify(out, lse, lists=None, decoded=True)
+    j = 4
+    for x in p.tail_d:
+        x[0, 50 + j, :, ::7] = NAN
+    out, lse = p.call(lists=None)
+    for i in range(9):
+        assert torch.isfinite(out[0, i]).all().item() == (not p.see[0][i, j])
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -60, 2.0 ** -20, 3.0e4, 2.0 ** 60])
+def test_quantised_pages_take_queries_of_any_size(ctx, scale):
+    """bf16 queries far outside fp16's range; the logit scale keeps the logits where they were."""
+    p = Problem(ctx, 27, 1, 4, 8, 2, 128, 64, 12, 6, [700], [0], torch.bfloat16, kinds=(U.Q8_0, U.Q8_0))
+    p.q = (p.q.float() * scale).to(torch.bfloat16)
+    p.tail_d[0].zero_(), p.tail[0].zero_()
+    out, lse = p.call(scale=0.09 / scale)
+    ctx.check_status()
+    p.verify(out, lse, scale=0.09 / scale, decoded=True)
 
 
 @pytest.mark.parametrize("kinds", [None, (U.Q8_0, U.Q4_0)])
