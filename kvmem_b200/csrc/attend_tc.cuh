@@ -44,6 +44,8 @@ constexpr uint32_t kAcUnit = 16384;      // bytes per ring unit
 constexpr uint32_t kAcTable = 512;       // page boxes of one CTA's key chunk
 constexpr uint32_t kAcScans = 8;         // V tiles that the scan's barriers tell apart
 constexpr uint32_t kAcMaxTiles = 8;
+constexpr uint32_t kAcRaw = 3;           // quantised pages: stages of 32 blocks on their way to a decoding warp
+constexpr uint32_t kAcRawBytes = 32 * 34;
 
 // Two shapes. Wide (head_dim 256): one CTA per SM, two S accumulators, eight softmax
 // warps, a deep ring. Narrow (64, 128): two CTAs per SM, each with one S accumulator and
@@ -54,7 +56,7 @@ __host__ __device__ constexpr bool ac_wide(int D) { return D == 256; }
 __host__ __device__ constexpr int ac_threads(int D, bool quant) { return quant ? 640 : ac_wide(D) ? 384 : 256; }
 __host__ __device__ constexpr uint32_t ac_units(int D, int mode, bool quant) {
     // What is left of the SM's 227 KiB (or half of it) beside the query tile and the page table.
-    return D == 256 ? (mode == kAtTree ? 9u : 10u) : D == 128 ? (quant ? 8u : 4u) : (quant ? 6u : 5u);
+    return D == 256 ? (quant ? 8u : mode == kAtTree ? 9u : 10u) : D == 128 ? (quant ? 8u : 4u) : (quant ? 6u : 5u);
 }
 // A K or V tile (D / 64 units) has one full barrier (per half); that of tile q serves tile
 // q + ac_tiles again, whose first unit waits for a unit of a tile behind q.
@@ -63,7 +65,7 @@ __host__ __device__ constexpr uint32_t ac_tiles(int D, int mode, bool quant) {
 }
 __host__ __device__ constexpr uint32_t ac_smem_bytes(int D, int mode, bool quant) {
     return 128u * uint32_t(D) * 2u + ac_units(D, mode, quant) * kAcUnit + (ac_wide(D) || quant ? 2048u : 0u) +
-           (quant ? 512u : 0u) + (mode == kAtTree ? kAcTable * 8u : 0u) + 544u;
+           (quant ? 512u + 8u * kAcRaw * kAcRawBytes : 0u) + (mode == kAtTree ? kAcTable * 8u : 0u) + 544u;
 }
 static_assert(ac_smem_bytes(256, kAtTree, true) <= 227 * 1024 && ac_smem_bytes(256, kAtWindow, false) <= 227 * 1024, "shared memory");
 static_assert(ac_smem_bytes(128, kAtTree, false) <= 113 * 1024 && ac_smem_bytes(64, kAtTree, false) <= 113 * 1024, "shared memory");
@@ -133,16 +135,18 @@ __device__ __forceinline__ uint32_t ac_zero_times(uint32_t x, uint32_t acc) {
 // Words of one block of a quantised row that starts at byte 2 * (odd ? 1 : 0) of its first
 // word: {scale, codes}. The last block of a row is an odd one (rows are whole words), so
 // its last word ends with the row.
-template <int WORDS>
 struct AcBlock {
-    uint32_t w[WORDS];
-    __device__ __forceinline__ void load(const uint8_t* row, uint32_t bi) {
-        const uint32_t at = bi * (4 * WORDS - 2);  // 34 or 18 bytes per block
-        const uint32_t* p = reinterpret_cast<const uint32_t*>(row + (at & ~3u));
+    uint32_t w[9];
+    __device__ __forceinline__ void load(const uint8_t* row, uint32_t bi, bool q8) {  // 34 or 18 bytes per block
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(row + ((bi * (q8 ? 34u : 18u)) & ~3u));
 #pragma unroll
-        for (int i = 0; i < WORDS; ++i) w[i] = __ldg(p + i);
+        for (int i = 0; i < 5; ++i) w[i] = p[i];
+        if (q8) {
+#pragma unroll
+            for (int i = 5; i < 9; ++i) w[i] = p[i];
+        }
     }
-    __device__ __forceinline__ uint32_t code(int i, bool odd) const { return odd ? w[i + 1] : __funnelshift_r(w[i], w[i + 1], 16); }
+    __device__ __forceinline__ uint32_t code(int i, bool odd) const { return __funnelshift_rc(w[i], w[i + 1], odd ? 32 : 16); }
     __device__ __forceinline__ uint32_t scale2(bool odd) const {  // the fp16 scale twice
         return __byte_perm(w[0], 0, odd ? 0x3232 : 0x1010);
     }
@@ -154,12 +158,12 @@ __device__ __forceinline__ uint32_t ac_mul2(uint32_t a, uint32_t b) {
 }
 
 // 16-byte chunk c (8 values) of a decoded block: code times scale, rounded to fp16 once.
-__device__ __forceinline__ uint4 ac_decode8(const AcBlock<9>& x, int c, bool odd, uint32_t d2) {
+__device__ __forceinline__ uint4 ac_decode_q8(const AcBlock& x, int c, bool odd, uint32_t d2) {
     const uint32_t a = x.code(2 * c, odd), b = x.code(2 * c + 1, odd);
     return make_uint4(ac_mul2(at_codes8<false>(__byte_perm(a, 0, 0x4140)), d2), ac_mul2(at_codes8<false>(__byte_perm(a, 0, 0x4342)), d2),
                       ac_mul2(at_codes8<false>(__byte_perm(b, 0, 0x4140)), d2), ac_mul2(at_codes8<false>(__byte_perm(b, 0, 0x4342)), d2));
 }
-__device__ __forceinline__ uint4 ac_decode8(const AcBlock<5>& x, int c, bool odd, uint32_t d2) {
+__device__ __forceinline__ uint4 ac_decode_q4(const AcBlock& x, int c, bool odd, uint32_t d2) {
     const uint32_t sh = (c >> 1) * 4;  // chunks 0, 1: low nibbles of bytes 0-7, 8-15; 2, 3: high nibbles
     const uint32_t a = (x.code(2 * (c & 1), odd) >> sh) & 0x0F0F0F0Fu, b = (x.code(2 * (c & 1) + 1, odd) >> sh) & 0x0F0F0F0Fu;
     return make_uint4(ac_mul2(at_codes4<false>(__byte_perm(a, 0, 0x4140)), d2), ac_mul2(at_codes4<false>(__byte_perm(a, 0, 0x4342)), d2),
@@ -197,7 +201,8 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
     uint8_t* ring = qsm + kQTile;
     float* pair_max = reinterpret_cast<float*>(ring + NU * kAcUnit);  // HS = 2: [2 (tile parity)][2 (half)][128]
     float* row_scale = pair_max + (HS == 2 ? 512 : 0);  // QUANT: [128] what the query rows were divided by
-    int2* table = reinterpret_cast<int2*>(row_scale + (QUANT ? 128 : 0));
+    uint8_t* raw = reinterpret_cast<uint8_t*>(row_scale + (QUANT ? 128 : 0));  // QUANT: [8 warps][kAcRaw] blocks
+    int2* table = reinterpret_cast<int2*>(raw + (QUANT ? 8 * kAcRaw * kAcRawBytes : 0));
     uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(table) + (MODE == kAtTree ? kAcTable * 8 : 0));
     uint64_t* full = bars;                    // [NB][2] half of the tile's units loaded (its one unit: [0])
     uint64_t* done = full + 2 * kAcMaxTiles;  // [NB] its product is done: S is there (K), O is and P is free (V)
@@ -388,6 +393,9 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
     // One S: K0 V0 K1 V1 ..; two: K0 K1 V0 K2 V1 .. V(n - 1).
     auto k_seq = [&](uint32_t j) { return SB == 1 ? 2 * j : (j ? 2 * j - 1 : 0); };
     auto v_seq = [&](uint32_t j) { return SB == 1 ? 2 * j + 1 : (j + 1 == n ? 2 * n - 1 : 2 * j + 2); };
+    // The q-th tile of the ring (SB = 2): K or V, and which.
+    [[maybe_unused]] auto ring_v = [&](uint32_t q) { return q + 1 == 2 * n || (q && !(q & 1)); };
+    [[maybe_unused]] auto ring_tile = [&](uint32_t q) { return q + 1 == 2 * n ? n - 1 : ring_v(q) ? q / 2 - 1 : (q + 1) / 2; };
     // Whether some row of the CTA does not see all of tile t.
     auto in_part = [&](uint32_t t) -> bool {
         if constexpr (MODE == kAtWindow) {
@@ -406,7 +414,7 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
         if constexpr (QUANT) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         else if constexpr (HS == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (QUANT && (warp == 0 || warp == 2)) {
-            // (decoding warps fill the ring)
+            // (the decoding warps fill the ring)
         } else if (warp == 0 || (kScanWarps == 1 && warp == 2)) {
             // ---- TMA producer; in the wide shape two, warp 0 for K and warp 2 for V (one thread's 20 copies
             // per tile of head_dim 256 took 2,600 cycles to issue, more than the tile's products) ----
@@ -522,6 +530,8 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
                 for (uint32_t a = 0; a < U; ++a) {
                     if (a == 0 || a == U / 2) {
                         if (!pf_warp_wait(&full[kp.b * 2 + (a ? 1 : 0)], kp.ph)) return false;
+                        // Decoded K comes in halves of keys, loaded K in halves of dims.
+                        if (QUANT && U > 1 && a == 0 && !pf_warp_wait(&full[kp.b * 2 + 1], kp.ph)) return false;
                         tc_fence_after();
                     }
                     const uint64_t kd = kdesc + kp.s * (kAcUnit >> 4);
@@ -619,11 +629,13 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
     } else if (QUANT && warp >= 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         // ---- decoding warps: K and V tiles in ring order, 256 threads per tile ----
-        // A block of 32 codes per thread and round, code times scale in fp16 (each product rounded once,
-        // half a step of fp16, 2^-11; reported where a scale above 511 could leave its range). Keys
-        // without a token become zeros.
-        const uint32_t dt = uint32_t(tid) - 384;
-        constexpr uint32_t kBlk = D / 32, kHalves = U > 1 ? 2 : 1, kPerHalf = 128 * kBlk / 256 / kHalves;  // blocks
+        // Each warp brings the rows of 32 blocks at a time into stages of its own (16, 8 or 4 bytes per copy,
+        // as the rows' sizes and strides allow; a thread's loads of its own block touch 8 or more lines per
+        // word, and with them a tile of head_dim 256 took 12,400 cycles), then one thread decodes
+        // one block: code times scale in fp16, each product rounded once, half a step of fp16, 2^-11;
+        // reported where a scale above 511 could leave its range. Keys without a token become zeros.
+        const uint32_t dw = uint32_t(warp) - 12, dt = uint32_t(tid) - 384;
+        constexpr uint32_t kBlk = D / 32, kWarpKeys = 32 / kBlk, kKeys = 8 * kWarpKeys, kHalves = U > 1 ? 2 : 1;
         uint32_t freed = 0;
         bool ok = true, wild = false;
         // 16-byte chunk c (of the row's D / 8) of key `key` of the tile whose first unit is `at`.
@@ -632,82 +644,127 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
             return reinterpret_cast<uint4*>(ring + ((at + u) % NU) * kAcUnit + (v ? (c >> 3) * VK * 128 : 0u) + r * 128 +
                                             (((c & 7) ^ (r & 7)) << 4));
         };
-        auto blocks = [&](uint32_t at, uint32_t j, uint32_t hf, bool v, auto words) {
-            constexpr int W = decltype(words)::value;
-            AcBlock<W> x[kPerHalf];
-            bool live[kPerHalf];
-            uint32_t key[kPerHalf], bi[kPerHalf];
-#pragma unroll
-            for (uint32_t i = 0; i < kPerHalf; ++i) {
-                // K: this half's 64-dim units of every key; V: every dim of this half's keys.
-                const uint32_t e = dt + i * 256;
-                constexpr uint32_t kKb = kBlk / kHalves;
-                key[i] = v ? hf * (128 / kHalves) + e / kBlk : e / kKb;
-                bi[i] = v ? e % kBlk : hf * kKb + e % kKb;
-                const int2 ent = table[j * nb + (key[i] >> bsh)];
-                const uint32_t in = key[i] & (box - 1);
-                live[i] = in < uint32_t(ent.y) >> 24;
-                const uint8_t* base = v ? P.pv + uint64_t(prow) * P.pv_row + uint64_t(h) * P.pv_head
-                                        : P.pk + uint64_t(prow) * P.pk_row + uint64_t(h) * P.pk_head;
-                const uint64_t off = uint64_t(uint32_t(ent.x)) * (v ? P.pv_slot : P.pk_slot) +
-                                     uint64_t((uint32_t(ent.y) & 0x7FFFFFu) + in) * (v ? P.pv_tok : P.pk_tok);
-                if (live[i]) x[i].load(base + off, bi[i]);
-            }
-#pragma unroll
-            for (uint32_t i = 0; i < kPerHalf; ++i) {
-                const bool odd = bi[i] & 1;
-                const uint32_t d2 = live[i] ? x[i].scale2(odd) : 0u;
-                wild = wild || (live[i] && (d2 & 0x7FFFu) > 0x5FFCu);  // 511
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint4 y = make_uint4(0, 0, 0, 0);
-                    if (live[i]) y = ac_decode8(x[i], c, odd, d2);
-                    *place(at, v, key[i], bi[i] * 4 + c) = y;
-                }
-            }
+        auto done_half = [&](uint32_t q, uint32_t hf) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[(q % NB) * 2 + hf]);
         };
-        auto fill = [&](uint32_t j, bool v) {
-            const uint32_t q = v ? v_seq(j) : k_seq(j), t = tb + j, at = q * U;
-            const uint32_t last = at + U - 1;  // waits for all tiles whose units this one replaces
-            while (ok && last >= NU && freed <= (last - NU) / U) {
+        const bool kq8 = P.pk_type == KVM_Q8_0, vq8 = P.pv_type == KVM_Q8_0;
+        // This thread's key (of a stage) and block: the stores of eight lanes fall on the eight chunks of the
+        // swizzle (eight keys, or four keys and a pair of blocks).
+        const uint32_t mine = kBlk == 8 ? lane & 3u : (uint32_t(lane) >> 3) / kBlk * 8 + (lane & 7u);
+        const uint32_t bi = kBlk == 8 ? uint32_t(lane) >> 2 : (uint32_t(lane) >> 3) % kBlk;
+        const bool odd = bi & 1;
+        const uint8_t* kbase = P.pk + uint64_t(prow) * P.pk_row + uint64_t(h) * P.pk_head;
+        const uint8_t* vbase = P.pv + uint64_t(prow) * P.pv_row + uint64_t(h) * P.pv_head;
+        uint8_t* stage = raw + dw * kAcRaw * kAcRawBytes;
+        // The warp's keys of a stage lie in one box (boxes hold 16 tokens or more): its entry.
+        auto entry = [&](uint32_t q, uint32_t k0) {
+            const uint32_t key = k0 + dw * kWarpKeys;
+            int2 e = table[ring_tile(q) * nb + (key >> bsh)];
+            const uint32_t in = key & (box - 1), held = uint32_t(e.y) >> 24;
+            e.y = int((uint32_t(e.y) & 0x7FFFFFu) + in | (held > in ? min(held - in, kWarpKeys) : 0u) << 24);
+            return e;  // {slot, first token | tokens << 24}
+        };
+        uint32_t cq = 0, ck = 0, cs = 0;  // next stage to copy: ring position, key, buffer
+        auto copy = [&]() {
+            while (cq < 2 * n && tb + ring_tile(cq) >= n_first) ++cq;
+            if (cq < 2 * n) {
+                const bool v = ring_v(cq);
+                const int2 e = entry(cq, ck);
+                const uint64_t tok_bytes = v ? P.pv_tok : P.pk_tok;
+                const uint8_t* src = (v ? vbase : kbase) + uint64_t(uint32_t(e.x)) * (v ? P.pv_slot : P.pk_slot) +
+                                     uint64_t(uint32_t(e.y) & 0xFFFFFFu) * tok_bytes;
+                const uint32_t rb = v ? P.pv_bytes : P.pk_bytes, gran = v ? P.pv_gran : P.pk_gran;
+                const uint32_t some = uint32_t(e.y) >> 24, dst = smem_u32(stage + cs * kAcRawBytes);
+                auto rows_of = [&](auto g, auto bytes) {
+                    constexpr uint32_t kG = decltype(g)::value, kPer = kBlk * decltype(bytes)::value / kG;
+#pragma unroll
+                    for (uint32_t i0 = 0; i0 < kWarpKeys * kPer; i0 += 32) {
+                        const uint32_t i = i0 + lane, r = i / kPer, o = (i - r * kPer) * kG;
+                        if (r >= some) continue;
+                        const uint8_t* from = src + r * tok_bytes + o;
+                        if constexpr (kG == 16) at_cp16(dst + i * kG, from, true);
+                        else if constexpr (kG == 8) at_cp8(dst + i * kG, from, true);
+                        else at_cp4(dst + i * kG, from, true);
+                    }
+                };
+                auto plane = [&](auto bytes) {
+                    if constexpr (kBlk * decltype(bytes)::value % 16 == 0) {
+                        if (gran == 16) return rows_of(std::integral_constant<uint32_t, 16>{}, bytes);
+                    }
+                    if constexpr (kBlk * decltype(bytes)::value % 8 == 0) {
+                        if (gran >= 8) return rows_of(std::integral_constant<uint32_t, 8>{}, bytes);
+                    }
+                    rows_of(std::integral_constant<uint32_t, 4>{}, bytes);
+                };
+                if (rb == kBlk * 34) plane(std::integral_constant<uint32_t, 34>{});
+                else plane(std::integral_constant<uint32_t, 18>{});
+                cs = cs + 1 == kAcRaw ? 0 : cs + 1;
+                ck += kKeys;
+                if (ck == uint32_t(kAcKeys)) ck = 0, ++cq;
+            }
+            at_commit();
+        };
+#pragma unroll 1
+        for (uint32_t i = 0; i < kAcRaw; ++i) copy();
+        uint32_t rs = 0;  // the buffer to read next
+        AcBlock x;
+        for (uint32_t q = 0; q < 2 * n && ok; ++q) {
+            const bool v = ring_v(q);
+            const uint32_t j = ring_tile(q), t = tb + j, at = q * U, last = at + U - 1;
+            while (ok && last >= NU && freed <= (last - NU) / U) {  // the tiles whose units this one replaces
                 ok = pf_warp_wait(&done[freed % NB], (freed / NB) & 1);
                 ++freed;
             }
             if (ok && v && j >= 2) ok = pf_warp_wait(&scanned[(j - 2) % kAcScans], ((j - 2) / kAcScans) & 1);
-            if (!ok) return;
-            for (uint32_t hf = 0; hf < kHalves; ++hf) {
-                if (t < n_first) {
-                    if ((v ? P.pv_type : P.pk_type) == KVM_Q8_0) blocks(at, j, hf, v, std::integral_constant<int, 9>{});
-                    else blocks(at, j, hf, v, std::integral_constant<int, 5>{});
-                } else {
-                    // The tail's 16-bit rows.
-                    const uint32_t tok0 = (t - n_first) * kAcKeys, live = recent + rows;
-                    constexpr uint32_t kCh = D / 8, kKc = kCh / kHalves;
-#pragma unroll 4
-                    for (uint32_t e = dt; e < 128 * kCh / kHalves; e += 256) {
-                        const uint32_t key = v ? hf * (128 / kHalves) + e / kCh : e / kKc, c = v ? e % kCh : hf * kKc + e % kKc;
-                        uint4 y = make_uint4(0, 0, 0, 0);
-                        if (tok0 + key < live) {
-                            const uint8_t* row = v ? P.v + uint64_t(b) * P.v_seq + uint64_t(h) * P.v_head + uint64_t(tok0 + key) * P.v_tok
-                                                   : P.k + uint64_t(b) * P.k_seq + uint64_t(h) * P.k_head + uint64_t(tok0 + key) * P.k_tok;
-                            y = __ldg(reinterpret_cast<const uint4*>(row) + c);
-                            y = make_uint4(ac_to_half2<BF16>(y.x), ac_to_half2<BF16>(y.y), ac_to_half2<BF16>(y.z), ac_to_half2<BF16>(y.w));
-                        }
-                        *place(at, v, key, c) = y;
-                    }
+            if (!ok || __shfl_sync(0xffffffffu, *abort_flag, 0)) break;
+            if (t < n_first) {
+                for (uint32_t k0 = 0; k0 < uint32_t(kAcKeys) && ok; k0 += kKeys) {
+                    at_wait<kAcRaw - 1>();
+                    __syncwarp();
+                    x.load(stage + rs * kAcRawBytes + mine * (v ? P.pv_bytes : P.pk_bytes), bi, v ? vq8 : kq8);
+                    rs = rs + 1 == kAcRaw ? 0 : rs + 1;
+                    const bool live = mine < uint32_t(entry(q, k0).y) >> 24;
+                    __syncwarp();
+                    copy();
+                    const uint32_t key = k0 + dw * kWarpKeys + mine, d2 = live ? x.scale2(odd) : 0u;
+                    wild = wild || (d2 & 0x7FFFu) > 0x5FFCu;  // 511
+                    // (a dead key's bytes are whatever the stage held; its scale is zero)
+                    uint4* to[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) to[c] = place(at, v, key, bi * 4 + c);
+                    auto put = [&](auto as_q8) {
+                        uint4 z[4];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) z[c] = decltype(as_q8)::value ? ac_decode_q8(x, c, odd, d2) : ac_decode_q4(x, c, odd, d2);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) *to[c] = z[c];
+                    };
+                    if (v ? vq8 : kq8) put(std::true_type{});
+                    else put(std::false_type{});
+                    if ((k0 + kKeys) % (kAcKeys / kHalves) == 0) done_half(q, (k0 + kKeys) / (kAcKeys / kHalves) - 1);
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&full[(q % NB) * 2 + hf]);
+            } else {
+                // The tail's 16-bit rows.
+                const uint32_t tok0 = (t - n_first) * kAcKeys, most = recent + rows;
+                constexpr uint32_t kCh = D / 8;
+#pragma unroll 4
+                for (uint32_t e = dt; e < 128 * kCh; e += 256) {
+                    const uint32_t key = e / kCh, c = e % kCh;
+                    uint4 z = make_uint4(0, 0, 0, 0);
+                    if (tok0 + key < most) {
+                        const uint8_t* row = v ? P.v + uint64_t(b) * P.v_seq + uint64_t(h) * P.v_head + uint64_t(tok0 + key) * P.v_tok
+                                               : P.k + uint64_t(b) * P.k_seq + uint64_t(h) * P.k_head + uint64_t(tok0 + key) * P.k_tok;
+                        z = __ldg(reinterpret_cast<const uint4*>(row) + c);
+                        z = make_uint4(ac_to_half2<BF16>(z.x), ac_to_half2<BF16>(z.y), ac_to_half2<BF16>(z.z), ac_to_half2<BF16>(z.w));
+                    }
+                    *place(at, v, key, c) = z;
+                }
+                for (uint32_t hf = 0; hf < kHalves; ++hf) done_half(q, hf);
             }
-        };
-        if (n) fill(0, false);
-        if (SB == 2 && n > 1) fill(1, false);
-        for (uint32_t j = 0; j < n && ok; ++j) {
-            fill(j, true);
-            if (j + SB < n && ok) fill(j + SB, false);
-            if (__shfl_sync(0xffffffffu, *abort_flag, 0)) break;
         }
+        at_wait<0>();
         if (wild) record_error(P.status, KVM_ERR_NONFINITE, 128);
         if (!ok && lane == 0) {
             record_error(P.status, KVM_ERR_TIMEOUT, 129);
