@@ -658,24 +658,33 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
         const uint8_t* kbase = P.pk + uint64_t(prow) * P.pk_row + uint64_t(h) * P.pk_head;
         const uint8_t* vbase = P.pv + uint64_t(prow) * P.pv_row + uint64_t(h) * P.pv_head;
         uint8_t* stage = raw + dw * kAcRaw * kAcRawBytes;
-        // The warp's keys of a stage lie in one box (boxes hold 16 tokens or more): its entry.
-        auto entry = [&](uint32_t q, uint32_t k0) {
+        // The warp's keys of a stage lie in one box (boxes hold 16 tokens or more): {slot, first token | tokens << 24}.
+        auto entry = [&](const int2* ents, uint32_t k0) {
             const uint32_t key = k0 + dw * kWarpKeys;
-            int2 e = table[ring_tile(q) * nb + (key >> bsh)];
+            int2 e = ents[key >> bsh];
             const uint32_t in = key & (box - 1), held = uint32_t(e.y) >> 24;
             e.y = int((uint32_t(e.y) & 0x7FFFFFu) + in | (held > in ? min(held - in, kWarpKeys) : 0u) << 24);
-            return e;  // {slot, first token | tokens << 24}
+            return e;
         };
-        uint32_t cq = 0, ck = 0, cs = 0;  // next stage to copy: ring position, key, buffer
+        // Next stage to copy: ring position, key, buffer; and what its tile's stages share.
+        uint32_t cq = 0, ck = 0, cs = 0, c_gran = 0;
+        const int2* c_ents = table;
+        const uint8_t* c_base = nullptr;
+        uint64_t c_slot = 0, c_tok = 0;
+        bool c_q8 = false;
         auto copy = [&]() {
-            while (cq < 2 * n && tb + ring_tile(cq) >= n_first) ++cq;
-            if (cq < 2 * n) {
+            if (ck == 0) {
+                while (cq < 2 * n && tb + ring_tile(cq) >= n_first) ++cq;
                 const bool v = ring_v(cq);
-                const int2 e = entry(cq, ck);
-                const uint64_t tok_bytes = v ? P.pv_tok : P.pk_tok;
-                const uint8_t* src = (v ? vbase : kbase) + uint64_t(uint32_t(e.x)) * (v ? P.pv_slot : P.pk_slot) +
-                                     uint64_t(uint32_t(e.y) & 0xFFFFFFu) * tok_bytes;
-                const uint32_t rb = v ? P.pv_bytes : P.pk_bytes, gran = v ? P.pv_gran : P.pk_gran;
+                c_ents = table + ring_tile(cq) * nb;
+                c_base = v ? vbase : kbase, c_slot = v ? P.pv_slot : P.pk_slot, c_tok = v ? P.pv_tok : P.pk_tok;
+                c_gran = v ? P.pv_gran : P.pk_gran, c_q8 = v ? vq8 : kq8;
+            }
+            if (cq < 2 * n) {
+                const int2 e = entry(c_ents, ck);
+                const uint64_t tok_bytes = c_tok;
+                const uint8_t* src = c_base + uint64_t(uint32_t(e.x)) * c_slot + uint64_t(uint32_t(e.y) & 0xFFFFFFu) * tok_bytes;
+                const uint32_t gran = c_gran;
                 const uint32_t some = uint32_t(e.y) >> 24, dst = smem_u32(stage + cs * kAcRawBytes);
                 auto rows_of = [&](auto g, auto bytes) {
                     constexpr uint32_t kG = decltype(g)::value, kPer = kBlk * decltype(bytes)::value / kG;
@@ -698,7 +707,7 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
                     }
                     rows_of(std::integral_constant<uint32_t, 4>{}, bytes);
                 };
-                if (rb == kBlk * 34) plane(std::integral_constant<uint32_t, 34>{});
+                if (c_q8) plane(std::integral_constant<uint32_t, 34>{});
                 else plane(std::integral_constant<uint32_t, 18>{});
                 cs = cs + 1 == kAcRaw ? 0 : cs + 1;
                 ck += kKeys;
@@ -725,7 +734,7 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
                     __syncwarp();
                     x.load(stage + rs * kAcRawBytes + mine * (v ? P.pv_bytes : P.pk_bytes), bi, v ? vq8 : kq8);
                     rs = rs + 1 == kAcRaw ? 0 : rs + 1;
-                    const bool live = mine < uint32_t(entry(q, k0).y) >> 24;
+                    const bool live = mine < uint32_t(entry(table + j * nb, k0).y) >> 24;
                     __syncwarp();
                     copy();
                     const uint32_t key = k0 + dw * kWarpKeys + mine, d2 = live ? x.scale2(odd) : 0u;
