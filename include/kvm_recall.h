@@ -811,8 +811,11 @@ int kvm_window_attention(kvm_ctx* ctx, const kvm_window_desc* desc, const kvm_ro
  *    (layer, KV head)) are calls with kv_heads = 1 and one sequence per head.
  *  - tail_k / tail_v: kvm_kcache views of the desc's type, layer_stride between
  *    sequences, capacity_tokens >= recent + nodes.
- *  - Block scales of quantised V above 1023 with fp16 queries are reported as
- *    KVM_ERR_NONFINITE (their products would leave the range of fp16).
+ *  - Quantised pages of a multiple of 16 tokens are decoded to fp16, code times
+ *    scale rounded once (2^-11 of the value), and a bf16 tail goes through fp16 beside
+ *    them; block scales above 511 and bf16 tail values above 65504 are reported as
+ *    KVM_ERR_NONFINITE, as they could leave its range. Other page sizes keep the codes
+ *    as integers; V scales above 1023 with fp16 queries are reported there.
  * kvm_plan_residency, the stage-in and this call are ordered by the stream;
  * KVM_ERR_PENDING while a transfer is pending on the pool. */
 typedef struct kvm_tree_desc {

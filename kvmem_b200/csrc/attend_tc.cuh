@@ -177,6 +177,11 @@ __device__ __forceinline__ uint32_t ac_to_half2(uint32_t w) {
     const __half2 h = __floats2half2_rn(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+// Whether one of two finite bf16 values lies beyond fp16's largest, 65504: from 65536 on, the next bf16 after 65280.
+__device__ __forceinline__ bool ac_over_half2(uint32_t w) {
+    const uint32_t a = w & 0x7FFFu, b = (w >> 16) & 0x7FFFu;
+    return (a >= 0x4780u && a < 0x7F80u) || (b >= 0x4780u && b < 0x7F80u);
+}
 
 template <int D, bool BF16, int MODE, bool QUANT>
 __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 : 2)
@@ -633,7 +638,8 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
         // as the rows' sizes and strides allow; a thread's loads of its own block touch 8 or more lines per
         // word, and with them a tile of head_dim 256 took 12,400 cycles), then one thread decodes
         // one block: code times scale in fp16, each product rounded once, half a step of fp16, 2^-11;
-        // reported where a scale above 511 could leave its range. Keys without a token become zeros.
+        // reported where a scale above 511 (or a bf16 value of the tail) could leave its range. Keys without
+        // a token become zeros.
         const uint32_t dw = uint32_t(warp) - 12, dt = uint32_t(tid) - 384;
         constexpr uint32_t kBlk = D / 32, kWarpKeys = 32 / kBlk, kKeys = 8 * kWarpKeys, kHalves = U > 1 ? 2 : 1;
         uint32_t freed = 0;
@@ -766,6 +772,8 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
                         const uint8_t* row = v ? P.v + uint64_t(b) * P.v_seq + uint64_t(h) * P.v_head + uint64_t(tok0 + key) * P.v_tok
                                                : P.k + uint64_t(b) * P.k_seq + uint64_t(h) * P.k_head + uint64_t(tok0 + key) * P.k_tok;
                         z = __ldg(reinterpret_cast<const uint4*>(row) + c);
+                        if constexpr (BF16)
+                            wild = wild || ac_over_half2(z.x) || ac_over_half2(z.y) || ac_over_half2(z.z) || ac_over_half2(z.w);
                         z = make_uint4(ac_to_half2<BF16>(z.x), ac_to_half2<BF16>(z.y), ac_to_half2<BF16>(z.z), ac_to_half2<BF16>(z.w));
                     }
                     *place(at, v, key, c) = z;

@@ -5,10 +5,13 @@
 // list of moves {source slot, destination slot}) and a copy that walks the lists
 // on the device, so no count is read back. A group is one source row and the rows
 // its pages go to. The copy is bound by HBM: every page is read once and written
-// once per destination. It moves 16 KiB chunks through a ring in shared memory
-// with bulk TMA copies (global -> shared, then shared -> each destination), issued
-// by one thread per CTA: no registers hold data in flight, so one warp per SM keeps
-// kPcStages chunks moving.
+// once per destination. 16 KiB chunks go through shared memory with bulk TMA copies
+// (global -> shared, then shared -> each destination); no registers hold data in
+// flight, so one CTA of kPcStages warps per SM, each with one chunk on its way, keeps
+// the memory busy. One thread for all stages spent more on finding the chunks'
+// addresses than the copies took (333 items of 512 KiB: 108 us against 61). 61 us are
+// 0.88 of the measured copy rate; a fork of 16 rows of 34 pages of 1 MiB into three
+// rows each (2.2 GB read and written) takes 380 us, 0.90.
 #pragma once
 #include "stagein.cuh"
 

@@ -311,6 +311,27 @@ def test_a_v_scale_out_of_range_is_reported(ctx):
     assert ctx.status() == K._abi.ERR_NONFINITE
 
 
+@pytest.mark.parametrize("plane", [0, 1])
+@pytest.mark.parametrize("value,err", [(65280.0, False), (65536.0, True), (-1e5, True), (float("inf"), False)])
+def test_a_bf16_tail_beside_quantised_pages_keeps_to_the_range_of_fp16(ctx, plane, value, err):
+    """65280 is bf16's last value below 65504; infinities are passed on as they are."""
+    import kvmem_b200 as K
+    p = Problem(ctx, 22, 1, 3, 4, 1, 128, 16, 4, 3, [64], [5], torch.bfloat16, kinds=(U.Q8_0, U.Q4_0))
+    p.tail_d[plane][0, 2, 0, 7] = value
+    p.call()
+    assert ctx.status() == (K._abi.ERR_NONFINITE if err else 0)
+
+
+@pytest.mark.parametrize("scale,err", [(511.0, False), (512.0, True)])
+def test_a_k_scale_out_of_range_is_reported(ctx, scale, err):
+    import kvmem_b200 as K
+    p = Problem(ctx, 23, 1, 2, 4, 1, 64, 32, 4, 3, [128], [0], torch.bfloat16, kinds=(U.Q4_0, U.Q4_0))
+    s = int(p.slot_of[0, p.lists[0][0]])
+    p.cache[0][0, s, 0, 0, :2] = torch.tensor([scale], dtype=torch.float16).view(torch.uint8)
+    p.call()
+    assert ctx.status() == (K._abi.ERR_NONFINITE if err else 0)
+
+
 def test_long_list_with_table_refills(ctx, monkeypatch):
     """Pages of 2 tokens, 1,500 of them: more entries than the kernel holds at a time."""
     monkeypatch.setenv("KVM_ATTEND_SPLITS", "1")
