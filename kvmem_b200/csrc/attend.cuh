@@ -784,36 +784,47 @@ __global__ void __launch_bounds__(256) attend_combine_kernel(const __grid_consta
         const uint32_t rows = P.seq_rows ? min(__ldg(P.seq_rows + b), P.width) : P.width;
         if (recent > P.capacity || rows > P.capacity - recent) return;
     }
-    constexpr int E = D / 32;
+    // Lane: W neighbouring dims of each 32 * W. Four chunks' loads are started before the first is used.
+    constexpr int E = D / 32, W = E < 4 ? E : 4, kAhead = 4;
     float acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
     float m = -INFINITY, l = 0.f;
-#pragma unroll 4
-    for (uint32_t c = warp; c < P.splits; c += nw) {
-        const float2 ml = P.part_ml[c * stride + row_id];
-        const float* src = P.part_o + (c * stride + row_id) * D + lane * E;
-        float x[E];
-        if constexpr (E == 2) {
-            const float2 v = *reinterpret_cast<const float2*>(src);
-            x[0] = v.x, x[1] = v.y;
-        } else {
+    for (uint32_t c0 = warp; c0 < P.splits; c0 += nw * kAhead) {
+        float2 ml[kAhead];
+        float x[kAhead][E];
 #pragma unroll
-            for (int e = 0; e < E; e += 4) {
-                const float4 v = *reinterpret_cast<const float4*>(src + e);
-                x[e] = v.x, x[e + 1] = v.y, x[e + 2] = v.z, x[e + 3] = v.w;
+        for (int i = 0; i < kAhead; ++i) {
+            const uint32_t c = c0 + i * nw;
+            ml[i] = make_float2(-INFINITY, 0.f);
+            if (c < P.splits) {
+                ml[i] = P.part_ml[c * stride + row_id];
+                const float* src = P.part_o + (c * stride + row_id) * D + lane * W;
+#pragma unroll
+                for (int e = 0; e < E; e += W) {
+                    if constexpr (W == 2) {
+                        const float2 v = *reinterpret_cast<const float2*>(src);
+                        x[i][0] = v.x, x[i][1] = v.y;
+                    } else {
+                        const float4 v = *reinterpret_cast<const float4*>(src + e * 32);
+                        x[i][e] = v.x, x[i][e + 1] = v.y, x[i][e + 2] = v.z, x[i][e + 3] = v.w;
+                    }
+                }
             }
         }
-        if (ml.y == 0.f) continue;
-        const float nm = fmaxf(m, ml.x);
-        const float a0 = m == -INFINITY ? 0.f : fast_exp2(m - nm), a1 = fast_exp2(ml.x - nm);
-        m = nm;
-        l = l * a0 + ml.y * a1;
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = acc[e] * a0 + x[e] * a1;
+        for (int i = 0; i < kAhead; ++i) {
+            if (ml[i].y == 0.f) continue;
+            const float nm = fmaxf(m, ml[i].x);
+            const float a0 = m == -INFINITY ? 0.f : fast_exp2(m - nm), a1 = fast_exp2(ml[i].x - nm);
+            m = nm;
+            l = l * a0 + ml[i].y * a1;
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = acc[e] * a0 + x[i][e] * a1;
+        }
     }
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc_s[warp][lane * E + e] = acc[e];
+    for (int e = 0; e < E; ++e) acc_s[warp][(e / W) * 32 * W + lane * W + e % W] = acc[e];
     if (lane == 0) ml_s[warp] = make_float2(m, l);
     __syncthreads();
     float mm = -INFINITY, ll = 0.f;
