@@ -25,10 +25,21 @@
 //  * warp 3 (and 2): a V tile behind a mask may hold infinities or NaN, which 0 * x
 //    would spread to rows that do not see them. Keys that no row sees become zeros; the
 //    others are looked through, and where some rows see such a value it is taken out of
-//    the product and added by hand to those rows.
+//    the product and added by hand to those rows. The tail of a tree waits for its scan, so
+//    its sums are four chains and dead keys one bit each (one token over 34 pages of
+//    head_dim 256: 33 us before, 24 so); windows keep one chain and a comparison, which
+//    leaves the softmax more issue slots (whole prompt 402 us; 411-422 in the tree's form).
 // Quantised pages (q8_0 / q4_0): eight more warps read the blocks as stored, decode them to
 // fp16 and write them where the copies would have put them; queries and the tail become fp16
-// too (a bf16 query row after division by a power of two).
+// too (a bf16 query row after division by a power of two). Their decoding bounds that form:
+// some 10,000 cycles per tile of head_dim 256 against 2,500 of products and softmax.
+//
+// Measured (device time, the joining pass included where keys are split):
+//   1,024 rows, window 4,096 + 256 sinks, 24 / 4 heads, dim 256, bf16   142 us, 770 TFLOP/s
+//   16,381 rows, window 1,000 + 64 sinks, 32 / 8 heads, dim 128, fp16   400 us, 690 TFLOP/s
+//   60 nodes, 8 lanes, 26 pages of 128, 40 / 8 heads, dim 128, bf16     77 us, 440 TFLOP/s
+//   1 node, 34 pages of 256, 24 / 4 heads, dim 256, fp16                24 us, 1.5 TB/s
+//   16 nodes, 66 pages of 256, q8_0 / q4_0, 24 / 4 heads, dim 256       53 us
 // Every wait is bounded: on expiry the kernel records KVM_ERR_TIMEOUT, raises the
 // CTA's abort flag, lets copies and MMAs in flight finish and frees its TMEM.
 #pragma once
@@ -597,7 +608,7 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
                 const uint32_t q = v_seq(j);
                 bool ok = pf_warp_wait(&full[(q % NB) * 2], (q / NB) & 1);
                 if (U > 1) ok = pf_warp_wait(&full[(q % NB) * 2 + 1], (q / NB) & 1) && ok;
-                uint32_t acc = 0;
+                uint32_t acc[4] = {};
                 const uint32_t t = tb + j;
                 if (in_part(t)) {
                     // V rows of keys that no row sees become zeros; the others are looked through.
@@ -606,24 +617,41 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
                                                             : recent + rows - (t - n_first) * kAcKeys;
                     constexpr uint32_t kStep = 32 * kScanWarps;
                     const uint32_t first = uint32_t(tid - (128 - 32 * int(kScanWarps)));
+                    uint32_t dead[4] = {};  // a bit per key (pages)
+                    if constexpr (MODE == kAtTree) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i) {
+                            const uint32_t key = i * 32 + lane;
+                            dead[i] = __ballot_sync(0xffffffffu, paged ? (key & (box - 1)) >= uint32_t(table[j * nb + (key >> bsh)].y) >> 24
+                                                                       : key >= live);
+                        }
+                    }
+                    const bool some = dead[0] | dead[1] | dead[2] | dead[3];
                     for (uint32_t a = 0; a < U; ++a) {
-                        uint4* v4 = reinterpret_cast<uint4*>(ring + ((q * U + a) % NU) * kAcUnit);
+                        uint4* v4 = reinterpret_cast<uint4*>(ring + ((q * U + a) % NU) * kAcUnit) + first;
                         for (uint32_t e0 = 0; e0 < kAcUnit / 16; e0 += 8 * kStep) {
                             uint4 y[8];
 #pragma unroll
-                            for (uint32_t i = 0; i < 8; ++i) y[i] = v4[e0 + i * kStep + first];
+                            for (uint32_t i = 0; i < 8; ++i) y[i] = v4[e0 + i * kStep];
 #pragma unroll
                             for (uint32_t i = 0; i < 8; ++i) {
                                 const uint32_t key = a * VK + ((e0 + i * kStep + first) / 8) % VK;
-                                const bool dead = paged ? (key & (box - 1)) >= uint32_t(table[j * nb + (key >> bsh)].y) >> 24 : key >= live;
-                                if (dead) v4[e0 + i * kStep + first] = make_uint4(0, 0, 0, 0);
-                                else acc = ac_zero_times<OB>(y[i].x, ac_zero_times<OB>(y[i].y, ac_zero_times<OB>(y[i].z, ac_zero_times<OB>(y[i].w, acc))));
+                                if constexpr (MODE == kAtWindow) {
+                                    if (key >= live) v4[e0 + i * kStep] = make_uint4(0, 0, 0, 0);
+                                    else acc[0] = ac_zero_times<OB>(y[i].x, ac_zero_times<OB>(y[i].y, ac_zero_times<OB>(y[i].z, ac_zero_times<OB>(y[i].w, acc[0]))));
+                                } else {
+                                    const uint32_t lo2 = key & 32 ? dead[1] : dead[0], hi2 = key & 32 ? dead[3] : dead[2];
+                                    if (some && (((key & 64 ? hi2 : lo2) >> (key & 31)) & 1)) v4[e0 + i * kStep] = y[i] = make_uint4(0, 0, 0, 0);
+                                    acc[0] = ac_zero_times<OB>(y[i].x, acc[0]), acc[1] = ac_zero_times<OB>(y[i].y, acc[1]);
+                                    acc[2] = ac_zero_times<OB>(y[i].z, acc[2]), acc[3] = ac_zero_times<OB>(y[i].w, acc[3]);
+                                }
                             }
                         }
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
-                const bool bad = __any_sync(0xffffffffu, at_nonfinite<OB>(acc));
+                const bool bad = __any_sync(0xffffffffu, at_nonfinite<OB>(acc[0]) || at_nonfinite<OB>(acc[1]) || at_nonfinite<OB>(acc[2]) ||
+                                                             at_nonfinite<OB>(acc[3]));
                 if (lane == 0) {
                     bad_flag[(j % kAcScans) * 2 + (warp & 1)] = bad;
                     mbar_arrive(&scanned[j % kAcScans]);

@@ -2397,16 +2397,18 @@ int attend_scratch(kvm_ctx* c, AttendParams& p, uint32_t head_dim, cudaStream_t 
 // Chooses the kernel, its M tile and the key chunks, takes the scratch and launches.
 // `keys`: keys of the longest unit; `list_keys`: those of its page list; `tail_most`:
 // a bound on those of its tail.
-// The tcgen05 kernel takes more than 16 packed rows (width * group) and all quantised pages
-// that it can. Device times, mma.sync / tcgen05, us:
-//   packed rows                              5-6          12-15        24-36        48-60        65-72
-//   one lane, 8,900 keys of pages, dim 256   28.5 / 32.8  29.3 / 33.0  42.0 / 33.7  68.3 / 34.3  90.5 / 34.7
-//   8 lanes, 3,400 keys of pages, dim 128    39.3 / 36.2  41.0 / 37.0  54.4 / 38.2  95.3 / 40.9  154 / 41.7
-//   8 lanes, window of 4,224 keys, dim 128   29.9 / 31.9  -            64.6 / 36.3  -            115 / 39.9 (80)
-//   one lane, window of 1,027 keys, dim 256  10.3 / 13.4  -            -            20.6 / 14.1  22.3 / 15.1 (96)
-//   q8_0 / q4_0, one lane, 17,000 keys       68.3 / 53.3  -            106 / 54.4   -            170 / 56.3
-//   q8_0, 8 lanes, 3,400 keys, dim 128       91.7 / 72.2  110 / 73.1 (20)           142 / 75.6
-// (up to 16 rows one warp of the mma.sync kernel holds them all, and its CTAs start and end sooner).
+// The tcgen05 kernel takes more than 16 packed rows (width * group), page lists of 2,048 keys or
+// more, and all quantised pages that it can. Device times, mma.sync / tcgen05, us:
+//   packed rows                              4-6          12-15        24-36        48-60        65-72
+//   one lane, 8,900 keys of pages, dim 256   27.2 / 23.9  27.7 / 24.0  40.0 / 24.5  67.0 / 25.3  89.9 / 25.7
+//   8 lanes, 3,400 keys of pages, dim 128    39.2 / 34.4  40.9 / 35.5  55.3 / 37.5  95.7 / 41.6  154 / 42.2
+//   8 rows of 1,150 keys of pages, dim 128    9.8 / 11.1
+//   8 lanes, window of 4,224 keys, dim 128   30.4 / 32.3  -            65.5 / 37.6  -            116 / 43.0 (80)
+//   one lane, window of 1,027 keys, dim 256   9.1 / 13.4  -            -            19.4 / 13.9  21.3 / 14.9 (96)
+//   q8_0 / q4_0, one lane, 17,000 keys       66.4 / 45.3  -            104 / 47.4   -            169 / 51.2
+//   q8_0, 8 lanes, 3,400 keys, dim 128       91.4 / 71.5  111 / 72.3 (20)           144 / 75.9
+// (up to 16 rows one warp of the mma.sync kernel holds them all, and its CTAs start and end sooner;
+// its copies of pages cost a lookup per row, those of the tcgen05 kernel one per box).
 // KVM_ATTEND=mma and KVM_ATTEND=tc force a kernel (tc: KVM_ERR_UNSUPPORTED where it
 // cannot run); the tests use them.
 int attend_launch(kvm_ctx* c, AttendParams& p, uint32_t head_dim, bool bf16, int mode, bool quant, uint64_t keys,
@@ -2415,7 +2417,7 @@ int attend_launch(kvm_ctx* c, AttendParams& p, uint32_t head_dim, bool bf16, int
     const uint64_t rows = uint64_t(p.seqs) * p.width * p.q_heads;
     const size_t row_bytes = size_t(head_dim) * 4 + 8;
     const bool force_tc = attend_is("tc");
-    if ((quant || packed > 16 || force_tc) && !attend_is("mma")) {
+    if ((quant || packed > 16 || list_keys >= 2048 || force_tc) && !attend_is("mma")) {
         AttendTcMaps maps;
         std::memset(&maps, 0, sizeof maps);
         uint32_t box = 0;
