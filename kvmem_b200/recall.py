@@ -43,6 +43,13 @@ def _bad(where: str, what: str, code: int = A.ERR_INVALID_ARGUMENT) -> A.KvmErro
     return A.KvmError(code, f"{where}: {what}")
 
 
+def _pack(where: str, form: struct.Struct, *values) -> bytes:
+    try:
+        return form.pack(*values)
+    except struct.error as e:  # negative, or past 32 bits
+        raise _bad(where, f"an argument is out of range ({e})") from None
+
+
 def _on_device(device: int, where: str, *tensors) -> None:
     for t in tensors:
         if t is not None and t.get_device() != device:
@@ -289,8 +296,8 @@ class RecallContext:
         out, lse, lse_p, t, (B, W, Hq, D), hkv, qq, kk, vv, oo = _attention_args(w, dev, q, k, v, out, lse, want_lse, stream)
         base, seq_base = _seq_arg(base, dev, B, w, torch.int64)
         seq_rows = 0 if rows is None else _seq_arg(rows, dev, B, w, torch.int32)[1]
-        d = _WINDOW.pack(Hq, hkv, D, t, B, W, min(window, 0xFFFFFFFF), min(sinks, 0xFFFFFFFF), base, seq_base, seq_rows,
-                         scale, 0)
+        d = _pack(w, _WINDOW, Hq, hkv, D, t, B, W, min(window, 0xFFFFFFFF), min(sinks, 0xFFFFFFFF), base, seq_base,
+                  seq_rows, scale, 0)
         rc = self.lib.kvm_window_attention(self.h, d, qq, kk, vv, oo, lse_p, _stream_on(dev, stream))
         if rc:
             A.check(rc, w)
@@ -566,21 +573,21 @@ class ResidencyPool:
         if sel_ids is not None:
             n0, width = sel_ids.shape if sel_ids.dim() == 2 else (0, 0)
             stride = sel_ids.stride(0) if n0 > 1 else width
-            if sel_n is None or n0 < R or sel_ids.element_size() != 4 or stride < width or \
+            if sel_n is None or n0 < R or sel_ids.dtype is not torch.int32 or stride < width or \
                     (width > 1 and sel_ids.stride(1) != 1) or sel_ids.get_device() != dev:
                 raise _bad(w, "sel_ids is int32 [seqs][.] on the device, with sel_n [seqs]")
             ids, ns = sel_ids.data_ptr(), _seq_arg(sel_n, dev, R, w, torch.int32)[1]
         if tree is not None:
             shape = tree.shape
-            if tree.element_size() != 4 or not tree.is_contiguous() or tree.get_device() != dev or \
+            if tree.dtype is not torch.int32 or not tree.is_contiguous() or tree.get_device() != dev or \
                     shape[:-1] not in ((N,), (R, N)):
                 raise _bad(w, "tree is contiguous int32 [nodes][words] or [seqs][nodes][words] on the device")
             words = shape[-1]
             tree_p, tree_stride = tree.data_ptr(), (N * words if len(shape) == 3 else 0)
         seq_rows = 0 if rows is None else _seq_arg(rows, dev, R, w, torch.int32)[1]
-        d = _TREE.pack(Hq, hkv, D, t, t if k_type is None else k_type, t if v_type is None else v_type, R, N, row0, row_step,
-                       page_tokens, recent, tokens, seq_tokens, seq_recent, seq_rows, ids, ns, stride, words, tree_p,
-                       tree_stride, scale, 0)
+        d = _pack(w, _TREE, Hq, hkv, D, t, t if k_type is None else k_type, t if v_type is None else v_type, R, N, row0,
+                  row_step, page_tokens, recent, tokens, seq_tokens, seq_recent, seq_rows, ids, ns, stride, words, tree_p,
+                  tree_stride, scale, 0)
         rc = self.ctx.lib.kvm_tree_attention(self.ctx.h, self.h, d, layout, qq, kk, vv, oo, lse_p, _stream_on(dev, stream))
         if rc:
             A.check(rc, w)
@@ -627,7 +634,7 @@ class ResidencyPool:
         n = len(rows)
         w = "kvm_pool_free"
         _on_device(self.ctx.device, w, ids)
-        if ids.dim() != 2 or ids.shape[0] < n or ids.element_size() != 4 or not ids.is_contiguous():
+        if ids.dim() != 2 or ids.shape[0] < n or ids.dtype is not torch.int32 or not ids.is_contiguous():
             raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{w}: ids is contiguous int32 [rows][.]")
         arr = (C.c_uint32 * max(1, n))(*rows)
         A.check(self.ctx.lib.kvm_pool_free(self.ctx.h, self.h, arr, n, ids.data_ptr(),

@@ -434,3 +434,15 @@ def test_refusals(ctx):
     t.abort()
     t.close()
     ctx.check_status()
+
+
+def test_lists_of_another_type_and_negative_rows_are_refused(ctx):
+    import kvmem_b200 as K
+    p = Problem(ctx, 26, 2, 3, 4, 2, 64, 16, 10, 4, [100, 90], [2, 2], torch.float16)
+    sel, n = p.lists_d()
+    for kw in (dict(sel_ids=sel.float(), sel_n=n), dict(row0=-1), dict(row_step=1 << 32), dict(page_tokens=-16),
+               dict(tree=torch.zeros(3, 1, device=DEV))):
+        with pytest.raises(K.KvmError) as e:
+            p.call(**kw)
+        assert e.value.code == K._abi.ERR_INVALID_ARGUMENT, kw
+    ctx.check_status()

@@ -212,3 +212,12 @@ def test_refusals(ctx):
     out, _ = ctx.window_attention(q[:, :0], k, v, base=0, window=8)
     assert out.shape[1] == 0
     ctx.check_status()
+
+
+@pytest.mark.parametrize("bad", [dict(window=-1), dict(sinks=-1), dict(window=-(1 << 40))])
+def test_negative_arguments_are_refused_as_the_librarys_errors(ctx, bad):
+    import kvmem_b200 as K
+    q, k, v = [x.to(DEV) for x in make(9, 1, 2, 4, 2, 64, 50, torch.float16)]
+    with pytest.raises(K.KvmError) as e:
+        ctx.window_attention(q, k, v, **{**dict(base=10, window=8, sinks=0), **bad})
+    assert e.value.code == K._abi.ERR_INVALID_ARGUMENT
