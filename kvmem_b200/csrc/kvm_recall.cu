@@ -2432,6 +2432,8 @@ int attend_launch(kvm_ctx* c, AttendParams& p, uint32_t head_dim, bool bf16, int
                 const uint64_t all = (list_keys + kAcKeys - 1) / kAcKeys + (tail_most + kAcKeys - 1) / kAcKeys;
                 if (all / most >= 256) too_many = true;
                 least = uint32_t(all / most + 1);
+                // A bound workspace without room for that many leaves the call to the kernel that needs none.
+                if (least > 1 && c->ws_borrowed && rows * least * row_bytes + 256 > c->ws_bytes) too_many = true;
             }
             if (!too_many) {
                 const uint64_t tiles = (keys + kAcKeys - 1) / kAcKeys + 1;

@@ -436,6 +436,18 @@ def test_refusals(ctx):
     ctx.check_status()
 
 
+def test_a_long_list_of_small_pages_with_a_small_bound_workspace():
+    """More page boxes than one key chunk of the tcgen05 kernel holds, and no room for a second chunk's rows."""
+    import kvmem_b200 as K
+    c = K.RecallContext(0)
+    c.bind_workspace(torch.empty(1024, dtype=torch.uint8, device=DEV))
+    p = Problem(c, 27, 1, 20, 2, 2, 64, 16, 700, 640, [11200], [5], torch.bfloat16)
+    p2 = [np.flatnonzero(p.slot_of[0] >= 0)]
+    out, lse = p.call(lists=p2)
+    c.check_status()
+    p.verify(out, lse, lists=p2)
+
+
 def test_lists_of_another_type_and_negative_rows_are_refused(ctx):
     import kvmem_b200 as K
     p = Problem(ctx, 26, 2, 3, 4, 2, 64, 16, 10, 4, [100, 90], [2, 2], torch.float16)
