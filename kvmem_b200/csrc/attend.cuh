@@ -779,17 +779,13 @@ __global__ void __launch_bounds__(256) attend_combine_kernel(const __grid_consta
     const uint64_t row_id = blockIdx.x, stride = uint64_t(P.seqs) * P.width * P.q_heads;
     const uint32_t qh = uint32_t(row_id % P.q_heads);
     const uint32_t i = uint32_t((row_id / P.q_heads) % P.width), b = uint32_t(row_id / P.q_heads / P.width);
-    if (P.seq_rows && i >= min(__ldg(P.seq_rows + b), P.width)) return;
-    if (P.seq_base) {  // a sequence whose rows do not fit its cache was left out
-        const uint64_t base = __ldg(reinterpret_cast<const unsigned long long*>(P.seq_base + b));
-        const uint32_t rows = P.seq_rows ? min(__ldg(P.seq_rows + b), P.width) : P.width;
-        if (base > P.capacity || rows > P.capacity - base) return;
-    }
-    if (P.seq_recent) {
-        const uint32_t recent = __ldg(P.seq_recent + b);
-        const uint32_t rows = P.seq_rows ? min(__ldg(P.seq_rows + b), P.width) : P.width;
-        if (recent > P.capacity || rows > P.capacity - recent) return;
-    }
+    const uint32_t rows = P.seq_rows ? min(__ldg(P.seq_rows + b), P.width) : P.width;
+    if (i >= rows) return;
+    // A sequence whose rows do not fit its cache was left out: its partial rows were not written. (A window has no
+    // recent tokens and a tree no base: the other's number is 0.)
+    const uint64_t base = P.seq_base ? __ldg(reinterpret_cast<const unsigned long long*>(P.seq_base + b)) : P.base;
+    const uint32_t recent = P.seq_recent ? __ldg(P.seq_recent + b) : P.recent;
+    if (base > P.capacity || rows > P.capacity - base || recent > P.capacity || rows > P.capacity - recent) return;
     // Lane: W neighbouring dims of each 32 * W. Four chunks' loads are started before the first is used.
     constexpr int E = D / 32, W = E < 4 ? E : 4, kAhead = 4;
     float acc[E];
