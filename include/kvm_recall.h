@@ -617,9 +617,12 @@ int kvm_recall_step(kvm_ctx* ctx, const kvm_step_desc* step, kvm_pool* pool, con
  *   2. kvm_shard_merge_stats: gathered [ranks][count] pairs -> global
  *      [count] {max, 1/sum}.
  *   3. kvm_shard_score_finish: local page masses normalised by the global
- *      statistics (outputs as kvm_score_pages, over local_pages). Nothing else
- *      may score on the context between steps 1 and 3 (the LSE stays in its
- *      workspace); KVM_ERR_STALE when no partial pass left one.
+ *      statistics (outputs as kvm_score_pages, over local_pages). The LSE stays
+ *      in the context's workspace, so no other call that writes there may come
+ *      between steps 1 and 3: scores, split prefill attention, and with a bound
+ *      workspace split window or tree attention. KVM_ERR_STALE when no partial
+ *      pass left one or such a call (or kvm_ctx_bind_workspace) came between;
+ *      replays of captured calls are not seen.
  *   4. kvm_shard_candidates: per score row the top-k local pages that are not
  *      keep pages (keep = GLOBAL page ids), as (score, global id) in
  *      cand_scores / cand_ids [nrows][k], padded with (-inf, 0xffffffff).
@@ -763,7 +766,9 @@ int kvm_prefill_attention(kvm_ctx* ctx, const kvm_prefill_desc* desc, const void
  *    call of a size and is kept until the context is destroyed, so a captured
  *    call stays valid; growing it inside a capture is KVM_ERR_LENGTH (make the
  *    call once before). With a bound workspace (kvm_ctx_bind_workspace) that is
- *    used instead, with as many chunks as it has room for.
+ *    used instead, with as many chunks as it has room for; a page LSE that
+ *    kvm_shard_score_partial left there is lost then (kvm_shard_score_finish:
+ *    KVM_ERR_STALE).
  * Asynchronous on `stream`. */
 
 /* Sliding window with sinks over a dense cache: row i of sequence b stands at

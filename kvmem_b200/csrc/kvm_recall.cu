@@ -97,9 +97,11 @@ int transfer_drain(kvm_transfer* t, uint64_t timeout_us);
 
 namespace {
 
+// Makes `ws` at least `bytes` for a call that is about to write to it.
 int ensure_ws(kvm_ctx* c, size_t bytes) {
+    if (bytes > c->ws_bytes && c->ws_borrowed) return KVM_ERR_LENGTH;
+    ++c->ws_writes;
     if (bytes <= c->ws_bytes) return KVM_OK;
-    if (c->ws_borrowed) return KVM_ERR_LENGTH;
     if (c->ws) {
         cudaDeviceSynchronize();
         cudaFree(c->ws);
@@ -885,6 +887,7 @@ int kvm_ctx_bind_workspace(kvm_ctx* c, void* ws, size_t bytes) {
     c->ws = ws;
     c->ws_bytes = bytes;
     c->ws_borrowed = true;
+    ++c->ws_writes;  // what the one before held is gone
     return KVM_OK;
 }
 
@@ -1999,6 +2002,7 @@ int kvm_shard_score_partial(kvm_ctx* c, const kvm_score_desc* desc, const kvm_qu
     lse_stats_kernel<<<(nrows + 7) / 8, 256, 0, s>>>(lse, nrows, local_pages, reinterpret_cast<float2*>(stats));
     ++c->launches;
     KVM_CUDA(cudaGetLastError());
+    c->ws_partial = c->ws_writes;
     return KVM_OK;
 }
 
@@ -2049,7 +2053,9 @@ int kvm_shard_score_finish(kvm_ctx* c, const kvm_score_desc* desc, uint32_t rows
     if (desc->groups != 1 && desc->groups != desc->kv_heads) return KVM_ERR_INVALID_ARGUMENT;
     kvm_score_desc local = *desc;
     local.tokens = uint64_t(local_pages) * desc->page_tokens;
-    if (lse_bytes(&local, local.layers, rows) > c->ws_bytes) return KVM_ERR_STALE;  // no partial pass ran
+    // No partial pass ran, or another call has written to the workspace since.
+    if (!c->ws_partial || c->ws_partial != c->ws_writes || lse_bytes(&local, local.layers, rows) > c->ws_bytes)
+        return KVM_ERR_STALE;
     DeviceGuard guard(c->device);
     return normalize_layers(c, &local, rows, 0, local.layers, local_pages, static_cast<const float*>(c->ws),
                             reinterpret_cast<const float2*>(global_stats), mass_rows, mass_mean,
@@ -2231,8 +2237,10 @@ bool aligned_to(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t
 // KVM_ERR_LENGTH when it would have to grow inside a capture.
 int ensure_attn_ws(kvm_ctx* c, size_t bytes, cudaStream_t s, void** out) {
     if (c->ws_borrowed) {
+        if (bytes > c->ws_bytes) return KVM_ERR_LENGTH;
+        ++c->ws_writes;
         *out = c->ws;
-        return bytes <= c->ws_bytes ? KVM_OK : KVM_ERR_LENGTH;
+        return KVM_OK;
     }
     if (bytes > c->attn_ws_bytes) {
         cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;

@@ -22,6 +22,9 @@ struct kvm_ctx {
     void* ws = nullptr;                         // scoring workspace
     size_t ws_bytes = 0;
     bool ws_borrowed = false;
+    // Calls that wrote to `ws`, counted; the count of the partial pass whose page LSE is in it (0: none).
+    uint64_t ws_writes = 0;
+    uint64_t ws_partial = 0;
     void* small = nullptr;  // device copy of short host-built tables
     size_t small_bytes = 0;
     void* aux = nullptr;  // device copy of per-call host-built tables (propagation weights)
