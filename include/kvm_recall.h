@@ -805,10 +805,11 @@ int kvm_window_attention(kvm_ctx* ctx, const kvm_window_desc* desc, const kvm_ro
  * is set in its words of `tree` (bit j%32 of word j/32; without a tree, j <= n).
  * nodes = 1 is plain decode attention over the recalled pages.
  *  - Pages: sel_ids / sel_n are device lists as kvm_select_topk writes them (one
- *    row of sel_stride per sequence; a page listed twice counts twice); NULL
- *    reads every resident page of the row. A listed page that is not resident is
- *    left out and reported as KVM_ERR_STALE, an id past the pool's pages (or a
- *    count past sel_stride) as KVM_ERR_INVALID_ARGUMENT.
+ *    row of sel_stride per sequence; a page listed twice counts twice; rows of
+ *    sel_stride 0 name no page); NULL reads every resident page of the row. A
+ *    listed page that is not resident is left out and reported as KVM_ERR_STALE,
+ *    an id past the pool's pages (or a count past sel_stride) as
+ *    KVM_ERR_INVALID_ARGUMENT.
  *  - layout: dev_base / dev_row_stride / dev_slot_stride of planes 0 (K) and 1 (V)
  *    as for kvm_stagein_pool (host fields unused). A page is token-major,
  *    [page_tokens][kv_heads] rows of its type; k_type / v_type: both the desc's

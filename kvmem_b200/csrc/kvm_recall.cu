@@ -2535,7 +2535,7 @@ int kvm_tree_attention(kvm_ctx* c, const kvm_pool* pool, const kvm_tree_desc* d,
     if (!aligned_to(d->seq_tokens, 8) || !aligned_to(d->seq_recent, 4) || !aligned_to(d->seq_rows, 4) ||
         !aligned_to(d->sel_ids, 4) || !aligned_to(d->sel_n, 4) || !aligned_to(d->tree, 4))
         return KVM_ERR_INVALID_ARGUMENT;
-    if (d->sel_ids && (!d->sel_n || !d->sel_stride)) return KVM_ERR_INVALID_ARGUMENT;
+    if (d->sel_ids && !d->sel_n) return KVM_ERR_INVALID_ARGUMENT;
     if (d->tree && (uint64_t(d->tree_words) * 32 < d->nodes ||
                     (d->tree_stride && d->tree_stride < uint64_t(d->nodes) * d->tree_words)))
         return KVM_ERR_INVALID_ARGUMENT;
@@ -2747,7 +2747,7 @@ int kvm_pool_free(kvm_ctx* c, kvm_pool* pool, const uint32_t* rows, uint32_t n, 
                   const uint32_t* counts, uint32_t stride, void* stream) try {
     KVM_TRY(pages_check(c, pool));
     if (!n) return KVM_OK;
-    if (!rows || !ids || !counts || !stride || !aligned_to(ids, 4) || !aligned_to(counts, 4)) return KVM_ERR_INVALID_ARGUMENT;
+    if (!rows || !ids || !counts || !aligned_to(ids, 4) || !aligned_to(counts, 4)) return KVM_ERR_INVALID_ARGUMENT;
     std::vector<uint8_t> seen;
     KVM_TRY(distinct_rows(pool, rows, n, &seen));
     DeviceGuard guard(c->device);

@@ -572,15 +572,16 @@ class ResidencyPool:
         ids = ns = stride = words = tree_p = tree_stride = 0
         if sel_ids is not None:
             n0, width = sel_ids.shape if sel_ids.dim() == 2 else (0, 0)
-            stride = sel_ids.stride(0) if n0 > 1 else width
+            stride = sel_ids.stride(0) if n0 > 1 and width else width
             if sel_n is None or n0 < R or sel_ids.dtype is not torch.int32 or stride < width or \
                     (width > 1 and sel_ids.stride(1) != 1) or sel_ids.get_device() != dev:
                 raise _bad(w, "sel_ids is int32 [seqs][.] on the device, with sel_n [seqs]")
-            ids, ns = sel_ids.data_ptr(), _seq_arg(sel_n, dev, R, w, torch.int32)[1]
+            ns = _seq_arg(sel_n, dev, R, w, torch.int32)[1]
+            ids = sel_ids.data_ptr() or ns  # (a table without columns has no address, and 0 means every resident page)
         if tree is not None:
             shape = tree.shape
             if tree.dtype is not torch.int32 or not tree.is_contiguous() or tree.get_device() != dev or \
-                    shape[:-1] not in ((N,), (R, N)):
+                    shape[:-1] not in ((N,), (R, N)) or shape[-1] * 32 < N:
                 raise _bad(w, "tree is contiguous int32 [nodes][words] or [seqs][nodes][words] on the device")
             words = shape[-1]
             tree_p, tree_stride = tree.data_ptr(), (N * words if len(shape) == 3 else 0)
@@ -637,8 +638,9 @@ class ResidencyPool:
         if ids.dim() != 2 or ids.shape[0] < n or ids.dtype is not torch.int32 or not ids.is_contiguous():
             raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{w}: ids is contiguous int32 [rows][.]")
         arr = (C.c_uint32 * max(1, n))(*rows)
-        A.check(self.ctx.lib.kvm_pool_free(self.ctx.h, self.h, arr, n, ids.data_ptr(),
-                                           _seq_arg(counts, self.ctx.device, n, w, torch.int32)[1], ids.shape[1],
+        n_ids = _seq_arg(counts, self.ctx.device, n, w, torch.int32)[1]
+        # (a table without columns has no address)
+        A.check(self.ctx.lib.kvm_pool_free(self.ctx.h, self.h, arr, n, ids.data_ptr() or n_ids, n_ids, ids.shape[1],
                                            _stream_on(self.ctx.device, stream)), w)
 
     def compact(self, layout: A.StageLayout, rows: Optional[Sequence[int]] = None, *, used: Optional[torch.Tensor] = None,
