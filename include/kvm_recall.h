@@ -808,7 +808,7 @@ int kvm_window_attention(kvm_ctx* ctx, const kvm_window_desc* desc, const kvm_ro
  *    row of sel_stride per sequence; a page listed twice counts twice; rows of
  *    sel_stride 0 name no page); NULL reads every resident page of the row. A
  *    listed page that is not resident is left out and reported as KVM_ERR_STALE,
- *    an id past the pool's pages (or a count past sel_stride) as
+ *    an id past the pool's pages (or a count past the row's ids) as
  *    KVM_ERR_INVALID_ARGUMENT.
  *  - layout: dev_base / dev_row_stride / dev_slot_stride of planes 0 (K) and 1 (V)
  *    as for kvm_stagein_pool (host fields unused). A page is token-major,
@@ -843,7 +843,7 @@ typedef struct kvm_tree_desc {
     const uint32_t* tree;         /* device [seqs][nodes][tree_words] or NULL: a chain */
     uint64_t tree_stride;         /* words between sequences' trees; 0: one tree for all */
     float scale;
-    uint32_t reserved;
+    uint32_t sel_width;           /* ids of a row of sel_ids, where they are the first of wider rows; 0: sel_stride */
 } kvm_tree_desc;
 int kvm_tree_attention(kvm_ctx* ctx, const kvm_pool* pool, const kvm_tree_desc* desc, const kvm_stage_layout* layout,
                        const kvm_rows* q, const kvm_kcache* tail_k, const kvm_kcache* tail_v, const kvm_rows* out,

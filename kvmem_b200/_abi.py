@@ -141,7 +141,7 @@ class TreeDesc(C.Structure):
                 ("tokens", C.c_uint64), ("seq_tokens", C.c_void_p), ("seq_recent", C.c_void_p),
                 ("seq_rows", C.c_void_p), ("sel_ids", C.c_void_p), ("sel_n", C.c_void_p), ("sel_stride", C.c_uint32),
                 ("tree_words", C.c_uint32), ("tree", C.c_void_p), ("tree_stride", C.c_uint64), ("scale", C.c_float),
-                ("reserved", C.c_uint32)]
+                ("sel_width", C.c_uint32)]
 
 
 class PageCopy(C.Structure):

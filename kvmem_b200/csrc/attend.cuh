@@ -65,7 +65,7 @@ struct AttendParams {
     const int32_t *slot_of, *page_of;
     uint32_t pool_pages, pool_slots, row0, row_step;
     const uint32_t *sel_ids, *sel_n;
-    uint32_t sel_stride, page_tokens;
+    uint32_t sel_stride, sel_width, page_tokens;
     uint64_t pt_magic;  // u / page_tokens = (u * pt_magic) >> pt_shift for u < 2^31
     uint32_t pt_shift;
     uint64_t tokens;
@@ -274,9 +274,9 @@ __global__ void __launch_bounds__(kAtThreads) attend_mma_kernel(const __grid_con
         if (P.sel_ids) {
             ids = P.sel_ids + uint64_t(b) * P.sel_stride;
             n_list = __ldg(P.sel_n + b);
-            if (n_list > P.sel_stride) {
+            if (n_list > P.sel_width) {
                 if (tid == 0) record_error(P.status, KVM_ERR_INVALID_ARGUMENT, 102);
-                n_list = P.sel_stride;
+                n_list = P.sel_width;
             }
         } else {
             n_list = P.pool_slots;

@@ -279,9 +279,9 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
         uint32_t n_list = P.pool_slots;
         if (P.sel_ids) {
             n_list = __ldg(P.sel_n + b);
-            if (n_list > P.sel_stride) {
+            if (n_list > P.sel_width) {
                 if (tid == 0) record_error(P.status, KVM_ERR_INVALID_ARGUMENT, 122);
-                n_list = P.sel_stride;
+                n_list = P.sel_width;
             }
         }
         n_keys = n_list * P.page_tokens;

@@ -2535,11 +2535,12 @@ int kvm_tree_attention(kvm_ctx* c, const kvm_pool* pool, const kvm_tree_desc* d,
     if (!aligned_to(d->seq_tokens, 8) || !aligned_to(d->seq_recent, 4) || !aligned_to(d->seq_rows, 4) ||
         !aligned_to(d->sel_ids, 4) || !aligned_to(d->sel_n, 4) || !aligned_to(d->tree, 4))
         return KVM_ERR_INVALID_ARGUMENT;
-    if (d->sel_ids && !d->sel_n) return KVM_ERR_INVALID_ARGUMENT;
+    if (d->sel_ids && (!d->sel_n || d->sel_width > d->sel_stride)) return KVM_ERR_INVALID_ARGUMENT;
     if (d->tree && (uint64_t(d->tree_words) * 32 < d->nodes ||
                     (d->tree_stride && d->tree_stride < uint64_t(d->nodes) * d->tree_words)))
         return KVM_ERR_INVALID_ARGUMENT;
-    const uint64_t list = d->sel_ids ? d->sel_stride : view.slots;
+    const uint32_t width = d->sel_width ? d->sel_width : d->sel_stride;
+    const uint64_t list = d->sel_ids ? width : view.slots;
     if (list * d->page_tokens > 0x7fffff00ull) return KVM_ERR_LENGTH;
     if (!d->seq_recent && (d->recent > p.capacity || (!d->seq_rows && d->nodes > p.capacity - d->recent))) return KVM_ERR_LENGTH;
     GatherLayout g{};
@@ -2566,7 +2567,7 @@ int kvm_tree_attention(kvm_ctx* c, const kvm_pool* pool, const kvm_tree_desc* d,
     p.slot_of = view.slot_of, p.page_of = view.page_of;
     p.pool_pages = view.pages, p.pool_slots = view.slots;
     p.row0 = d->row0, p.row_step = d->row_step;
-    p.sel_ids = d->sel_ids, p.sel_n = d->sel_n, p.sel_stride = d->sel_stride;
+    p.sel_ids = d->sel_ids, p.sel_n = d->sel_n, p.sel_stride = d->sel_stride, p.sel_width = width;
     p.page_tokens = d->page_tokens;
     division(d->page_tokens, &p.pt_magic, &p.pt_shift);
     p.tokens = d->tokens, p.seq_tokens = d->seq_tokens;

@@ -569,7 +569,7 @@ class ResidencyPool:
                                                                                  stream)
         tokens, seq_tokens = _seq_arg(tokens, dev, R, w, torch.int64)
         recent, seq_recent = _seq_arg(recent, dev, R, w, torch.int32)
-        ids = ns = stride = words = tree_p = tree_stride = 0
+        ids = ns = stride = width = words = tree_p = tree_stride = 0
         if sel_ids is not None:
             n0, width = sel_ids.shape if sel_ids.dim() == 2 else (0, 0)
             stride = sel_ids.stride(0) if n0 > 1 and width else width
@@ -588,7 +588,7 @@ class ResidencyPool:
         seq_rows = 0 if rows is None else _seq_arg(rows, dev, R, w, torch.int32)[1]
         d = _pack(w, _TREE, Hq, hkv, D, t, t if k_type is None else k_type, t if v_type is None else v_type, R, N, row0,
                   row_step, page_tokens, recent, tokens, seq_tokens, seq_recent, seq_rows, ids, ns, stride, words, tree_p,
-                  tree_stride, scale, 0)
+                  tree_stride, scale, width)
         rc = self.ctx.lib.kvm_tree_attention(self.ctx.h, self.h, d, layout, qq, kk, vv, oo, lse_p, _stream_on(dev, stream))
         if rc:
             A.check(rc, w)
