@@ -50,6 +50,12 @@ def _pack(where: str, form: struct.Struct, *values) -> bytes:
         raise _bad(where, f"an argument is out of range ({e})") from None
 
 
+def _u32s(where: str, values) -> None:
+    """ctypes takes integers modulo 2^32; here they are refused."""
+    if len(values) and (min(values) < 0 or max(values) > 0xFFFFFFFF):
+        raise _bad(where, "an argument is out of range")
+
+
 def _on_device(device: int, where: str, *tensors) -> None:
     for t in tensors:
         if t is not None and t.get_device() != device:
@@ -611,20 +617,25 @@ class ResidencyPool:
         n = len(dst_rows)
         if len(src_rows) != n:
             raise A.KvmError(A.ERR_INVALID_ARGUMENT, "kvm_pool_fork: as many sources as destinations")
+        page_end = self.pages if page_end is None else page_end
+        for x in (src_rows, dst_rows, (page_end, ctas)):
+            _u32s("kvm_pool_fork", x)
         src, dst = (C.c_uint32 * max(1, n))(*src_rows), (C.c_uint32 * max(1, n))(*dst_rows)
-        A.check(self.ctx.lib.kvm_pool_fork(self.ctx.h, self.h, C.byref(layout), src, dst, n,
-                                           self.pages if page_end is None else page_end, ctas,
+        A.check(self.ctx.lib.kvm_pool_fork(self.ctx.h, self.h, C.byref(layout), src, dst, n, page_end, ctas,
                                            _stream_on(self.ctx.device, stream)), "kvm_pool_fork")
 
     def copy_pages(self, layout: A.StageLayout, items, *, ctas: int = 0, stream=None) -> None:
         """items: (src_row, src_page, dst_row, dst_page) tuples, or a contiguous int32 CPU tensor [n][4]
         (kvm_pool_copy)."""
+        _u32s("kvm_pool_copy", (ctas,))
         if isinstance(items, torch.Tensor):
             if items.device.type != "cpu" or items.dtype != torch.int32 or items.dim() != 2 or items.shape[1] != 4 or \
                     not items.is_contiguous():
                 raise A.KvmError(A.ERR_INVALID_ARGUMENT, "kvm_pool_copy: items is a contiguous int32 CPU tensor [n][4]")
             n, ptr = items.shape[0], items.data_ptr()
         else:
+            for x in items:
+                _u32s("kvm_pool_copy", x)
             arr = (A.PageCopy * max(1, len(items)))(*[A.PageCopy(*x) for x in items])
             n, ptr = len(items), C.cast(arr, C.c_void_p)
         A.check(self.ctx.lib.kvm_pool_copy(self.ctx.h, self.h, C.byref(layout), ptr, n, ctas,
@@ -634,6 +645,7 @@ class ResidencyPool:
         """Drops the pages ids[i][: counts[i]] (int32, device) of row rows[i] (kvm_pool_free)."""
         n = len(rows)
         w = "kvm_pool_free"
+        _u32s(w, rows)
         _on_device(self.ctx.device, w, ids)
         if ids.dim() != 2 or ids.shape[0] < n or ids.dtype is not torch.int32 or not ids.is_contiguous():
             raise A.KvmError(A.ERR_INVALID_ARGUMENT, f"{w}: ids is contiguous int32 [rows][.]")
@@ -650,6 +662,8 @@ class ResidencyPool:
         rows = range(self.rows) if rows is None else rows
         n = len(rows)
         w = "kvm_pool_compact"
+        _u32s(w, rows)
+        _u32s(w, (ctas,))
         arr = (C.c_uint32 * max(1, n))(*rows)
         ptr = None if used is None else _seq_arg(used, self.ctx.device, n, w, torch.int32)[1]
         A.check(self.ctx.lib.kvm_pool_compact(self.ctx.h, self.h, C.byref(layout), arr, n, ptr, ctas,
