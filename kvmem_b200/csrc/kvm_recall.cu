@@ -10,6 +10,7 @@
 #include <vector>
 
 #include "attend_launch.cuh"
+#include "attend_plan.cuh"
 #include "attend_tc_launch.cuh"
 #include "common.cuh"
 #include "layerwise.cuh"
@@ -2431,17 +2432,13 @@ int attend_launch(kvm_ctx* c, AttendParams& p, uint32_t head_dim, bool bf16, int
         uint32_t box = 0;
         if (quant ? page_box(p.page_tokens, &box) : attend_tc_maps(p, head_dim, bf16, mode, pool_rows, &maps, &box)) {
             p.m_tiles = (packed + 127) / 128;
-            // One CTA's chunk has at most kAcTable page boxes
             uint32_t least = 1;
             bool too_many = false;
             if (mode == kAtTree) {
-                // (chunks are even shares of all tiles, the longest tail's among them).
-                const uint64_t most = uint64_t(kAcTable) * box / kAcKeys;
-                const uint64_t all = (list_keys + kAcKeys - 1) / kAcKeys + (tail_most + kAcKeys - 1) / kAcKeys;
-                if (all / most >= 256) too_many = true;
-                least = uint32_t(all / most + 1);
+                least = attend_least_chunks((list_keys + kAcKeys - 1) / kAcKeys, (tail_most + kAcKeys - 1) / kAcKeys,
+                                            uint64_t(kAcTable) * box / kAcKeys);
                 // A bound workspace without room for that many leaves the call to the kernel that needs none.
-                if (least > 1 && c->ws_borrowed && rows * least * row_bytes + 256 > c->ws_bytes) too_many = true;
+                too_many = !least || (least > 1 && c->ws_borrowed && rows * least * row_bytes + 256 > c->ws_bytes);
             }
             if (!too_many) {
                 const uint64_t tiles = (keys + kAcKeys - 1) / kAcKeys + 1;
