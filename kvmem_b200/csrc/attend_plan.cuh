@@ -15,4 +15,17 @@ inline uint32_t attend_least_chunks(uint64_t list_tiles, uint64_t tail_tiles, ui
     return all / most >= kAttendMaxSplits ? 0 : uint32_t(all / most + 1);
 }
 
+// Registers per thread that the warps of the tcgen05 kernel take (setmaxnreg). Narrow shape: 4 warps for copies and
+// MMAs, 4 of softmax. Quantised pages: 4, 8 of softmax, 8 that decode.
+constexpr int kAcNarrowIssue = 72, kAcNarrowSoftmax = 184;
+constexpr int kAcQuantIssue = 64, kAcQuantSoftmax = 136, kAcQuantDecode = 72;
+
+// Whether a kernel compiled to `regs` registers per thread can make that split: warps that ask for more than the launch
+// brought would wait for ever.
+constexpr bool ac_registers_fit(bool quant, int regs) {
+    return quant ? regs <= kAcQuantSoftmax &&
+                       640 * regs >= 128 * kAcQuantIssue + 256 * kAcQuantSoftmax + 256 * kAcQuantDecode
+                 : regs <= kAcNarrowSoftmax && 256 * regs >= 128 * kAcNarrowIssue + 128 * kAcNarrowSoftmax;
+}
+
 }  // namespace kvmb

@@ -46,6 +46,7 @@
 #include <type_traits>
 
 #include "attend.cuh"
+#include "attend_plan.cuh"
 #include "prefill_attn.cuh"
 
 namespace kvmb {
@@ -427,8 +428,8 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
     // Two CTAs per SM: registers go to the softmax warps, 4 x 32 x 72 + 4 x 32 x 184 = 256 x 128.
     // With decoding warps: 4 x 32 x 64 + 8 x 32 x 136 + 8 x 32 x 72 = 640 x 96.
     if (warp < 4) {
-        if constexpr (QUANT) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-        else if constexpr (HS == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if constexpr (QUANT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kAcQuantIssue));
+        else if constexpr (HS == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kAcNarrowIssue));
         if (QUANT && (warp == 0 || warp == 2)) {
             // (the decoding warps fill the ring)
         } else if (warp == 0 || (kScanWarps == 1 && warp == 2)) {
@@ -660,7 +661,7 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
             }
         }
     } else if (QUANT && warp >= 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kAcQuantDecode));
         // ---- decoding warps: K and V tiles in ring order, 256 threads per tile ----
         // Each warp brings the rows of 32 blocks at a time into stages of its own (16, 8 or 4 bytes per copy,
         // as the rows' sizes and strides allow; a thread's loads of its own block touch 8 or more lines per
@@ -816,8 +817,8 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
             *abort_flag = 1;
         }
     } else {
-        if constexpr (QUANT) asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
-        else if constexpr (HS == 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+        if constexpr (QUANT) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kAcQuantSoftmax));
+        else if constexpr (HS == 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kAcNarrowSoftmax));
         // ---- softmax: thread = packed row (tensor-memory lane), NK of the tile's keys ----
         // With two warps per 32 rows these exchange their maxes through shared memory, behind a
         // barrier of their own. A warp that gives up raises the abort flag and then arrives there,

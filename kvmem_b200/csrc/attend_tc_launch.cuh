@@ -1,21 +1,29 @@
 // Launcher of the tcgen05 decode-attention kernels (attend_tc.cuh), instantiated
 // per type in attend_tc_<type>.cu.
 #pragma once
+#include <atomic>
+
 #include "attend_tc.cuh"
 #include "lse_launch.cuh"
 
 namespace kvmb {
 
+// KVM_ERR_UNSUPPORTED (nothing launched): this build of the kernel cannot split its registers.
 template <int D, bool BF16, int MODE, bool QUANT>
 int launch_attend_tc_k(kvm_ctx* c, const AttendTcMaps& maps, const AttendParams& p, uint32_t box, cudaStream_t s) {
     auto fn = attend_tc_kernel<D, BF16, MODE, QUANT>;
     if constexpr (!ac_wide(D) || QUANT) {
-        // The register split needs every register of the launch: with fewer the warps would wait for more for ever.
-        static const int regs = [&] {
+        static std::atomic<int> known{0};  // registers of the compiled kernel
+        int regs = known.load(std::memory_order_relaxed);
+        if (!regs) {
             cudaFuncAttributes a{};
-            return cudaFuncGetAttributes(&a, fn) == cudaSuccess ? a.numRegs : 0;
-        }();
-        if (regs != (QUANT ? 96 : 128)) return KVM_ERR_CUDA;
+            if (cudaFuncGetAttributes(&a, fn) != cudaSuccess) {
+                cudaGetLastError();
+                return KVM_ERR_CUDA;
+            }
+            known.store(regs = a.numRegs, std::memory_order_relaxed);
+        }
+        if (!ac_registers_fit(QUANT, regs)) return KVM_ERR_UNSUPPORTED;
     }
     constexpr uint32_t smem = ac_smem_bytes(D, MODE, QUANT);
     if (smem_attr(reinterpret_cast<const void*>(fn), int(smem)) != cudaSuccess) return KVM_ERR_CUDA;

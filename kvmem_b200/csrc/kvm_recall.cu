@@ -2447,9 +2447,10 @@ int attend_launch(kvm_ctx* c, AttendParams& p, uint32_t head_dim, bool bf16, int
                 p.splits = attend_splits(c, uint64_t(p.seqs) * p.kv_heads * p.m_tiles, uint64_t(c->num_sms) * (wide ? 1 : 2),
                                          tiles, quant ? double(head_dim) / 51.2 : wide ? 1.3 : 1.8, 7.0, rows, row_bytes, least);
                 KVM_TRY(attend_scratch(c, p, head_dim, s));
-                KVM_TRY(bf16 ? launch_attend_tc_t<true>(c, maps, p, head_dim, mode, quant, box, s)
-                             : launch_attend_tc_t<false>(c, maps, p, head_dim, mode, quant, box, s));
-                return launch_attend_combine(c, p, head_dim, bf16, s);
+                const int rc = bf16 ? launch_attend_tc_t<true>(c, maps, p, head_dim, mode, quant, box, s)
+                                    : launch_attend_tc_t<false>(c, maps, p, head_dim, mode, quant, box, s);
+                if (rc == KVM_OK) return launch_attend_combine(c, p, head_dim, bf16, s);
+                if (rc != KVM_ERR_UNSUPPORTED) return rc;
             }
         }
     }

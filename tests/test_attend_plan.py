@@ -35,3 +35,12 @@ def test_chunks_of_lists_and_tails(tmp_path, box):
                 for x, y in ((a, b), (a, 0), (a - 1, b), (most + 1, b)):
                     t = x + y
                     assert max(min(t * (c + 1) // n, x) - min(t * c // n, x) for c in range(n)) <= most
+
+
+def test_registers_that_the_split_needs(tmp_path):
+    """640 x 96 = 128 x 64 + 256 x 136 + 256 x 72; 256 x 128 = 128 x 72 + 128 x 184. A kernel compiled to fewer cannot make
+    the split (the launcher takes the other kernel then)."""
+    quant = run(tmp_path, 'for (int r = 0; r <= 255; ++r) printf("%d\\n", ac_registers_fit(true, r));')
+    narrow = run(tmp_path, 'for (int r = 0; r <= 255; ++r) printf("%d\\n", ac_registers_fit(false, r));')
+    assert [r for r in range(256) if quant[r] == "1"] == list(range(96, 137))
+    assert [r for r in range(256) if narrow[r] == "1"] == list(range(128, 185))
