@@ -818,10 +818,12 @@ int kvm_window_attention(kvm_ctx* ctx, const kvm_window_desc* desc, const kvm_ro
  *  - tail_k / tail_v: kvm_kcache views of the desc's type, layer_stride between
  *    sequences, capacity_tokens >= recent + nodes.
  *  - Quantised pages of a multiple of 16 tokens are decoded to fp16, code times
- *    scale rounded once (2^-11 of the value), and a bf16 tail goes through fp16 beside
- *    them; block scales above 511 and bf16 tail values above 65504 are reported as
- *    KVM_ERR_NONFINITE, as they could leave its range. Other page sizes keep the codes
- *    as integers; V scales above 1023 with fp16 queries are reported there.
+ *    scale rounded once (2^-11 of the value). bf16 rows of q and tail_k become
+ *    fp16 beside them after division by a power of two per row (exact for
+ *    values down to 2^-30 of the row's largest, off by 2^-38 of it below); tail_v stays bf16.
+ *    Block scales above 511 and bf16 tail values above 65504 are reported as
+ *    KVM_ERR_NONFINITE. Other page sizes keep the codes as integers; V scales
+ *    above 1023 with fp16 queries are reported there.
  * kvm_plan_residency, the stage-in and this call are ordered by the stream;
  * KVM_ERR_PENDING while a transfer is pending on the pool. */
 typedef struct kvm_tree_desc {

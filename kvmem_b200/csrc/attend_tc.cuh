@@ -30,8 +30,9 @@
 //    head_dim 256: 33 us before, 24 so); windows keep one chain and a comparison, which
 //    leaves the softmax more issue slots (whole prompt 402 us; 411-422 in the tree's form).
 // Quantised pages (q8_0 / q4_0): eight more warps read the blocks as stored, decode them to
-// fp16 and write them where the copies would have put them; queries and the tail become fp16
-// too (a bf16 query row after division by a power of two). Their decoding bounds that form:
+// fp16 and write them where the copies would have put them. Beside them bf16 queries and keys of
+// the tail become fp16, each row after division by a power of two of its own; the tail's values
+// stay bf16 (a product of its own type on the same accumulator). The decoding bounds that form:
 // some 10,000 cycles per tile of head_dim 256 against 2,500 of products and softmax.
 //
 // Measured (device time, the joining pass included where keys are split):
@@ -58,6 +59,7 @@ constexpr uint32_t kAcScans = 8;         // V tiles that the scan's barriers tel
 constexpr uint32_t kAcMaxTiles = 8;
 constexpr uint32_t kAcRaw = 3;           // quantised pages: stages of 32 blocks on their way to a decoding warp
 constexpr uint32_t kAcRawBytes = 32 * 34;
+constexpr uint32_t kAcScales = 8;        // tail tiles whose key scales are held (K runs at most four tiles ahead of the softmax)
 
 // Two shapes. Wide (head_dim 256): one CTA per SM, two S accumulators, eight softmax
 // warps, a deep ring. Narrow (64, 128): two CTAs per SM, each with one S accumulator and
@@ -77,7 +79,7 @@ __host__ __device__ constexpr uint32_t ac_tiles(int D, int mode, bool quant) {
 }
 __host__ __device__ constexpr uint32_t ac_smem_bytes(int D, int mode, bool quant) {
     return 128u * uint32_t(D) * 2u + ac_units(D, mode, quant) * kAcUnit + (ac_wide(D) || quant ? 2048u : 0u) +
-           (quant ? 512u + 8u * kAcRaw * kAcRawBytes : 0u) + (mode == kAtTree ? kAcTable * 8u : 0u) + 544u;
+           (quant ? 512u + kAcScales * 128u + 8u * kAcRaw * kAcRawBytes : 0u) + (mode == kAtTree ? kAcTable * 8u : 0u) + 544u;
 }
 static_assert(ac_smem_bytes(256, kAtTree, true) <= 227 * 1024 && ac_smem_bytes(256, kAtWindow, false) <= 227 * 1024, "shared memory");
 static_assert(ac_smem_bytes(128, kAtTree, false) <= 113 * 1024 && ac_smem_bytes(64, kAtTree, false) <= 113 * 1024, "shared memory");
@@ -182,14 +184,14 @@ __device__ __forceinline__ uint4 ac_decode_q4(const AcBlock& x, int c, bool odd,
                       ac_mul2(at_codes4<false>(__byte_perm(b, 0, 0x4140)), d2), ac_mul2(at_codes4<false>(__byte_perm(b, 0, 0x4342)), d2));
 }
 
-// Two 16-bit values of the tensors' type as fp16 (a bf16 value past fp16's range gives an infinity).
-template <bool BF16>
-__device__ __forceinline__ uint32_t ac_to_half2(uint32_t w) {
-    if constexpr (!BF16) return w;
-    const __half2 h = __floats2half2_rn(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-    return *reinterpret_cast<const uint32_t*>(&h);
+// Exponent of the power of two by which a bf16 row is divided before it becomes fp16: it brings the row's largest value
+// `top` to [2^13, 2^14). bf16 numbers down to 2^-30 of it are exact then, smaller ones off by at most 2^-38 of it.
+__device__ __forceinline__ int ac_row_exponent(float top) {
+    const int ex = int((__float_as_uint(top) >> 23) & 255) - 127 - 13;
+    return top > 0.f ? min(max(ex, -120), 114) : 0;
 }
-// Whether one of two finite bf16 values lies beyond fp16's largest, 65504: from 65536 on, the next bf16 after 65280.
+// Whether one of two finite bf16 values lies beyond fp16's largest, 65504: from 65536 on, the next bf16 after 65280
+// (the limit that the call sets for a tail beside quantised pages).
 __device__ __forceinline__ bool ac_over_half2(uint32_t w) {
     const uint32_t a = w & 0x7FFFu, b = (w >> 16) & 0x7FFFu;
     return (a >= 0x4780u && a < 0x7F80u) || (b >= 0x4780u && b < 0x7F80u);
@@ -201,6 +203,9 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
                      const uint32_t box) {
     constexpr bool kWide = ac_wide(D) || QUANT;
     constexpr bool OB = BF16 && !QUANT;          // operands of the products in bf16 (decoded pages are fp16)
+    // The values of a bf16 tail beside decoded pages stay bf16 (fp16 would lose those below 2^-17), and its P is the sum
+    // of two bf16 numbers, 2^-16 of it or less left over: no more is lost than with the fp16 P of the pages.
+    constexpr bool kTail16 = BF16 && QUANT;
     constexpr int HS = kWide ? 2 : 1;            // softmax warps per 32 rows
     constexpr uint32_t SB = kWide ? 2 : 1;       // S accumulators
     constexpr uint32_t kScanWarps = kWide ? 1 : 2;
@@ -218,7 +223,9 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
     uint8_t* ring = qsm + kQTile;
     float* pair_max = reinterpret_cast<float*>(ring + NU * kAcUnit);  // HS = 2: [2 (tile parity)][2 (half)][128]
     float* row_scale = pair_max + (HS == 2 ? 512 : 0);  // QUANT: [128] what the query rows were divided by
-    uint8_t* raw = reinterpret_cast<uint8_t*>(row_scale + (QUANT ? 128 : 0));  // QUANT: [8 warps][kAcRaw] blocks
+    // QUANT, bf16: [kAcScales][128] what the tail's K rows were divided by, 2^(x - 127)
+    uint8_t* key_scale = reinterpret_cast<uint8_t*>(row_scale + (QUANT ? 128 : 0));
+    uint8_t* raw = key_scale + (QUANT ? kAcScales * 128 : 0);  // QUANT: [8 warps][kAcRaw] blocks
     int2* table = reinterpret_cast<int2*>(raw + (QUANT ? 8 * kAcRaw * kAcRawBytes : 0));
     uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(table) + (MODE == kAtTree ? kAcTable * 8 : 0));
     uint64_t* full = bars;                    // [NB][2] half of the tile's units loaded (its one unit: [0])
@@ -228,10 +235,11 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
     uint64_t* fin = p_full + 4;
     uint64_t* together = p_full + 5;        // all softmax threads (a barrier whose wait is bounded)
     uint64_t* scanned = p_full + 6;         // [kAcScans] V tile looked through
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scanned + kAcScans);
+    uint64_t* scaled = scanned + kAcScans;  // [kAcScales] scales of a tail tile's keys are there
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scaled + kAcScales);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile uint32_t* bad_flag = tmem_slot + 2;  // [kAcScans][2] what the scanning warps found
-    static_assert((3 * kAcMaxTiles + 6 + kAcScans) * 8 + 8 + kAcScans * 8 <= 544, "barriers");
+    static_assert((3 * kAcMaxTiles + 6 + kAcScans + kAcScales) * 8 + 8 + kAcScans * 8 <= 544, "barriers");
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (smem_u32(ac_smem) & 1023u) {
@@ -335,6 +343,8 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
             mbar_init(&done[i], 1);
         }
         for (uint32_t i = 0; i < kAcScans; ++i) mbar_init(&scanned[i], kScanWarps);
+        if (QUANT)
+            for (uint32_t i = 0; i < kAcScales; ++i) mbar_init(&scaled[i], 8);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&p_full[i], 128);
             mbar_init(&p_half[i], 128);
@@ -369,7 +379,7 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
                 // (rows past the last hold copies of it: computed and not written)
                 const uint32_t row = base_row + (it + k) * kRows;
                 if constexpr (QUANT && BF16) {
-                    // As fp16, divided by a power of two that brings the row's largest value to [2^13, 2^14).
+                    // As fp16, divided by a power of two.
                     float v[8], top = 0.f;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -380,8 +390,7 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
                     }
 #pragma unroll
                     for (uint32_t o = kLanes / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    int ex = int((__float_as_uint(top) >> 23) & 255) - 127 - 13;
-                    ex = top > 0.f ? min(max(ex, -120), 114) : 0;
+                    const int ex = ac_row_exponent(top);
                     const float inv = __uint_as_float(uint32_t(127 - ex) << 23);
                     __half2 hv[4];
 #pragma unroll
@@ -521,7 +530,8 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
             // ---- MMA issue: tile j, S accumulator j % SB ----
             // The warp only adds constants to descriptors and ring positions.
             constexpr uint32_t idesc_s = pf_idesc(128, kAcKeys, OB, false);
-            constexpr uint32_t idesc_o = pf_idesc(128, D, OB, true);
+            constexpr uint32_t idesc_o = pf_idesc(128, D, OB, true), idesc_tail = pf_idesc(128, D, true, true);
+            const uint32_t page_steps = kTail16 ? __shfl_sync(0xffffffffu, tb < n_first ? n_first - tb : 0, 0) : 0;
             const uint64_t qdesc = tc_desc_sw128(smem_u32(qsm)), kdesc = tc_desc_sw128(smem_u32(ring));
             const uint64_t vdesc = pf_desc_mn_sw128(smem_u32(ring), VK * 128);
             const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), steps = __shfl_sync(0xffffffffu, n, 0);
@@ -583,8 +593,11 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
                             if (!pf_warp_wait(&p_half[slot], ph)) err = 136;
                             tc_fence_after();
                         }
-                        ac_mma_ts(tm + kColO, tm + slot * 128 + (a * (VK / 16) + kk) * 8, vd + kk * (2048 >> 4), idesc_o,
-                                  j > 0 || (a | kk) != 0);
+                        const bool tail = kTail16 && j >= page_steps;
+                        ac_mma_ts(tm + kColO, tm + slot * 128 + (a * (VK / 16) + kk) * 8, vd + kk * (2048 >> 4),
+                                  tail ? idesc_tail : idesc_o, j > 0 || (a | kk) != 0);
+                        if (tail)
+                            ac_mma_ts(tm + kColO, tm + slot * 128 + 64 + (a * (VK / 16) + kk) * 8, vd + kk * (2048 >> 4), idesc_tail, 1);
                     }
                     vp.unit();
                 }
@@ -609,9 +622,11 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
                 const uint32_t q = v_seq(j);
                 bool ok = pf_warp_wait(&full[(q % NB) * 2], (q / NB) & 1);
                 if (U > 1) ok = pf_warp_wait(&full[(q % NB) * 2 + 1], (q / NB) & 1) && ok;
-                uint32_t acc[4] = {};
                 const uint32_t t = tb + j;
-                if (in_part(t)) {
+                bool found = false;
+                auto scan = [&](auto as_bf16) {  // (in the type of the tile's values)
+                    constexpr bool B = decltype(as_bf16)::value;
+                    uint32_t acc[4] = {};
                     // V rows of keys that no row sees become zeros; the others are looked through.
                     const bool paged = MODE == kAtTree && t < n_first;
                     const uint32_t live = MODE == kAtWindow ? (t < n_first ? few - t * kAcKeys : hi - lo - (t - n_first) * kAcKeys)
@@ -639,20 +654,24 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
                                 const uint32_t key = a * VK + ((e0 + i * kStep + first) / 8) % VK;
                                 if constexpr (MODE == kAtWindow) {
                                     if (key >= live) v4[e0 + i * kStep] = make_uint4(0, 0, 0, 0);
-                                    else acc[0] = ac_zero_times<OB>(y[i].x, ac_zero_times<OB>(y[i].y, ac_zero_times<OB>(y[i].z, ac_zero_times<OB>(y[i].w, acc[0]))));
+                                    else acc[0] = ac_zero_times<B>(y[i].x, ac_zero_times<B>(y[i].y, ac_zero_times<B>(y[i].z, ac_zero_times<B>(y[i].w, acc[0]))));
                                 } else {
                                     const uint32_t lo2 = key & 32 ? dead[1] : dead[0], hi2 = key & 32 ? dead[3] : dead[2];
                                     if (some && (((key & 64 ? hi2 : lo2) >> (key & 31)) & 1)) v4[e0 + i * kStep] = y[i] = make_uint4(0, 0, 0, 0);
-                                    acc[0] = ac_zero_times<OB>(y[i].x, acc[0]), acc[1] = ac_zero_times<OB>(y[i].y, acc[1]);
-                                    acc[2] = ac_zero_times<OB>(y[i].z, acc[2]), acc[3] = ac_zero_times<OB>(y[i].w, acc[3]);
+                                    acc[0] = ac_zero_times<B>(y[i].x, acc[0]), acc[1] = ac_zero_times<B>(y[i].y, acc[1]);
+                                    acc[2] = ac_zero_times<B>(y[i].z, acc[2]), acc[3] = ac_zero_times<B>(y[i].w, acc[3]);
                                 }
                             }
                         }
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    found = at_nonfinite<B>(acc[0]) || at_nonfinite<B>(acc[1]) || at_nonfinite<B>(acc[2]) || at_nonfinite<B>(acc[3]);
+                };
+                if (in_part(t)) {
+                    if (kTail16 && t >= n_first) scan(std::true_type{});
+                    else scan(std::bool_constant<OB>{});
                 }
-                const bool bad = __any_sync(0xffffffffu, at_nonfinite<OB>(acc[0]) || at_nonfinite<OB>(acc[1]) || at_nonfinite<OB>(acc[2]) ||
-                                                             at_nonfinite<OB>(acc[3]));
+                const bool bad = __any_sync(0xffffffffu, found);
                 if (lane == 0) {
                     bad_flag[(j % kAcScans) * 2 + (warp & 1)] = bad;
                     mbar_arrive(&scanned[j % kAcScans]);
@@ -667,8 +686,7 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
         // as the rows' sizes and strides allow; a thread's loads of its own block touch 8 or more lines per
         // word, and with them a tile of head_dim 256 took 12,400 cycles), then one thread decodes
         // one block: code times scale in fp16, each product rounded once, half a step of fp16, 2^-11;
-        // reported where a scale above 511 (or a bf16 value of the tail) could leave its range. Keys without
-        // a token become zeros.
+        // reported where a scale above 511 could leave its range. Keys without a token become zeros.
         const uint32_t dw = uint32_t(warp) - 12, dt = uint32_t(tid) - 384;
         constexpr uint32_t kBlk = D / 32, kWarpKeys = 32 / kBlk, kKeys = 8 * kWarpKeys, kHalves = U > 1 ? 2 : 1;
         uint32_t freed = 0;
@@ -803,9 +821,30 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
                         z = __ldg(reinterpret_cast<const uint4*>(row) + c);
                         if constexpr (BF16)
                             wild = wild || ac_over_half2(z.x) || ac_over_half2(z.y) || ac_over_half2(z.z) || ac_over_half2(z.w);
-                        z = make_uint4(ac_to_half2<BF16>(z.x), ac_to_half2<BF16>(z.y), ac_to_half2<BF16>(z.z), ac_to_half2<BF16>(z.w));
+                    }
+                    if constexpr (BF16) {
+                        if (!v) {  // K rows as fp16, divided by a power of two as the query rows are
+                            float f[8], top = 0.f;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float2 two = at_unpack<BF16>(i == 0 ? z.x : i == 1 ? z.y : i == 2 ? z.z : z.w);
+                                f[2 * i] = two.x, f[2 * i + 1] = two.y;
+                                top = fmaxf(top, fmaxf(fabsf(two.x), fabsf(two.y)));
+                            }
+#pragma unroll
+                            for (uint32_t o = kCh / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                            const int ex = ac_row_exponent(top);
+                            const float inv = __uint_as_float(uint32_t(127 - ex) << 23);
+                            z = make_uint4(pf_pack2<false>(f[0] * inv, f[1] * inv), pf_pack2<false>(f[2] * inv, f[3] * inv),
+                                           pf_pack2<false>(f[4] * inv, f[5] * inv), pf_pack2<false>(f[6] * inv, f[7] * inv));
+                            if (c == 0) key_scale[((t - max(tb, n_first)) % kAcScales) * 128 + key] = uint8_t(127 + ex);
+                        }
                     }
                     *place(at, v, key, c) = z;
+                }
+                if (kTail16 && !v) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&scaled[(t - max(tb, n_first)) % kAcScales]);
                 }
                 for (uint32_t hf = 0; hf < kHalves; ++hf) done_half(q, hf);
             }
@@ -901,6 +940,22 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
 #pragma unroll
                 for (int q = 0; q < NW; ++q) tc_wait_ld(u + q * 32);
             }
+            const bool tail = kTail16 && t >= n_first;
+            if (tail) {  // the powers of two that the keys were divided by
+                const uint32_t jt = t - max(tb, n_first);
+                ok = pf_warp_wait(&scaled[jt % kAcScales], (jt / kAcScales) & 1);
+                if (!ok) break;
+                const uint4* ks = reinterpret_cast<const uint4*>(key_scale + (jt % kAcScales) * 128 + half * NK);
+#pragma unroll
+                for (int k = 0; k < NK; k += 16) {
+                    const uint4 w = ks[k / 16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const uint32_t u = i < 4 ? w.x : i < 8 ? w.y : i < 12 ? w.z : w.w;
+                        x[k + i] *= __uint_as_float(((u >> (i % 4 * 8)) & 255u) << 23);
+                    }
+                }
+            }
             if (part) {
 #pragma unroll
                 for (int k = 0; k < NK; ++k)
@@ -959,6 +1014,18 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
             };
             auto store = [&](int from, uint32_t part64) {
                 uint32_t pk[32];
+                if (tail) {  // P = hi + lo, lo in the other half of the columns that S has left
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) pk[i] = pf_pack2<true>(x[from + 2 * i], x[from + 2 * i + 1]);
+                    tc_st32(lane_addr + slot * 128 + part64 * 32, pk);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const float2 hi = at_unpack<true>(pk[i]);
+                        pk[i] = pf_pack2<true>(x[from + 2 * i] - hi.x, x[from + 2 * i + 1] - hi.y);
+                    }
+                    tc_st32(lane_addr + slot * 128 + 64 + part64 * 32, pk);
+                    return;
+                }
 #pragma unroll
                 for (int i = 0; i < 32; ++i) pk[i] = pf_pack2<OB>(x[from + 2 * i], x[from + 2 * i + 1]);
                 tc_st32(lane_addr + slot * 128 + part64 * 32, pk);
@@ -995,6 +1062,7 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
 #pragma unroll
                 for (int q = 0; q < NW; ++q) sl[q] = see[q];
                 const uint32_t at = v_seq(j) * U;
+                auto nonfinite = [&](uint32_t bits) { return tail ? at_nonfinite<true>(bits) : at_nonfinite<OB>(bits); };
 #pragma unroll 1
                 for (uint32_t d = 0; d < D; ++d) {
                     float f = 0.f;
@@ -1004,7 +1072,8 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
                         const uint16_t bits = *reinterpret_cast<const uint16_t*>(
                             ring + ((at + key / VK) % NU) * kAcUnit + (d / 64) * VK * 128 + kr * 128 +
                             ((((d % 64) / 8) ^ (kr & 7)) << 4) + (d % 8) * 2);
-                        if (at_nonfinite<OB>(bits) && ((sl[k >> 5] >> (k & 31)) & 1)) f += pl[k] * at_unpack<OB>(bits).x;
+                        if (nonfinite(bits) && ((sl[k >> 5] >> (k & 31)) & 1))
+                            f += pl[k] * (tail ? at_unpack<true>(bits).x : at_unpack<OB>(bits).x);
                     }
                     fix[d] = f;
                 }
@@ -1012,7 +1081,7 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
                 for (uint32_t a = 0; a < U; ++a) {
                     uint16_t* v2 = reinterpret_cast<uint16_t*>(ring + ((at + a) % NU) * kAcUnit);
                     for (uint32_t e = uint32_t(tid - 128); e < kAcUnit / 2; e += 128 * HS)
-                        if (at_nonfinite<OB>(v2[e])) v2[e] = 0;
+                        if (nonfinite(v2[e])) v2[e] = 0;
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 meet();
