@@ -143,11 +143,12 @@ class RecallContext:
         h = C.c_void_p()
         A.check(self.lib.kvm_ctx_create(device, C.byref(h)), "kvm_ctx_create")
         self.h = h
+        self._workspace: Optional[torch.Tensor] = None
 
     def close(self) -> None:
         if getattr(self, "h", None):
             self.lib.kvm_ctx_destroy(self.h)
-            self.h = None
+            self.h = self._workspace = None
 
     def __del__(self):
         try:
@@ -167,8 +168,10 @@ class RecallContext:
         return int(self.lib.kvm_ctx_launches(self.h))
 
     def bind_workspace(self, tensor: torch.Tensor) -> None:
+        """The context's scratch from now on; held until another one is bound or the context is closed."""
         A.check(self.lib.kvm_ctx_bind_workspace(self.h, tensor.data_ptr(), tensor.numel() * tensor.element_size()),
                 "kvm_ctx_bind_workspace")
+        self._workspace = tensor
 
     def device_bytes(self) -> int:
         return int(self.lib.kvm_ctx_device_bytes(self.h))
