@@ -758,7 +758,8 @@ int kvm_prefill_attention(kvm_ctx* ctx, const kvm_prefill_desc* desc, const void
  *  - Arrays marked "device" may be rewritten between replays of a captured call:
  *    grids depend on host values only. Values out of range in them are reported
  *    by kvm_ctx_status: the affected sequence's rows are left as they were
- *    (KVM_ERR_LENGTH), or the page is left out (below).
+ *    (KVM_ERR_LENGTH; also where seq_rows[i] is more than the batch's rows), or
+ *    the page is left out (below).
  *  - Rows at or past seq_rows[i] are left as they were.
  *  - Split key ranges are joined in device scratch of the context: calls on one
  *    context are ordered by their stream, and calls that may overlap (two streams,

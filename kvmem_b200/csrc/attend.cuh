@@ -231,7 +231,11 @@ __global__ void __launch_bounds__(kAtThreads) attend_mma_kernel(const __grid_con
     u /= P.splits;
     const uint32_t h = u % P.kv_heads, b = u / P.kv_heads;
     const uint32_t G = P.group;
-    const uint32_t rows = P.seq_rows ? min(__ldg(P.seq_rows + b), P.width) : P.width;
+    const uint32_t rows = P.seq_rows ? __ldg(P.seq_rows + b) : P.width;
+    if (rows > P.width) {
+        if (tid == 0) record_error(P.status, KVM_ERR_LENGTH, 106);
+        return;
+    }
     const uint32_t m0 = mt * M, m_end = rows * G;  // packed rows [m0, min(m0 + M, m_end))
     if (m0 >= m_end) return;
     const uint32_t i0 = m0 / G, i1 = min(m0 + M - 1, m_end - 1) / G;  // rows of this M tile
@@ -779,10 +783,10 @@ __global__ void __launch_bounds__(256) attend_combine_kernel(const __grid_consta
     const uint64_t row_id = blockIdx.x, stride = uint64_t(P.seqs) * P.width * P.q_heads;
     const uint32_t qh = uint32_t(row_id % P.q_heads);
     const uint32_t i = uint32_t((row_id / P.q_heads) % P.width), b = uint32_t(row_id / P.q_heads / P.width);
-    const uint32_t rows = P.seq_rows ? min(__ldg(P.seq_rows + b), P.width) : P.width;
-    if (i >= rows) return;
-    // A sequence whose rows do not fit its cache was left out: its partial rows were not written. (A window has no
-    // recent tokens and a tree no base: the other's number is 0.)
+    const uint32_t rows = P.seq_rows ? __ldg(P.seq_rows + b) : P.width;
+    if (i >= rows || rows > P.width) return;
+    // A sequence of more rows than the batch has, or than fit its cache, was left out: its partial rows were not
+    // written. (A window has no recent tokens and a tree no base: the other's number is 0.)
     const uint64_t base = P.seq_base ? __ldg(reinterpret_cast<const unsigned long long*>(P.seq_base + b)) : P.base;
     const uint32_t recent = P.seq_recent ? __ldg(P.seq_recent + b) : P.recent;
     if (base > P.capacity || rows > P.capacity - base || recent > P.capacity || rows > P.capacity - recent) return;

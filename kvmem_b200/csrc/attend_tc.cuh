@@ -253,7 +253,11 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
     un /= P.splits;
     const uint32_t h = un % P.kv_heads, b = un / P.kv_heads;
     const uint32_t G = P.group;
-    const uint32_t rows = P.seq_rows ? min(__ldg(P.seq_rows + b), P.width) : P.width;
+    const uint32_t rows = P.seq_rows ? __ldg(P.seq_rows + b) : P.width;
+    if (rows > P.width) {
+        if (tid == 0) record_error(P.status, KVM_ERR_LENGTH, 118);
+        return;
+    }
     const uint32_t m0 = mt * 128, m_end = rows * G;
     if (m0 >= m_end) return;
     auto row_div = [&](uint32_t m) { return uint32_t((uint64_t(m) * P.g_magic) >> P.g_shift); };
@@ -628,7 +632,7 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
                     constexpr bool B = decltype(as_bf16)::value;
                     uint32_t acc[4] = {};
                     // V rows of keys that no row sees become zeros; the others are looked through.
-                    const bool paged = MODE == kAtTree && t < n_first;
+                    [[maybe_unused]] const bool paged = MODE == kAtTree && t < n_first;
                     const uint32_t live = MODE == kAtWindow ? (t < n_first ? few - t * kAcKeys : hi - lo - (t - n_first) * kAcKeys)
                                                             : recent + rows - (t - n_first) * kAcKeys;
                     constexpr uint32_t kStep = 32 * kScanWarps;
@@ -642,7 +646,7 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
                                                                        : key >= live);
                         }
                     }
-                    const bool some = dead[0] | dead[1] | dead[2] | dead[3];
+                    [[maybe_unused]] const bool some = dead[0] | dead[1] | dead[2] | dead[3];
                     for (uint32_t a = 0; a < U; ++a) {
                         uint4* v4 = reinterpret_cast<uint4*>(ring + ((q * U + a) % NU) * kAcUnit) + first;
                         for (uint32_t e0 = 0; e0 < kAcUnit / 16; e0 += 8 * kStep) {
