@@ -188,7 +188,7 @@ __device__ __forceinline__ uint4 ac_decode_q4(const AcBlock& x, int c, bool odd,
 // `top` to [2^13, 2^14). bf16 numbers down to 2^-30 of it are exact then, smaller ones off by at most 2^-38 of it.
 __device__ __forceinline__ int ac_row_exponent(float top) {
     const int ex = int((__float_as_uint(top) >> 23) & 255) - 127 - 13;
-    return top > 0.f ? min(max(ex, -120), 114) : 0;
+    return top == 0.f ? 0 : min(max(ex, -120), 114);  // (a NaN or an infinity: the row's products are that anyway)
 }
 // Whether one of two finite bf16 values lies beyond fp16's largest, 65504: from 65536 on, the next bf16 after 65280
 // (the limit that the call sets for a tail beside quantised pages).
@@ -814,37 +814,43 @@ __global__ void __launch_bounds__(ac_threads(D, QUANT), ac_wide(D) || QUANT ? 1 
             } else {
                 // The tail's 16-bit rows.
                 const uint32_t tok0 = (t - n_first) * kAcKeys, most = recent + rows;
-                constexpr uint32_t kCh = D / 8;
-#pragma unroll 4
-                for (uint32_t e = dt; e < 128 * kCh; e += 256) {
-                    const uint32_t key = e / kCh, c = e % kCh;
-                    uint4 z = make_uint4(0, 0, 0, 0);
-                    if (tok0 + key < most) {
-                        const uint8_t* row = v ? P.v + uint64_t(b) * P.v_seq + uint64_t(h) * P.v_head + uint64_t(tok0 + key) * P.v_tok
-                                               : P.k + uint64_t(b) * P.k_seq + uint64_t(h) * P.k_head + uint64_t(tok0 + key) * P.k_tok;
-                        z = __ldg(reinterpret_cast<const uint4*>(row) + c);
-                        if constexpr (BF16)
-                            wild = wild || ac_over_half2(z.x) || ac_over_half2(z.y) || ac_over_half2(z.z) || ac_over_half2(z.w);
-                    }
-                    if constexpr (BF16) {
-                        if (!v) {  // K rows as fp16, divided by a power of two as the query rows are
-                            float f[8], top = 0.f;
+                // A row by kCh lanes; kBatch rows' loads are started before the first is used.
+                constexpr uint32_t kCh = D / 8, kIts = 128 * kCh / 256, kBatch = kIts < 8 ? kIts : 8;
+                const uint32_t c = uint32_t(lane) % kCh;
+                const uint8_t* head = v ? P.v + uint64_t(b) * P.v_seq + uint64_t(h) * P.v_head : P.k + uint64_t(b) * P.k_seq + uint64_t(h) * P.k_head;
+                const uint64_t tok_bytes = v ? P.v_tok : P.k_tok;
+#pragma unroll 1
+                for (uint32_t i0 = 0; i0 < kIts; i0 += kBatch) {
+                    uint4 z[kBatch];
+                    const uint32_t key0 = (dt + i0 * 256) / kCh;
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const float2 two = at_unpack<BF16>(i == 0 ? z.x : i == 1 ? z.y : i == 2 ? z.z : z.w);
-                                f[2 * i] = two.x, f[2 * i + 1] = two.y;
-                                top = fmaxf(top, fmaxf(fabsf(two.x), fabsf(two.y)));
+                    for (uint32_t k = 0; k < kBatch; ++k) {
+                        const uint32_t key = key0 + k * (256 / kCh);
+                        z[k] = make_uint4(0, 0, 0, 0);
+                        if (tok0 + key < most) z[k] = __ldg(reinterpret_cast<const uint4*>(head + uint64_t(tok0 + key) * tok_bytes) + c);
+                    }
+#pragma unroll
+                    for (uint32_t k = 0; k < kBatch; ++k) {
+                        const uint32_t key = key0 + k * (256 / kCh);
+                        if constexpr (BF16) {
+                            wild = wild || ac_over_half2(z[k].x) || ac_over_half2(z[k].y) || ac_over_half2(z[k].z) || ac_over_half2(z[k].w);
+                            if (!v) {  // K rows as fp16, divided by a power of two as the query rows are
+                                constexpr uint32_t kAbs = 0x7FFF7FFFu;
+                                uint32_t m = __vmaxu2(__vmaxu2(z[k].x & kAbs, z[k].y & kAbs), __vmaxu2(z[k].z & kAbs, z[k].w & kAbs));
+#pragma unroll
+                                for (uint32_t o = kCh / 2; o; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+                                const int ex = ac_row_exponent(__uint_as_float(max(m & 0xFFFFu, m >> 16) << 16));
+                                const float inv = __uint_as_float(uint32_t(127 - ex) << 23);
+                                auto scaled2 = [&](uint32_t w) {
+                                    const float2 f = at_unpack<BF16>(w);
+                                    return pf_pack2<false>(f.x * inv, f.y * inv);
+                                };
+                                z[k] = make_uint4(scaled2(z[k].x), scaled2(z[k].y), scaled2(z[k].z), scaled2(z[k].w));
+                                if (c == 0) key_scale[((t - max(tb, n_first)) % kAcScales) * 128 + key] = uint8_t(127 + ex);
                             }
-#pragma unroll
-                            for (uint32_t o = kCh / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                            const int ex = ac_row_exponent(top);
-                            const float inv = __uint_as_float(uint32_t(127 - ex) << 23);
-                            z = make_uint4(pf_pack2<false>(f[0] * inv, f[1] * inv), pf_pack2<false>(f[2] * inv, f[3] * inv),
-                                           pf_pack2<false>(f[4] * inv, f[5] * inv), pf_pack2<false>(f[6] * inv, f[7] * inv));
-                            if (c == 0) key_scale[((t - max(tb, n_first)) % kAcScales) * 128 + key] = uint8_t(127 + ex);
                         }
+                        *place(at, v, key, c) = z[k];
                     }
-                    *place(at, v, key, c) = z;
                 }
                 if (kTail16 && !v) {
                     __syncwarp();
