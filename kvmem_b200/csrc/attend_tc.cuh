@@ -32,15 +32,18 @@
 // Quantised pages (q8_0 / q4_0): eight more warps read the blocks as stored, decode them to
 // fp16 and write them where the copies would have put them. Beside them bf16 queries and keys of
 // the tail become fp16, each row after division by a power of two of its own; the tail's values
-// stay bf16 (a product of its own type on the same accumulator). The decoding bounds that form:
-// some 10,000 cycles per tile of head_dim 256 against 2,500 of products and softmax.
+// stay bf16 (a product of its own type on the same accumulator). A tile of head_dim 256 takes 5.3 us
+// of decoding against 1.3 of products and softmax; with four tiles per CTA that is 21 of the 47 us
+// below. The rest does not depend on the tiles: the CTA's start, the tail, and 34 chunks to be joined.
 //
-// Measured (device time, the joining pass included where keys are split):
+// Measured (device time at 1,965 MHz, the joining pass included where keys are split):
 //   1,024 rows, window 4,096 + 256 sinks, 24 / 4 heads, dim 256, bf16   142 us, 770 TFLOP/s
-//   16,381 rows, window 1,000 + 64 sinks, 32 / 8 heads, dim 128, fp16   400 us, 690 TFLOP/s
+//   16,381 rows, window 1,000 + 64 sinks, 32 / 8 heads, dim 128, fp16   398 us, 695 TFLOP/s
+//     (called for a second and more the GPU's 1,000 W hold it at 1,730 MHz: 447 us, 618 TFLOP/s)
 //   60 nodes, 8 lanes, 26 pages of 128, 40 / 8 heads, dim 128, bf16     77 us, 440 TFLOP/s
-//   1 node, 34 pages of 256, 24 / 4 heads, dim 256, fp16                24 us, 1.5 TB/s
-//   16 nodes, 66 pages of 256, q8_0 / q4_0, 24 / 4 heads, dim 256       53 us
+//   1 node, 34 pages of 256, 24 / 4 heads, dim 256, fp16                25 us, 1.5 TB/s
+//   16 nodes, 66 pages of 256, q8_0 / q4_0, 24 / 4 heads, dim 256       47 us (bf16), 40 us (fp16)
+//   1 node, the same pages                                              44 us (bf16), 37 us (fp16)
 // Every wait is bounded: on expiry the kernel records KVM_ERR_TIMEOUT, raises the
 // CTA's abort flag, lets copies and MMAs in flight finish and frees its TMEM.
 #pragma once

@@ -2371,7 +2371,9 @@ bool attend_tc_maps(const AttendParams& p, uint32_t head_dim, bool bf16, int mod
 
 // Key chunks of a launch: the split whose modelled time is least. A wave of CTAs takes
 // its tiles' time plus the start and end of a CTA; a split adds the joining pass over
-// its partial rows.
+// its partial rows. The model puts the splits in the order that was measured; as a time it
+// is too short (34 us where a call over quantised pages takes 47, 13 where one token over
+// 34 pages takes 25).
 uint32_t attend_splits(const kvm_ctx* c, uint64_t units, uint64_t slots, uint64_t tiles, double tile_us, double cta_us,
                        uint64_t rows, size_t row_bytes, uint32_t least) {
     uint32_t splits = least;
@@ -2414,10 +2416,15 @@ int attend_scratch(kvm_ctx* c, AttendParams& p, uint32_t head_dim, cudaStream_t 
 //   8 rows of 1,150 keys of pages, dim 128    9.8 / 11.1
 //   8 lanes, window of 4,224 keys, dim 128   30.4 / 32.3  -            65.5 / 37.6  -            116 / 43.0 (80)
 //   one lane, window of 1,027 keys, dim 256   9.1 / 13.4  -            -            19.4 / 13.9  21.3 / 14.9 (96)
-//   q8_0 / q4_0, one lane, 17,000 keys       66.4 / 45.3  -            104 / 47.4   -            169 / 51.2
-//   q8_0, 8 lanes, 3,400 keys, dim 128       91.4 / 71.5  111 / 72.3 (20)           144 / 75.9
+//   q8_0 / q4_0, one lane, 17,000 keys       66.7 / 43.6  -            104 / 44.8   -            168 / 46.5
+//   q8_0, 8 lanes, 3,400 keys, dim 128       91.6 / 72.2  112 / 72.9 (20)           144 / 75.3
+//   one token, one lane, 16-bit pages, keys    1,024        1,536        2,048        2,560        3,328        5,120
+//     8 / 8 heads, dim 64                     8.5 / 9.5    8.7 / 9.7    9.3 / 10.7   9.5 / 11.4  10.0 / 11.5  12.1 / 13.6
+//     40 / 8 heads, dim 128                  10.1 / 11.1  10.3 / 11.3  11.1 / 12.5  13.9 / 13.4  13.6 / 13.6  15.5 / 16.9
+//     24 / 4 heads, dim 256                  12.1 / 15.3  12.3 / 15.9  12.8 / 15.9  16.5 / 15.4  16.4 / 16.5  19.0 / 20.6
 // (up to 16 rows one warp of the mma.sync kernel holds them all, and its CTAs start and end sooner;
-// its copies of pages cost a lookup per row, those of the tcgen05 kernel one per box).
+// its copies of pages cost a lookup per row, those of the tcgen05 kernel one per box). The bound of 2,048 keys
+// suits many lanes and long lists; one lane alone loses up to 3 us behind it, up to some 5,000 keys.
 // KVM_ATTEND=mma and KVM_ATTEND=tc force a kernel (tc: KVM_ERR_UNSUPPORTED where it
 // cannot run); the tests use them.
 int attend_launch(kvm_ctx* c, AttendParams& p, uint32_t head_dim, bool bf16, int mode, bool quant, uint64_t keys,
